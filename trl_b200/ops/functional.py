@@ -159,3 +159,63 @@ def load_balancing_loss(router_probs, topk_idx, num_experts, top_k, token_mask=N
     if router_probs.is_cuda and num_experts <= 1024:
         return _cuda().moe_aux_loss(router_probs, topk_idx, num_experts, token_mask)
     return _ref.load_balancing_loss(router_probs, topk_idx, num_experts, top_k, token_mask)
+
+
+# ---- 8-bit paged cache and filtered sampling: the decode step of the rollout engine --------------------------------
+def kv8_alloc(num_blocks, kv_heads, block_size, head_dim, device=None):
+    """An 8-bit paged cache: ``(k_cache, v_cache, k_scale, v_scale)``.  The codes are e4m3 [blocks, heads, block size, head
+    dim]; an entry stands for its code times the scale [blocks, heads] of its page and head, a power of two."""
+    if block_size < 16 or block_size & (block_size - 1) or head_dim not in (64, 96, 128, 256):
+        raise ValueError(f"page sizes are powers of two from 16 on and head dims 64, 96, 128 or 256, not {block_size} and {head_dim}")
+    codes = [torch.zeros(num_blocks, kv_heads, block_size, head_dim, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+             for _ in range(2)]
+    return (*codes, *[torch.ones(num_blocks, kv_heads, dtype=torch.float32, device=device) for _ in range(2)])
+
+
+def kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, starts, cu_seqlens=None, slots=None, max_new=None):
+    """Appends the keys and values [T, heads, head dim] (bf16, fp16, fp32) of new tokens to an 8-bit cache, in place.
+
+    Sequence i has the tokens ``cu_seqlens[i] .. cu_seqlens[i + 1]`` (without ``cu_seqlens``: token i), which go to the
+    positions from ``starts[i]`` on of the pages in row ``slots[i]`` (without ``slots``: i) of ``block_table`` [rows, blocks];
+    a negative start skips it.  ``max_new``: a bound of the tokens per sequence, which sizes the launch (default T); tokens
+    beyond it may be left out.  All index tensors are int32.
+
+    With a the largest magnitude of the new tokens in a page and head, the scale there becomes the smallest power of two (at
+    least 2^-100) that brings a within 448, or stays where earlier tokens of the page have a larger one; those are brought to
+    the new scale.  A page whose first row is written forgets its scale.  Infinities and NaN are held as NaN.  No two sequences
+    of a call may write one page.  Pages that the table does not have are reported by ``check_status`` and left out."""
+    args = (k, v, k_cache, v_cache, k_scale, v_scale, block_table, starts)
+    if k.is_cuda:
+        return _cuda().kv8_append(*args, cu_seqlens=cu_seqlens, slots=slots, max_new=max_new)
+    return _ref.kv8_append(*args, cu_seqlens, slots)
+
+
+def kv8_decode_attn(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, scale, slots=None, window=None, out=None):
+    """Attention of one new token per sequence, ``q`` [B, heads, head dim] (bf16 or fp16), over an 8-bit cache.
+
+    Sequence i sees the positions up to ``seq_lens[slot]`` (its newest token, which has been appended) in row ``slots[i]``
+    (default: i) of ``block_table``, with ``window`` only the last so many of them; ``seq_lens`` below 0: none, and zeros come
+    back.  Query heads share key heads in equal groups.  ``out``: a dense tensor like ``q`` to write to."""
+    args = (q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, scale)
+    if q.is_cuda:
+        return _cuda().kv8_decode_attn(*args, slots=slots, window=window, out=out)
+    r = _ref.kv8_decode_attn(*args, slots, window)
+    return r if out is None else out.copy_(r)
+
+
+def sample_filtered(logits, rng, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """Draws one token per row of ``logits`` [B, V] (bf16, fp16, fp32) from given random numbers: ``(tokens int32 [B],
+    log-probabilities fp32 [B])``.
+
+    ``rng`` [B] int32 (or int64, of which the low 32 bits count) holds a random word per row, from which each column's uniform
+    number is hashed: a row's draw depends on its word and its logits alone.  ``temperature``, ``top_k``, ``top_p`` and
+    ``min_p`` are numbers or tensors [B].
+
+    With z = logits / temperature: top-k keeps what is at least the k-th largest z (0: all); top-p keeps, most likely first
+    and the lower token first among equals, each token before which at most ``top_p`` of the mass left by top-k stands (1:
+    all); min-p keeps what has at least ``min_p`` (up to 1) of the largest probability.  Temperature 0 takes the most likely
+    token, the lowest among equals.  The log-probability is that in the distribution over what is kept.  NaN counts as -inf;
+    a row without a finite logit gives token 0 and -inf."""
+    if logits.is_cuda:
+        return _cuda().sample_filtered(logits, rng, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+    return _ref.sample_filtered(logits, rng, temperature, top_k, top_p, min_p)

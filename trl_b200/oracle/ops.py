@@ -249,3 +249,100 @@ def dpo_sigmoid_loss(pol_c, pol_r, ref_c, ref_r, beta, label_smoothing=0.0):
     d = (pol_c - ref_c) - (pol_r - ref_r)
     loss = -F.logsigmoid(beta * d) * (1 - label_smoothing) - F.logsigmoid(-beta * d) * label_smoothing
     return loss, beta * (pol_c - ref_c), beta * (pol_r - ref_r)
+
+
+# ---- 8-bit paged cache and filtered sampling ------------------------------------------------------------------------
+def kv8_scale(amax: torch.Tensor) -> torch.Tensor:
+    """The smallest power of two, from 2^-100 to 2^120, that brings ``amax`` within 448 (the largest e4m3 number)."""
+    frac, exp = torch.frexp(amax.double() / 448.0)
+    exp = torch.where(frac > 0.5, exp, exp - 1).clamp(-100, 120)
+    return torch.ldexp(torch.ones_like(frac), torch.where(amax > 0, exp, torch.full_like(exp, -100))).float()
+
+
+def kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, starts, cu_seqlens=None, slots=None):
+    """New tokens into an 8-bit paged cache, sequence by sequence and page by page (see ``ops.functional.kv8_append``)."""
+    page = k_cache.shape[2]
+    cu = list(range(starts.shape[0] + 1)) if cu_seqlens is None else cu_seqlens.tolist()
+    for i, start in enumerate(starts.tolist()):
+        if start < 0:
+            continue
+        row = block_table[i if slots is None else int(slots[i])].tolist()
+        at, n = 0, cu[i + 1] - cu[i]
+        while at < n:
+            first = (start + at) % page
+            take, blk = min(page - first, n - at), row[(start + at) // page]
+            for x, codes, scale in ((k, k_cache, k_scale), (v, v_cache, v_scale)):
+                new = x[cu[i] + at:cu[i] + at + take].float().transpose(0, 1)  # [heads, take, dim]
+                new = torch.where(torch.isfinite(new), new, float("nan"))
+                now = kv8_scale(torch.nan_to_num(new.abs(), nan=0.0).amax((1, 2)))
+                if first:
+                    was = scale[blk].clone()
+                    now = torch.maximum(was, now)
+                    codes[blk, :, :first] = (codes[blk, :, :first].float() * (was / now)[:, None, None]).to(codes.dtype)
+                codes[blk, :, first:first + take] = (new / now[:, None, None]).to(codes.dtype)
+                scale[blk] = now
+            at += take
+
+
+def kv8_gather(codes, scale, blocks, lo, hi):
+    """Positions ``lo .. hi`` of the sequence whose pages are ``blocks``: fp32 [heads, hi - lo, dim]."""
+    x = codes[blocks].float() * scale[blocks][:, :, None, None]
+    return x.transpose(0, 1).reshape(codes.shape[1], -1, codes.shape[3])[:, lo:hi]
+
+
+def kv8_decode_attn(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, scale, slots=None, window=None):
+    B, Hq, D = q.shape
+    heads, page = k_cache.shape[1:3]
+    out = torch.zeros_like(q)
+    for i in range(B):
+        slot = i if slots is None else int(slots[i])
+        n = int(seq_lens[slot]) + 1
+        if n <= 0:
+            continue
+        lo = max(0, n - window) if window else 0
+        blocks = block_table[slot, :-(-n // page)].long()
+        kk, vv = kv8_gather(k_cache, k_scale, blocks, lo, n), kv8_gather(v_cache, v_scale, blocks, lo, n)
+        s = torch.einsum("hgd,htd->hgt", q[i].float().view(heads, -1, D), kk) * scale
+        out[i] = torch.einsum("hgt,htd->hgd", torch.softmax(s, -1), vv).reshape(Hq, D).to(q.dtype)
+    return out
+
+
+def _hash_u32(x: torch.Tensor) -> torch.Tensor:
+    x = x ^ (x >> 16)
+    x = (x * 0x7FEB352D) & 0xFFFFFFFF
+    x = x ^ (x >> 15)
+    x = (x * 0x846CA68B) & 0xFFFFFFFF
+    return x ^ (x >> 16)
+
+
+def row_uniforms(rng: torch.Tensor, vocab: int) -> torch.Tensor:
+    """The uniform numbers in (0, 1), fp64 [B, vocab], that the rows' random words stand for."""
+    col = torch.arange(vocab, device=rng.device)
+    h = _hash_u32((rng.long() & 0xFFFFFFFF)[:, None] ^ _hash_u32((col * 0x85EBCA6B + 0x165667B1) & 0xFFFFFFFF))
+    return (_hash_u32((h + col) & 0xFFFFFFFF).double() + 0.5) / 2.0**32
+
+
+def sample_filtered(logits, rng, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """Row by row, sums in fp64 (see ``ops.functional.sample_filtered``)."""
+    B, V = logits.shape
+    per = lambda x, i: x[i].item() if torch.is_tensor(x) else x  # noqa: E731
+    u = row_uniforms(rng, V)
+    toks, logps = torch.zeros(B, dtype=torch.int32), torch.full((B,), float("-inf"))
+    for i in range(B):
+        t, k, p, m = per(temperature, i), int(per(top_k, i)), per(top_p, i), per(min_p, i)
+        z = logits[i].float() / torch.tensor(t, dtype=torch.float32).clamp_min(1e-6)
+        z = torch.nan_to_num(z, nan=float("-inf"), posinf=torch.finfo(torch.float32).max, neginf=float("-inf")).double()
+        if z.max() == float("-inf"):
+            continue
+        zs, order = torch.sort(z, descending=True, stable=True)
+        keep = (zs >= zs[k - 1] if 0 < k < V else torch.ones(V, dtype=torch.bool)) & (zs > float("-inf"))
+        w = torch.where(keep, torch.exp(zs - zs[0]), 0.0)
+        if p < 1:
+            keep &= w.cumsum(0) - w <= max(p, 0.0) * w.sum()
+        if m > 0:
+            keep &= zs >= zs[0] + math.log(min(m, 1.0))
+        kept = order[keep]
+        key = z[kept] if not t > 0 else z[kept] - torch.log(-torch.log(u[i, kept]))
+        toks[i] = int(kept[key == key.max()].min())
+        logps[i] = float(z[toks[i]] - zs[0] - torch.logsumexp(z[kept] - zs[0], 0))
+    return toks.to(logits.device), logps.to(logits.device)
