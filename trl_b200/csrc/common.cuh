@@ -307,6 +307,9 @@ int make_tmap_2d_bf16(CUtensorMap* out, const void* base, uint64_t rows, uint64_
 // 3D bf16 map: dims (d0 innermost, d1, d2), strides in elements for d1 and d2, box (b0, b1, b2), 128-byte swizzle.
 int make_tmap_3d_bf16(CUtensorMap* out, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t stride1_elems,
                       uint64_t stride2_elems, uint32_t b0, uint32_t b1, uint32_t b2);
+// Dense 3D map of bytes: dims (d0 innermost, d1, d2), box (b0, b1, 1), swizzled over 128 or 64 bytes or (0) not.
+int make_tmap_3d_u8(CUtensorMap* out, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint32_t b0, uint32_t b1,
+                    int swizzle_bytes);
 int sm_count();
 // Process-wide switch for programmatic dependent launch of the decode-path kernels (trlb_set_pdl).
 bool pdl_enabled();

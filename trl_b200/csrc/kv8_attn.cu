@@ -4,24 +4,26 @@
 //
 // Bound by the cache's bytes: 2 D bytes a token and key head for 4 G D operations (G query heads share a key head).
 //
-// A warp takes 16 tokens a step.  Their codes go from memory straight into registers in the order that the matrix
-// instruction wants its operands (16 x 8 x 16, fp16 in, fp32 sums): nothing of the cache passes through shared memory and no
-// warp waits for another one until the sums are joined.
-//   S = Q K^T   A = Q (heads as rows), B = K: the lane (g, t) holds quarter t of token g's row.  Which dimension stands at
-//               which place of the sum is free, so a lane's dimensions are whatever its loads bring.
-//   O^T = V^T P^T   A = V^T, B = P: the probabilities are already where the B operand wants them (tokens 2t, 2t + 1 of head g),
-//               and the lane (g, t) holds dimensions of unit g for the tokens 2t, 2t + 1, 2t + 8, 2t + 9, whose bytes are
-//               interleaved in pairs.
-// Codes become fp16 exactly.  Queries are brought within fp16 by a power of two per row (exact for bf16 and fp16 but for
-// values 2^24 below the row's largest).
+// A warp takes 16 tokens a step.  Each warp has a queue of steps in shared memory that its first lane keeps filled by TMA, a few
+// steps ahead; no warp waits for another one, so rows of any length run side by side.  A lane reads its codes from the
+// (swizzled, so free of bank conflicts at head dims 128 and 256) tile in the order that the matrix instruction (16 x 8 x 16,
+// fp16 in, fp32 sums) wants its operands, and makes fp16 of them, exactly.
+//   S = Q K^T   A = Q (heads as rows), B = K: the lane (g, t) holds quarter t of token g's row.  Which dimension stands at which
+//               place of the sum is free, so a lane's dimensions are whatever its loads bring.
+//   O^T = V^T P^T   A = V^T, B = P: the probabilities are already where the B operand wants them (the 2t-th and 2t+1-th token of
+//               head g), and the lane (g, t) holds dimensions of unit g for those tokens, whose bytes are interleaved in pairs.
+// Queries are brought within fp16 by a power of two per row (exact for bf16 and fp16 but for values 2^24 below the row's
+// largest).
 //
 // Page scales.  k_scale multiplies the scores.  v_scale goes into the exponent: w_j = exp2(s_j + log2 v_scale - m) with m the
 // running maximum of that sum, so that weights stay within fp16 whatever the pages' scales, and the softmax's denominator is
 // sum w_j / v_scale.  m moves only when a weight would pass 2^8.
 //
-// Work: the steps of all (sequence, key head, head tile) are one list that is dealt to the blocks in equal runs, so any mix
-// of lengths fills the GPU.  A block whose run covers all steps of a row writes its output; else it leaves its (m, l, o) for
-// kv8_attn_join_kernel, which adds a row's parts in the order of the blocks.  No atomics: results do not depend on timing.
+// Work: the steps of all rows (sequence, key head, head tile) are one list that is dealt to the warps in equal runs, so any mix
+// of lengths fills the GPU; a row counts KA_ROW steps more than it has, the cost of beginning one.  A warp that has all steps of
+// a row writes its output.  Else it leaves (m, l, o); where all of a block's runs lie in one row, the block joins its warps'
+// first and leaves one.  The warp that has a row's first step says which row it is, for kv8_attn_join_kernel, which adds a
+// row's parts in the order of the warps.  No atomics: results do not depend on timing.
 #include <cuda_fp16.h>
 
 #include "kv8.cuh"
@@ -32,11 +34,16 @@ enum { SITE_KV8_ATTN = 1410 };
 
 constexpr int KA_WARPS = 4, KA_THREADS = KA_WARPS * 32;
 constexpr int KA_STEP = 16;          // tokens of a warp's step
+constexpr int KA_ROW = 2;            // steps that a row's beginning is worth
+constexpr int KA_JOIN = 512;         // threads of a joining block
 constexpr int KA_MAX_SEQS = 8192;    // the prefix sums of their steps stand in shared memory
 constexpr float KA_NONE = -1e30f;    // maximum of no token: finite, so that exp2(-inf - m) is 0
 
-// Blocks an SM holds: what the registers of a thread (codes of two steps, queries, sums) leave room for.
-__host__ __device__ constexpr int kv8_attn_per_sm(int D, int HT) { return D * HT > 128 * 8 ? 2 : 3; }
+// Steps in a warp's queue and blocks an SM holds: about 190 KB of codes under way on an SM, as registers allow.
+__host__ __device__ constexpr int kv8_attn_stages(int D) { return D == 256 ? 3 : 4; }
+__host__ __device__ constexpr int kv8_attn_per_sm(int D, int HT) { return D == 256 ? 2 : 3; }
+// Swizzle of a row's bytes in shared memory; 96 bytes stand as they are.
+__host__ __device__ constexpr int kv8_attn_swizzle(int D) { return D % 128 == 0 ? 128 : (D == 64 ? 64 : 0); }
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
@@ -59,27 +66,44 @@ __device__ __forceinline__ float2 unpack2<__half>(uint32_t u) { return __half22f
 __device__ __forceinline__ void store1(__nv_bfloat16* p, float x) { *p = __float2bfloat16(x); }
 __device__ __forceinline__ void store1(__half* p, float x) { *p = __float2half(x); }
 
-// Bytes that are read once: past the first-level cache.
 template <int BYTES>
-__device__ __forceinline__ void load_codes(uint32_t* w, const uint8_t* p) {
-  if constexpr (BYTES == 16) {
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
-  } else if constexpr (BYTES == 8) {
-    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
-  } else {
-    asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(w[0]) : "l"(p));
-  }
+__device__ __forceinline__ void read_codes(uint32_t* w, uint32_t src) {
+  if constexpr (BYTES == 16) asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(src) : "memory");
+  else if constexpr (BYTES == 8) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(src) : "memory");
+  else asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(src) : "memory");
 }
+// Address of byte x of row r in a tile of 16 rows of D bytes as TMA leaves it.
+template <int D>
+__device__ __forceinline__ uint32_t tile_at(int r, int x) {
+  if constexpr (D % 128 == 0) return (x >> 7) * 2048 + r * 128 + ((x & 127) ^ ((r & 7) << 4));
+  else if constexpr (D == 64) return r * 64 + (x ^ (((r >> 1) & 3) << 4));
+  else return r * D + x;
+}
+// The token of a step at place c of eight: an order in which lanes that read together read different banks.
+template <int D>
+__device__ __forceinline__ int place(int c) { return D % 128 == 0 ? (c >> 1) | ((c & 1) << 2) : c; }
+
+__device__ __forceinline__ uint32_t pack_out(float a, float b, __nv_bfloat16) { return pack_bf16(a, b); }
+__device__ __forceinline__ uint32_t pack_out(float a, float b, __half) { return pack_f16(a, b); }
+
+struct SharedRow {
+  int seq, head, heads;  // seq < 0: none
+  int last;              // warp of the last step
+  int joined0, joined1;  // blocks whose warps' parts are one, at the first warp's place
+  int pad[2];
+};
 
 struct Kv8AttnArgs {
+  CUtensorMap k, v;  // codes as [pages * heads][page size][D], boxes of 16 rows
   const void* q;
   long long q_row, q_head;
-  const uint8_t *k, *v;
   const float *k_scale, *v_scale;
   const int *table, *seq_lens, *slots;
   void* out;
-  float* part;  // [2 * blocks][HT][D + 2]
-  int *status;
+  float* part;      // [2 * warps][HT][D]: sums of the row that began before a warp's run, of the row that ends behind it
+  float2* part_ml;  // [2 * warps][HT]: their maxima and denominators
+  SharedRow* rows;  // [warps]: the row whose first step is in a warp's run and whose last is not
+  int* status;
   int pages, Hk, G, tiles, page_shift, table_rows, max_blocks, B, window, min_run;
   float scale;
 };
@@ -102,12 +126,16 @@ __device__ __forceinline__ int kv8_steps(const Kv8AttnArgs& a, int b, int& lo, i
   return (hi + KA_STEP - 1) / KA_STEP - lo / KA_STEP;
 }
 
-// prefix[b] = steps of the sequences before b, prefix[B] = of all
+// prefix[b] = cost of one row of each of the sequences before b, prefix[B] = of all
 __device__ __forceinline__ void kv8_prefix(const Kv8AttnArgs& a, int* prefix, int* warp_sums) {
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   const int per = (a.B + KA_THREADS - 1) / KA_THREADS;
   int sum = 0, lo, hi;
-  for (int i = tid * per; i < min(a.B, (tid + 1) * per); ++i) sum += kv8_steps(a, i, lo, hi);
+  auto cost = [&](int i) {
+    const int n = kv8_steps(a, i, lo, hi);
+    return n > 0 ? n + KA_ROW : 0;
+  };
+  for (int i = tid * per; i < min(a.B, (tid + 1) * per); ++i) sum += cost(i);
   int run = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -120,120 +148,174 @@ __device__ __forceinline__ void kv8_prefix(const Kv8AttnArgs& a, int* prefix, in
   for (int w = 0; w < wid; ++w) before += warp_sums[w];
   for (int i = tid * per; i < min(a.B, (tid + 1) * per); ++i) {
     prefix[i] = before;
-    before += kv8_steps(a, i, lo, hi);
+    before += cost(i);
   }
   if (tid == KA_THREADS - 1) prefix[a.B] = before;
   __syncthreads();
-}
-// Steps a block takes: all of them in equal runs, but no run so short that its warps would have less than a step.
-__device__ __forceinline__ long long kv8_run(const Kv8AttnArgs& a, long long total, int blocks) {
-  const long long even = (total + blocks - 1) / blocks;
-  return even > a.min_run ? even : a.min_run;
 }
 
 template <int D, int HT, typename T>
 __global__ void __launch_bounds__(KA_THREADS, kv8_attn_per_sm(D, HT))
 kv8_attn_kernel(const __grid_constant__ Kv8AttnArgs a) {
-  constexpr int KU = D % 64 == 0 ? 16 : 8, KN = D / (4 * KU);                         // K: units of a lane's loads, loads a row
+  constexpr int KU = D % 64 == 0 ? 16 : 8, KN = D / (4 * KU);                         // K: bytes of a lane's unit, units a row
   constexpr int VU = D % 128 == 0 ? 16 : (D % 64 == 0 ? 8 : 4), VN = D / (8 * VU);    // V: the same
   constexpr int KW = D / 16, VW = D / 32;                                             // words of a row in a lane
-  constexpr int NT = HT / 8;
-  extern __shared__ __align__(16) float smem[];
-  float* sh_o = smem;                                  // [warps][HT][D]
-  float* sh_m = sh_o + KA_WARPS * HT * D;              // [warps][HT]
-  float* sh_l = sh_m + KA_WARPS * HT;
-  int* prefix = reinterpret_cast<int*>(sh_l + KA_WARPS * HT);  // [B + 1]
+  constexpr int NT = HT / 8, S = kv8_attn_stages(D), STAGE = 32 * D, BOX = D % 128 == 0 ? 128 : D;
+  extern __shared__ uint8_t smem_raw[];  // [warps][S][K tile, V tile] on 1024 bytes, then prefix [B + 1]
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  int* prefix = reinterpret_cast<int*>(smem + KA_WARPS * S * STAGE);
+  __shared__ uint64_t full[KA_WARPS][S];
+  __shared__ int abort_flag;
+  __shared__ float2 sh_ml[KA_WARPS][HT];
+  __shared__ int4 sh_row;
   __shared__ int warp_sums[KA_WARPS];
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, t = lane & 3;
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < S; ++i) mbar_init(&full[wid][i], 1);
+    mbar_fence_init();
+    if (wid == 0) {
+      abort_flag = 0;
+      tma_prefetch_desc(&a.k);
+      tma_prefetch_desc(&a.v);
+    }
+  }
   pdl_launch_dependents();
   pdl_wait();
-  kv8_prefix(a, prefix, warp_sums);
-  const int rows_per_seq = a.Hk * a.tiles;
-  const long long total = (long long)prefix[a.B] * rows_per_seq, run = kv8_run(a, total, gridDim.x);
-  // rows without a token to see have no steps: their zeros are written here
+  kv8_prefix(a, prefix, warp_sums);  // its barriers show the mbarriers, too
+  // sequences without a token to see have no steps: their zeros are written here
   for (int b = blockIdx.x; b < a.B; b += gridDim.x)
     if (prefix[b + 1] == prefix[b])
       for (int i = tid; i < a.Hk * a.G * D; i += KA_THREADS)
         store1(reinterpret_cast<T*>(a.out) + (size_t)b * a.Hk * a.G * D + i, 0.f);
-  long long u = (long long)blockIdx.x * run;
-  const long long u1 = min(total, u + run);
-  const long long first = u;
+  const int rows_per_seq = a.Hk * a.tiles, warp = blockIdx.x * KA_WARPS + wid;
+  const long long total = (long long)prefix[a.B] * rows_per_seq, warps = (long long)gridDim.x * KA_WARPS;
+  const long long run = max((long long)a.min_run, (total + warps - 1) / warps);
+  const long long u0 = (long long)warp * run, u1 = min(total, u0 + run);
+  const long long block0 = (long long)blockIdx.x * KA_WARPS * run, block1 = min(total, block0 + KA_WARPS * run);
+  SharedRow shared = {-1, 0, 0, 0, 0, 0, {0, 0}};
   int b = 0;
-  if (u < u1) {  // the sequence that step u belongs to
-    int lo = 0, hi = a.B - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if ((long long)prefix[mid] * rows_per_seq <= u) lo = mid; else hi = mid - 1;
+  bool joined = false;  // all of the block's runs lie in one row
+  if (block0 < block1) {  // the sequence that the block begins in
+    int hi = a.B - 1;
+    while (b < hi) {
+      const int mid = (b + hi + 1) >> 1;
+      if ((long long)prefix[mid] * rows_per_seq <= block0) b = mid; else hi = mid - 1;
     }
-    b = lo;
-    // sequences without steps share their prefix with the next one: the last of equals is the one with steps
+    const int cost = prefix[b + 1] - prefix[b];
+    const long long seq0 = (long long)prefix[b] * rows_per_seq;
+    joined = seq0 + ((block0 - seq0) / cost + 1) * cost >= block1;
   }
-  while (u < u1) {
+  if (lane < HT) sh_ml[wid][lane] = make_float2(KA_NONE, 0.f);
+  uint8_t* queue = smem + wid * S * STAGE;
+  int slot_in = 0, slot_out = 0;
+  uint32_t parity = 0;
+  // of the block's row, where its warps join
+  int join_seq = 0, join_head = 0, join_heads = 0;
+  bool join_whole = false;
+  size_t join_part = 0;
+  for (long long u = u0; u < u1;) {
     while (prefix[b + 1] == prefix[b] || (long long)prefix[b + 1] * rows_per_seq <= u) ++b;
-    int tok_lo, tok_hi;
-    const int steps = kv8_steps(a, b, tok_lo, tok_hi);
-    const long long seq_u = u - (long long)prefix[b] * rows_per_seq;
-    const int row = (int)(seq_u / steps), s0 = (int)(seq_u % steps);
-    const int s1 = (int)min((long long)steps, s0 + (u1 - u));
+    const int cost = prefix[b + 1] - prefix[b], steps = cost - KA_ROW;
+    const long long seq0 = (long long)prefix[b] * rows_per_seq;
+    const int row = (int)((u - seq0) / cost);
+    const long long row0 = seq0 + (long long)row * cost;  // its beginning counts first, then its steps
+    const int s0 = (int)max(0ll, u - row0 - KA_ROW), s1 = (int)min((long long)steps, u1 - row0 - KA_ROW);
     const int kvh = row / a.tiles, h0 = (row % a.tiles) * HT, heads = min(HT, a.G - h0);
+    const bool begins = joined ? block0 - row0 <= KA_ROW : s0 == 0;  // the row's first step is in the run (of the block)
+    const bool whole = begins && row0 + cost <= (joined ? block1 : u1);
+    if (begins && !whole && (joined ? wid == 0 : s1 > 0)) {
+      const long long per = KA_WARPS * run;
+      // blocks that lie in the row; the list's last one may be shorter than the others
+      const long long end = row0 + cost >= total ? total + per - 1 : row0 + cost;
+      shared = {b, kvh * a.G + h0, heads, (int)((row0 + cost - 1) / run), (int)((row0 + per - 1) / per), (int)(end / per), {0, 0}};
+    }
+    join_seq = b;
+    join_head = kvh * a.G + h0;
+    join_heads = heads;
+    join_whole = whole;
+    join_part = (size_t)2 * blockIdx.x * KA_WARPS + (begins ? 1 : 0);
+    u = row0 + cost;
+    if (s1 <= s0) continue;  // no more of it than its beginning
+    int tok_lo, tok_hi;
+    kv8_steps(a, b, tok_lo, tok_hi);
     const int slot = a.slots ? a.slots[b] : b;
     const int base = tok_lo / KA_STEP;  // step s covers the tokens (base + s) * 16 ...
     const int* table = a.table + (size_t)slot * a.max_blocks;
+    const int per_page = a.page_shift - 4;  // log2 of the steps of a page
+    const int page_first = (base + s0) >> per_page, page_last = (base + s1 - 1) >> per_page;
 
-    uint32_t kw[2][2 * KW], vw[2][4 * VW];
-    float ks[2], vs[2];
-    const int page_mask = (1 << a.page_shift) - 1;
-    auto page_of = [&](int s) {
-      return table[((base + s) * KA_STEP) >> a.page_shift];
-    };
-    auto load = [&](int s, int blk, uint32_t* k, uint32_t* v, float& kscale, float& vscale) {
-      if (blk < 0 || blk >= a.pages) {  // not a page of the cache: no token of the step counts
-        report_error(a.status, ERR_BOUNDS, SITE_KV8_ATTN, blk);
-        vscale = 0.f;
-        kscale = 0.f;
-#pragma unroll
-        for (int i = 0; i < 2 * KW; ++i) k[i] = 0;
-#pragma unroll
-        for (int i = 0; i < 4 * VW; ++i) v[i] = 0;
-        return;
+    // Pages, 32 at a time, one a lane: those that loads are taken from and the ones behind them, and the scales of those that
+    // are computed with and of the ones behind them.
+    auto pages_from = [&](int first) {
+      int blk = -1;
+      if (first + lane <= page_last) {
+        blk = table[first + lane];
+        if (blk < 0 || blk >= a.pages) {  // not a page of the cache: its tokens count for nothing
+          report_error(a.status, ERR_BOUNDS, SITE_KV8_ATTN, blk);
+          blk = -1;
+        }
       }
-      const size_t tile = (size_t)blk * a.Hk + kvh;
-      const size_t at = ((tile << a.page_shift) + (((base + s) * KA_STEP) & page_mask)) * D;
-      const uint8_t* kp = a.k + at + (size_t)g * D + t * KU;
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int j = 0; j < KN; ++j) load_codes<KU>(k + r * KW + j * (KU / 4), kp + r * 8 * D + j * 4 * KU);
-      const uint8_t* vp = a.v + at + (size_t)(2 * t) * D + g * VU;
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int j = 0; j < VN; ++j) load_codes<VU>(v + r * VW + j * (VU / 4), vp + ((r >> 1) * 8 + (r & 1)) * D + j * 8 * VU);
-      kscale = a.k_scale[tile];
-      vscale = a.v_scale[tile];
+      return blk;
     };
+    auto scales_of = [&](int blk, float& k, float& v) {
+      k = v = 0.f;
+      if (blk >= 0) {
+        k = a.k_scale[(size_t)blk * a.Hk + kvh];
+        v = a.v_scale[(size_t)blk * a.Hk + kvh];
+      }
+    };
+    int load_from = page_first, pages = pages_from(page_first), pages_next = page_last - page_first >= 32 ? pages_from(page_first + 32) : -1;
+    float ks, vs, ks_next = 0.f, vs_next = 0.f;
+    int scale_from = page_first;
+    scales_of(pages, ks, vs);
+    int next = s0;
+    auto copy = [&]() {  // the codes of step `next` into the queue
+      if (next >= s1) return;
+      const int page = (base + next) >> per_page;
+      if (page - load_from >= 32) {
+        load_from += 32;
+        pages = pages_next;
+        scales_of(pages, ks_next, vs_next);
+        pages_next = pages_from(load_from + 32);
+      }
+      const int blk = __shfl_sync(0xffffffffu, pages, page - load_from);  // every lane is here: the slot has been read
+      if (lane == 0) {
+        uint64_t* bar = &full[wid][slot_in];
+        if (blk < 0) {
+          mbar_arrive(bar);  // nothing to read; the step has no weight
+        } else {
+          uint8_t* dst = queue + slot_in * STAGE;
+          const int y = ((base + next) & ((1 << per_page) - 1)) << 4, z = blk * a.Hk + kvh;
+          mbar_expect_tx(bar, STAGE);
+#pragma unroll
+          for (int i = 0; i < D / BOX; ++i) {
+            tma_load_3d(dst + i * 16 * BOX, &a.k, bar, i * BOX, y, z);
+            tma_load_3d(dst + 16 * D + i * 16 * BOX, &a.v, bar, i * BOX, y, z);
+          }
+        }
+      }
+      ++next;
+      slot_in = slot_in + 1 == S ? 0 : slot_in + 1;
+    };
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) copy();
 
-    int s = s0 + wid;
-    int blk_next = 0;
-    if (s < s1) {
-      const int blk = page_of(s);
-      if (s + KA_WARPS < s1) blk_next = page_of(s + KA_WARPS);
-      load(s, blk, kw[0], vw[0], ks[0], vs[0]);
-    }
-    // queries of this row tile: rows g (and g + 8) as A operands, brought to at most 2 in magnitude
+    // Queries of this row: heads g (and g + 8) as A operands, brought to at most 2 in magnitude.
     uint32_t qa[KW][2 * NT];
     float cq[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int h = g + 8 * n;
       const T* qp = reinterpret_cast<const T*>(a.q) + (long long)b * a.q_row + (long long)(kvh * a.G + h0 + h) * a.q_head;
-      uint2 raw[KW];
       float most = 0.f;
 #pragma unroll
       for (int w = 0; w < KW; ++w) {
         const int d = KU * (t + 4 * (w / (KU / 4))) + 4 * (w % (KU / 4));
-        raw[w] = h < heads ? *reinterpret_cast<const uint2*>(qp + d) : make_uint2(0, 0);
-        const float2 x = unpack2<T>(raw[w].x), y = unpack2<T>(raw[w].y);
+        const uint2 raw = h < heads ? *reinterpret_cast<const uint2*>(qp + d) : make_uint2(0, 0);
+        qa[w][2 * n] = raw.x;
+        qa[w][2 * n + 1] = raw.y;
+        const float2 x = unpack2<T>(raw.x), y = unpack2<T>(raw.y);
         most = fmaxf(fmaxf(most, fmaxf(kv8_magnitude(x.x), kv8_magnitude(x.y))), fmaxf(kv8_magnitude(y.x), kv8_magnitude(y.y)));
       }
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
@@ -242,11 +324,12 @@ kv8_attn_kernel(const __grid_constant__ Kv8AttnArgs a) {
       const float inv = kv8_pow2(-e);
       cq[n] = a.scale * 1.4426950408889634f * kv8_pow2(e);
 #pragma unroll
-      for (int w = 0; w < KW; ++w) {
-        const float2 x = unpack2<T>(raw[w].x), y = unpack2<T>(raw[w].y);
-        qa[w][2 * n] = pack_f16(x.x * inv, x.y * inv);
-        qa[w][2 * n + 1] = pack_f16(y.x * inv, y.y * inv);
-      }
+      for (int w = 0; w < KW; ++w)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float2 x = unpack2<T>(qa[w][2 * n + i]);
+          qa[w][2 * n + i] = pack_f16(x.x * inv, x.y * inv);
+        }
     }
     float m[NT], l[NT], o[2 * VW][NT][4];
 #pragma unroll
@@ -259,44 +342,70 @@ kv8_attn_kernel(const __grid_constant__ Kv8AttnArgs a) {
         for (int k = 0; k < 4; ++k) o[i][n][k] = 0.f;
     }
 
-    auto compute = [&](int step, const uint32_t* k, uint32_t* v, float kscale, float vscale) {
-      float sc[2][4];  // scores of the tokens 0-7 and 8-15: [head g: 2t, 2t + 1][head g + 8: 2t, 2t + 1]
+    int page_now = -1;
+    float kscale = 0.f, lv = 0.f, inv_v = 0.f;
+    for (int s = s0; s < s1; ++s) {
+      copy();
+      if (!mbar_wait(&full[wid][slot_out], parity, &abort_flag, a.status, SITE_KV8_ATTN)) break;
+      const uint32_t kq = smem_u32(queue) + slot_out * STAGE, vq = kq + 16 * D;
+      if (++slot_out == S) {
+        slot_out = 0;
+        parity ^= 1;
+      }
+      float sc[2][4];  // scores of the tokens 0-7 and 8-15: [head g: places 2t, 2t + 1][head g + 8: the same]
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
+        uint32_t k[KW];
+#pragma unroll
+        for (int j = 0; j < KN; ++j) read_codes<KU>(k + j * (KU / 4), kq + tile_at<D>(8 * r + place<D>(g), KU * (t + 4 * j)));
 #pragma unroll
         for (int i = 0; i < 4; ++i) sc[r][i] = 0.f;
 #pragma unroll
-        for (int w = 0; w < KW; ++w) {
-          const uint32_t b0 = kv8_decode2(k[r * KW + w]), b1 = kv8_decode2_hi(k[r * KW + w]);
-          mma_f16(sc[r], qa[w][0], NT == 2 ? qa[w][2 * (NT - 1)] : 0u, qa[w][1], NT == 2 ? qa[w][2 * (NT - 1) + 1] : 0u, b0, b1);
-        }
+        for (int w = 0; w < KW; ++w)
+          mma_f16(sc[r], qa[w][0], NT == 2 ? qa[w][2 * (NT - 1)] : 0u, qa[w][1], NT == 2 ? qa[w][2 * (NT - 1) + 1] : 0u,
+                  kv8_decode2(k[w]), kv8_decode2_hi(k[w]));
       }
-      const int tok = (base + step) * KA_STEP;
-      const bool edge = tok < tok_lo || tok + KA_STEP > tok_hi || vscale == 0.f;
+      uint32_t v[4 * VW];
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < VN; ++j)
+          read_codes<VU>(v + r * VW + j * (VU / 4), vq + tile_at<D>((r >> 1) * 8 + place<D>(2 * t + (r & 1)), VU * (place<D>(g) + 8 * j)));
+      const int page = (base + s) >> per_page;
+      if (page != page_now) {
+        page_now = page;
+        if (page - scale_from >= 32) {
+          scale_from += 32;
+          ks = ks_next;
+          vs = vs_next;
+        }
+        kscale = __shfl_sync(0xffffffffu, ks, page - scale_from);
+        const float vscale = __shfl_sync(0xffffffffu, vs, page - scale_from);
+        lv = __log2f(vscale);  // of a power of two; of 0, where no page is: -inf, no weight
+        inv_v = vscale > 0.f ? __frcp_rn(vscale) : 0.f;
+      }
+      const int tok = (base + s) * KA_STEP;
+      const bool edge = tok < tok_lo || tok + KA_STEP > tok_hi || inv_v == 0.f;
+      auto hidden = [&](int r) {
+        const int x = tok + (r >> 1) * 8 + place<D>(2 * t + (r & 1));
+        return x < tok_lo || x >= tok_hi || inv_v == 0.f;
+      };
       if (edge) {  // tokens out of sight: what stands there may be anything, NaN included
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int x = tok + (r >> 1) * 8 + 2 * t + (r & 1);
-          if (x < tok_lo || x >= tok_hi || vscale == 0.f) {
-            sc[r >> 1][r & 1] = -INFINITY;
-            sc[r >> 1][2 + (r & 1)] = -INFINITY;
+        for (int r = 0; r < 4; ++r)
+          if (hidden(r))
 #pragma unroll
             for (int i = 0; i < VW; ++i) v[r * VW + i] = 0;
-          }
-        }
       }
-      const float lv = vscale == 0.f ? 0.f : log2f(vscale), inv_v = vscale == 0.f ? 0.f : 1.f / vscale;
       uint32_t p[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const float c = cq[n] * kscale;
         float x[4] = {fmaf(sc[0][2 * n], c, lv), fmaf(sc[0][2 * n + 1], c, lv), fmaf(sc[1][2 * n], c, lv), fmaf(sc[1][2 * n + 1], c, lv)};
-        if (edge) {  // c may be 0 or negative: -inf again
+        if (edge) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int y = tok + (r >> 1) * 8 + 2 * t + (r & 1);
-            if (y < tok_lo || y >= tok_hi || vscale == 0.f) x[r] = -INFINITY;
-          }
+          for (int r = 0; r < 4; ++r)
+            if (hidden(r)) x[r] = -INFINITY;
         }
         const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
         if (__any_sync(0xffffffffu, top > m[n] + 8.f)) {
@@ -332,152 +441,196 @@ kv8_attn_kernel(const __grid_constant__ Kv8AttnArgs a) {
           for (int n = 0; n < NT; ++n) mma_f16(o[2 * i + half][n], a0, a1, a2, a3, p[n][0], p[n][1]);
         }
       }
-    };
-
-    // two steps a turn, so that the buffers' indexes are constants
-    for (; s < s1; s += 2 * KA_WARPS) {
-      const int sa = s + KA_WARPS, sb = s + 2 * KA_WARPS;
-      if (sa < s1) {
-        const int blk = blk_next;
-        if (sb < s1) blk_next = page_of(sb);
-        load(sa, blk, kw[1], vw[1], ks[1], vs[1]);
-      }
-      compute(s, kw[0], vw[0], ks[0], vs[0]);
-      if (sa >= s1) break;
-      if (sb < s1) {
-        const int blk = blk_next;
-        if (sb + KA_WARPS < s1) blk_next = page_of(sb + KA_WARPS);
-        load(sb, blk, kw[0], vw[0], ks[0], vs[0]);
-      }
-      compute(sa, kw[1], vw[1], ks[1], vs[1]);
     }
 
-    // join the warps
+    // o[2 i + half][n]: dimensions 4 i' + 2 half of the lane's units, for the heads 2t ([0], [2]) and 2t + 1 ([1], [3])
+    const size_t part = (size_t)2 * warp + (s0 > 0 ? 0 : 1);
+    const bool finish = whole && !joined;
+    T* out = reinterpret_cast<T*>(a.out) + ((size_t)b * a.Hk * a.G + kvh * a.G + h0) * D;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       l[n] += __shfl_xor_sync(0xffffffffu, l[n], 1);
       l[n] += __shfl_xor_sync(0xffffffffu, l[n], 2);
       if (t == 0) {
-        sh_m[wid * HT + 8 * n + g] = m[n];
-        sh_l[wid * HT + 8 * n + g] = l[n];
+        if (joined) sh_ml[wid][8 * n + g] = make_float2(m[n], l[n]);
+        else if (!whole && 8 * n + g < heads) a.part_ml[part * HT + 8 * n + g] = make_float2(m[n], l[n]);
       }
 #pragma unroll
-      for (int i = 0; i < VW; ++i)
+      for (int c = 0; c < 2; ++c) {
+        const float den = __shfl_sync(0xffffffffu, l[n], 8 * t + 4 * c), inv = den != 0.f ? 1.f / den : 0.f;
+        const int h = 8 * n + 2 * t + c;
+        if (h >= heads) continue;
+        float* keep = joined ? reinterpret_cast<float*>(queue) + h * D : a.part + (part * HT + h) * D;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int d = VU * (g + 8 * (i / (VU / 4))) + 4 * (i % (VU / 4)) + 2 * half;  // and d + 1
-          float* dst = sh_o + ((size_t)(wid * HT) + 8 * n + 2 * t) * D + d;
-          *reinterpret_cast<float2*>(dst) = make_float2(o[2 * i + half][n][0], o[2 * i + half][n][2]);
-          *reinterpret_cast<float2*>(dst + D) = make_float2(o[2 * i + half][n][1], o[2 * i + half][n][3]);
-        }
-    }
-    __syncthreads();
-    const bool whole = s0 == 0 && s1 == steps;
-    float* part = a.part + ((size_t)2 * blockIdx.x + (u - s0 < first ? 0 : 1)) * HT * (D + 2);
-    for (int i = tid; i < HT * D; i += KA_THREADS) {
-      const int h = i / D, d = i % D;
-      if (h >= heads) break;
-      float mx = sh_m[h];
-#pragma unroll
-      for (int w = 1; w < KA_WARPS; ++w) mx = fmaxf(mx, sh_m[w * HT + h]);
-      float acc = 0.f, den = 0.f;
-#pragma unroll
-      for (int w = 0; w < KA_WARPS; ++w) {
-        const float f = fast_exp2(sh_m[w * HT + h] - mx);
-        acc = fmaf(sh_o[(size_t)(w * HT + h) * D + d], f, acc);
-        den = fmaf(sh_l[w * HT + h], f, den);
-      }
-      if (whole) {
-        store1(reinterpret_cast<T*>(a.out) + ((size_t)b * a.Hk * a.G + kvh * a.G + h0 + h) * D + d, den != 0.f ? acc / den : 0.f);
-      } else {
-        part[h * (D + 2) + d] = acc;
-        if (d == 0) {
-          part[h * (D + 2) + D] = mx;
-          part[h * (D + 2) + D + 1] = den;
+        for (int i = 0; i < VW; ++i) {
+          const int d = VU * (place<D>(g) + 8 * (i / (VU / 4))) + 4 * (i % (VU / 4));
+          const float x0 = o[2 * i][n][c], x1 = o[2 * i][n][2 + c], x2 = o[2 * i + 1][n][c], x3 = o[2 * i + 1][n][2 + c];
+          if (finish) *reinterpret_cast<uint2*>(out + h * D + d) = make_uint2(pack_out(x0 * inv, x1 * inv, T()), pack_out(x2 * inv, x3 * inv, T()));
+          else *reinterpret_cast<float4*>(keep + d) = make_float4(x0, x1, x2, x3);
         }
       }
     }
-    __syncthreads();
-    u += s1 - s0;
+  }
+  if (lane == 0) a.rows[warp] = shared;
+  if (!joined) return;
+  __syncthreads();  // each warp's sums stand in its queue, which is empty
+  // (a warp behind the end of the list has seen no row)
+  if (wid == 0 && lane == 0) sh_row = make_int4(join_seq, join_head, join_heads, (join_whole ? 2 : 0) + (int)(join_part & 1));
+  __syncthreads();
+  const int4 jr = sh_row;
+  const int heads = jr.z;
+  const size_t part = (size_t)2 * blockIdx.x * KA_WARPS + (jr.w & 1);
+  for (int i = tid; i < heads * (D / 4); i += KA_THREADS) {
+    const int h = i / (D / 4), d = (i % (D / 4)) * 4;
+    float mx = sh_ml[0][h].x, den = 0.f;
+#pragma unroll
+    for (int w = 1; w < KA_WARPS; ++w) mx = fmaxf(mx, sh_ml[w][h].x);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < KA_WARPS; ++w) {
+      const float2 ml = sh_ml[w][h];
+      if (ml.x == KA_NONE) continue;  // a warp without steps has written no sums
+      const float f = fast_exp2(ml.x - mx);
+      const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + w * S * STAGE) + h * D + d);
+      den = fmaf(ml.y, f, den);
+      acc.x = fmaf(x.x, f, acc.x);
+      acc.y = fmaf(x.y, f, acc.y);
+      acc.z = fmaf(x.z, f, acc.z);
+      acc.w = fmaf(x.w, f, acc.w);
+    }
+    if (jr.w & 2) {
+      const float inv = den != 0.f ? 1.f / den : 0.f;
+      T* out = reinterpret_cast<T*>(a.out) + ((size_t)jr.x * a.Hk * a.G + jr.y + h) * D;
+      *reinterpret_cast<uint2*>(out + d) = make_uint2(pack_out(acc.x * inv, acc.y * inv, T()), pack_out(acc.z * inv, acc.w * inv, T()));
+    } else {
+      *reinterpret_cast<float4*>(a.part + (part * HT + h) * D + d) = acc;
+      if (d == 0) a.part_ml[part * HT + h] = make_float2(mx, den);
+    }
   }
 }
 
-// Rows that several blocks share: their parts in the order of the blocks.  One block per (sequence, row of the list).
+// Rows that several warps share: their parts in order.  One block per block of the attention kernel, for the rows that its
+// warps began.  A joining warp takes a run of the parts of one head; runs of one head are joined in their order.
 template <int D, int HT, typename T>
-__global__ void __launch_bounds__(KA_THREADS)
-kv8_attn_join_kernel(const __grid_constant__ Kv8AttnArgs a, int blocks) {
+__global__ void __launch_bounds__(KA_JOIN)
+kv8_attn_join_kernel(const __grid_constant__ Kv8AttnArgs a) {
+  constexpr int E = D / 32, WARPS = KA_JOIN / 32;  // a lane's dimensions
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  __shared__ float sh_o[WARPS][D];
+  __shared__ float2 sh_ml[WARPS];
   pdl_launch_dependents();
   pdl_wait();
-  const int b = blockIdx.x, row = blockIdx.y, rows_per_seq = a.Hk * a.tiles;
-  __shared__ int sums[2][KA_WARPS];
-  int before = 0, all = 0, lo, hi;
-  for (int i = threadIdx.x; i < a.B; i += KA_THREADS) {
-    const int n = kv8_steps(a, i, lo, hi);
-    all += n;
-    if (i < b) before += n;
-  }
+  int begun[KA_WARPS], n = 0;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-    all += __shfl_xor_sync(0xffffffffu, all, o);
-  }
-  if ((threadIdx.x & 31) == 0) {
-    sums[0][threadIdx.x >> 5] = before;
-    sums[1][threadIdx.x >> 5] = all;
+  for (int i = 0; i < KA_WARPS; ++i) begun[i] = a.rows[blockIdx.x * KA_WARPS + i].seq;
+#pragma unroll
+  for (int i = 0; i < KA_WARPS; ++i) n += begun[i] >= 0;
+  if (n == 0) return;
+  const int team = WARPS / n;  // warps a row: 16, 8, 5 or 4
+  const int mine = wid / team, rank = wid % team;
+  int c0 = -1, k = 0;
+#pragma unroll
+  for (int i = 0; i < KA_WARPS; ++i)
+    if (begun[i] >= 0 && k++ == mine) c0 = blockIdx.x * KA_WARPS + i;
+  int runs = 1, heads = 0;
+  if (c0 >= 0) {
+    const SharedRow r = a.rows[c0];
+    heads = r.heads;
+    // warps whose parts count: c0 .. 4 joined0 - 1, the first of each joined block, and what follows those
+    const int j0 = r.joined0 * KA_WARPS, j1 = max(r.joined0, r.joined1) * KA_WARPS;
+    const int n0 = max(0, j0 - c0), n1 = n0 + max(0, (j1 - max(j0, c0)) / KA_WARPS);
+    const bool any = j1 > j0 && j0 >= c0;
+    const int parts = any ? n1 + max(0, r.last - j1 + 1) : r.last - c0 + 1;
+    auto at = [&](int p, int h) {
+      const int w = !any || p < n0 ? c0 + p : (p < n1 ? j0 + (p - n0) * KA_WARPS : j1 + (p - n1));
+      return ((size_t)2 * w + (p == 0 ? 1 : 0)) * HT + h;
+    };
+    runs = max(1, team / heads);
+    const int len = (parts + runs - 1) / runs;
+    for (int x = rank; x < heads * runs; x += team) {
+      const int h = x / runs, p0 = (x % runs) * len, p1 = min(parts, p0 + len);
+      float m = KA_NONE, l = 0.f, o[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = 0.f;
+      for (int p = p0 + lane; p < p1; p += 32) m = fmaxf(m, a.part_ml[at(p, h)].x);
+      m = warp_max(m);
+#pragma unroll 8
+      for (int p = p0; p < p1; ++p) {
+        const float2 ml = a.part_ml[at(p, h)];
+        const float f = fast_exp2(ml.x - m);
+        l = fmaf(ml.y, f, l);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = fmaf(a.part[at(p, h) * D + lane + 32 * e], f, o[e]);
+      }
+      if (runs == 1) {
+        const float inv = l != 0.f ? 1.f / l : 0.f;
+        T* out = reinterpret_cast<T*>(a.out) + ((size_t)r.seq * a.Hk * a.G + r.head + h) * D;
+#pragma unroll
+        for (int e = 0; e < E; ++e) store1(out + lane + 32 * e, o[e] * inv);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) sh_o[wid][lane + 32 * e] = o[e];
+        if (lane == 0) sh_ml[wid] = make_float2(m, l);
+      }
+    }
   }
   __syncthreads();
-  before = all = 0;
-  for (int w = 0; w < KA_WARPS; ++w) {
-    before += sums[0][w];
-    all += sums[1][w];
+  if (c0 < 0 || runs == 1 || rank >= heads) return;
+  const SharedRow r = a.rows[c0];
+  const int w0 = mine * team + rank * runs;  // the warps that had head `rank`
+  float mx = KA_NONE, den = 0.f, o[E];
+  for (int w = w0; w < w0 + runs; ++w) mx = fmaxf(mx, sh_ml[w].x);
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+  for (int w = w0; w < w0 + runs; ++w) {
+    const float f = fast_exp2(sh_ml[w].x - mx);
+    den = fmaf(sh_ml[w].y, f, den);
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = fmaf(sh_o[w][lane + 32 * e], f, o[e]);
   }
-  const int steps = kv8_steps(a, b, lo, hi);
-  if (steps == 0) return;
-  const long long run = kv8_run(a, (long long)all * rows_per_seq, blocks);
-  const long long u0 = (long long)before * rows_per_seq + (long long)row * steps, u1 = u0 + steps;
-  const long long c0 = u0 / run, c1 = (u1 - 1) / run;
-  if (c0 == c1) return;  // one block had all of it
-  const int kvh = row / a.tiles, h0 = (row % a.tiles) * HT, heads = min(HT, a.G - h0);
-  for (int i = threadIdx.x; i < heads * D; i += KA_THREADS) {
-    const int h = i / D, d = i % D;
-    float mx = KA_NONE, acc = 0.f, den = 0.f;
-    for (long long c = c0; c <= c1; ++c) {
-      const float* p = a.part + ((size_t)2 * c + (u0 < c * run ? 0 : 1)) * HT * (D + 2) + h * (D + 2);
-      const float pm = p[D], up = fmaxf(mx, pm), fa = fast_exp2(mx - up), fb = fast_exp2(pm - up);
-      acc = fmaf(p[d], fb, acc * fa);
-      den = fmaf(p[D + 1], fb, den * fa);
-      mx = up;
-    }
-    store1(reinterpret_cast<T*>(a.out) + ((size_t)b * a.Hk * a.G + kvh * a.G + h0 + h) * D + d, den != 0.f ? acc / den : 0.f);
-  }
+  const float inv = den != 0.f ? 1.f / den : 0.f;
+  T* out = reinterpret_cast<T*>(a.out) + ((size_t)r.seq * a.Hk * a.G + r.head + rank) * D;
+#pragma unroll
+  for (int e = 0; e < E; ++e) store1(out + lane + 32 * e, o[e] * inv);
 }
 
 inline int kv8_head_tile(int D, int G) { return G <= 8 || D > 128 ? 8 : 16; }
 inline int kv8_attn_blocks(int D, int HT) { return trlb_host::sm_count() * kv8_attn_per_sm(D, HT); }
 
 template <int D, int HT, typename T>
-int kv8_attn_launch(Kv8AttnArgs& a, cudaStream_t st) {
-  const size_t smem = (size_t)KA_WARPS * HT * (D + 2) * 4 + (size_t)(a.B + 1) * 4;
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kv8_attn_kernel<D, HT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 72 * 1024);
-    if (e != cudaSuccess) return (int)e;
-  }
-  const int blocks = kv8_attn_blocks(D, HT);
-  const bool pdl = trlb_host::pdl_enabled();
-  cudaError_t e = trlb_host::launch_kernel(kv8_attn_kernel<D, HT, T>, dim3(blocks), dim3(KA_THREADS), smem, st, pdl, a);
+int kv8_attn_launch(Kv8AttnArgs& a, const void* k, const void* v, cudaStream_t st) {
+  const size_t queues = (size_t)KA_WARPS * kv8_attn_stages(D) * 32 * D + 1024, smem = queues + (size_t)(a.B + 1) * 4;
+  static bool ready[64] = {};  // per device; a second thread that sets it at once sets the same
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return (int)e;
-  return (int)trlb_host::launch_kernel(kv8_attn_join_kernel<D, HT, T>, dim3(a.B, a.Hk * a.tiles), dim3(KA_THREADS), 0, st, pdl, a, blocks);
+  if (dev >= 64 || !ready[dev]) {
+    e = cudaFuncSetAttribute(kv8_attn_kernel<D, HT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)queues + (KA_MAX_SEQS + 1) * 4);
+    if (e != cudaSuccess) return (int)e;
+    if (dev < 64) ready[dev] = true;
+  }
+  const uint64_t tiles = (uint64_t)a.pages * a.Hk, page = 1ull << a.page_shift;
+  const uint32_t box = D % 128 == 0 ? 128 : D;
+  if (trlb_host::make_tmap_3d_u8(&a.k, k, D, page, tiles, box, KA_STEP, kv8_attn_swizzle(D)) ||
+      trlb_host::make_tmap_3d_u8(&a.v, v, D, page, tiles, box, KA_STEP, kv8_attn_swizzle(D)))
+    return -6;
+  const int blocks = kv8_attn_blocks(D, HT);
+  a.part_ml = reinterpret_cast<float2*>(a.part + (size_t)2 * blocks * KA_WARPS * HT * D);  // each on 16 bytes
+  a.rows = reinterpret_cast<SharedRow*>(a.part_ml + (size_t)2 * blocks * KA_WARPS * HT);
+  e = trlb_host::launch_kernel(kv8_attn_kernel<D, HT, T>, dim3(blocks), dim3(KA_THREADS), smem, st, trlb_host::pdl_enabled(), a);
+  if (e != cudaSuccess) return (int)e;
+  // it waits for the attention kernel by itself, so it may always be set up under that kernel's end
+  return (int)trlb_host::launch_kernel(kv8_attn_join_kernel<D, HT, T>, dim3(blocks), dim3(KA_JOIN), 0, st, true, a);
 }
 template <typename T>
-int kv8_attn_pick(Kv8AttnArgs& a, int D, cudaStream_t st) {
+int kv8_attn_pick(Kv8AttnArgs& a, const void* k, const void* v, int D, cudaStream_t st) {
   const int ht = kv8_head_tile(D, a.G);
   a.tiles = (a.G + ht - 1) / ht;
-  if (a.Hk * a.tiles > 65535) return -5;
   switch (D) {
-    case 64: return ht == 8 ? kv8_attn_launch<64, 8, T>(a, st) : kv8_attn_launch<64, 16, T>(a, st);
-    case 96: return ht == 8 ? kv8_attn_launch<96, 8, T>(a, st) : kv8_attn_launch<96, 16, T>(a, st);
-    case 128: return ht == 8 ? kv8_attn_launch<128, 8, T>(a, st) : kv8_attn_launch<128, 16, T>(a, st);
-    case 256: return kv8_attn_launch<256, 8, T>(a, st);
+    case 64: return ht == 8 ? kv8_attn_launch<64, 8, T>(a, k, v, st) : kv8_attn_launch<64, 16, T>(a, k, v, st);
+    case 96: return ht == 8 ? kv8_attn_launch<96, 8, T>(a, k, v, st) : kv8_attn_launch<96, 16, T>(a, k, v, st);
+    case 128: return ht == 8 ? kv8_attn_launch<128, 8, T>(a, k, v, st) : kv8_attn_launch<128, 16, T>(a, k, v, st);
+    case 256: return kv8_attn_launch<256, 8, T>(a, k, v, st);
   }
   return -1;
 }
@@ -489,7 +642,7 @@ using namespace trlb;
 // fp32 words of scratch that a call needs: parts of rows that several blocks share
 TRLB_API long long trlb_kv8_attn_scratch(int Hq, int Hk, int D) {
   const int ht = kv8_head_tile(D, Hq / Hk);
-  return 2ll * kv8_attn_blocks(D, ht) * ht * (D + 2);
+  return (2ll * ht * (D + 2) + sizeof(SharedRow) / 4) * KA_WARPS * kv8_attn_blocks(D, ht);
 }
 
 // q [B, Hq, D] bf16 (dtype 0) or fp16 (1) with strides in elements (multiples of 4, rows 8 bytes aligned); out dense.
@@ -504,9 +657,10 @@ TRLB_API int trlb_kv8_decode_attn(const void* q, int dtype, long long q_row, lon
   if (page_size < KA_STEP || (page_size & (page_size - 1))) return -3;
   int shift = 0;
   while ((1 << shift) < page_size) ++shift;
-  Kv8AttnArgs a{q, q_row, q_head, (const uint8_t*)k_codes, (const uint8_t*)v_codes, k_scale, v_scale, table, seq_lens, slots,
-                out, part, status, pages, Hk, Hq / Hk, 1, shift, table_rows, max_blocks, B, window, KA_WARPS, scale};
-  if (dtype == 0) return kv8_attn_pick<__nv_bfloat16>(a, D, st);
-  if (dtype == 1) return kv8_attn_pick<__half>(a, D, st);
+  if ((long long)pages * Hk > 2147483647ll) return -5;
+  Kv8AttnArgs a{{}, {}, q, q_row, q_head, k_scale, v_scale, table, seq_lens, slots,
+                out, part, nullptr, nullptr, status, pages, Hk, Hq / Hk, 1, shift, table_rows, max_blocks, B, window, 1, scale};
+  if (dtype == 0) return kv8_attn_pick<__nv_bfloat16>(a, k_codes, v_codes, D, st);
+  if (dtype == 1) return kv8_attn_pick<__half>(a, k_codes, v_codes, D, st);
   return -4;
 }
