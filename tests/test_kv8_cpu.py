@@ -126,7 +126,7 @@ def test_append_refuses(change, message):
     (dict(q=torch.zeros(3, 3, 64, dtype=torch.bfloat16)), "multiple of 2 heads"), (dict(q=torch.zeros(3, 4, 64)), "bf16 or fp16"),
     (dict(q=torch.zeros(3, 4, 128, dtype=torch.bfloat16)), "q has to be"), (dict(lens=torch.zeros(2, dtype=torch.int32)), "lengths"),
     (dict(window=0), "window"), (dict(out=torch.zeros(3, 4, 64)), "out has to be"),
-    (dict(slots=torch.zeros(2, dtype=torch.int32)), "slots"), (dict(q=torch.zeros(8193, 4, 64, dtype=torch.bfloat16)), "8192")])
+    (dict(slots=torch.zeros(2, dtype=torch.int32)), "slots"), (dict(q=torch.zeros(4097, 4, 64, dtype=torch.bfloat16)), "4096")])
 def test_attention_refuses(change, message):
     from trl_b200.ops import cuda as K
 

@@ -32,16 +32,15 @@ namespace trlb {
 
 enum { SITE_KV8_ATTN = 1410 };
 
-constexpr int KA_WARPS = 4, KA_THREADS = KA_WARPS * 32;
 constexpr int KA_STEP = 16;          // tokens of a warp's step
-constexpr int KA_ROW = 2;            // steps that a row's beginning is worth
+constexpr int KA_ROW = 4;            // steps that a row's beginning is worth
 constexpr int KA_JOIN = 512;         // threads of a joining block
-constexpr int KA_MAX_SEQS = 8192;    // the prefix sums of their steps stand in shared memory
+constexpr int KA_MAX_SEQS = 4096;    // the prefix sums of their steps stand in shared memory
 constexpr float KA_NONE = -1e30f;    // maximum of no token: finite, so that exp2(-inf - m) is 0
 
-// Steps in a warp's queue and blocks an SM holds: about 190 KB of codes under way on an SM, as registers allow.
-__host__ __device__ constexpr int kv8_attn_stages(int D) { return D == 256 ? 3 : 4; }
-__host__ __device__ constexpr int kv8_attn_per_sm(int D, int HT) { return D == 256 ? 2 : 3; }
+// One block an SM, with as many warps as registers allow, and the steps in a warp's queue: about 190 KB of codes under way.
+__host__ __device__ constexpr int kv8_attn_warps(int D, int HT) { return D == 256 ? 8 : (D == 64 && HT == 8 ? 16 : 12); }
+__host__ __device__ constexpr int kv8_attn_stages(int D) { return D == 256 ? 3 : (D == 128 ? 4 : (D == 96 ? 5 : 6)); }
 // Swizzle of a row's bytes in shared memory; 96 bytes stand as they are.
 __host__ __device__ constexpr int kv8_attn_swizzle(int D) { return D % 128 == 0 ? 128 : (D == 64 ? 64 : 0); }
 
@@ -127,15 +126,16 @@ __device__ __forceinline__ int kv8_steps(const Kv8AttnArgs& a, int b, int& lo, i
 }
 
 // prefix[b] = cost of one row of each of the sequences before b, prefix[B] = of all
+template <int WARPS>
 __device__ __forceinline__ void kv8_prefix(const Kv8AttnArgs& a, int* prefix, int* warp_sums) {
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-  const int per = (a.B + KA_THREADS - 1) / KA_THREADS;
-  int sum = 0, lo, hi;
-  auto cost = [&](int i) {
+  const int per = (a.B + WARPS * 32 - 1) / (WARPS * 32), i0 = min(a.B, tid * per), i1 = min(a.B, i0 + per);
+  int sum = 0, last = 0, lo, hi;
+  for (int i = i0; i < i1; ++i) {
     const int n = kv8_steps(a, i, lo, hi);
-    return n > 0 ? n + KA_ROW : 0;
-  };
-  for (int i = tid * per; i < min(a.B, (tid + 1) * per); ++i) sum += cost(i);
+    last = n > 0 ? n + KA_ROW : 0;
+    sum += last;
+  }
   int run = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -146,20 +146,29 @@ __device__ __forceinline__ void kv8_prefix(const Kv8AttnArgs& a, int* prefix, in
   __syncthreads();
   int before = run - sum;
   for (int w = 0; w < wid; ++w) before += warp_sums[w];
-  for (int i = tid * per; i < min(a.B, (tid + 1) * per); ++i) {
+  for (int i = i0; i < i1; ++i) {
     prefix[i] = before;
-    before += cost(i);
+    if (per > 1) {
+      const int n = kv8_steps(a, i, lo, hi);
+      last = n > 0 ? n + KA_ROW : 0;
+    }
+    before += last;
   }
-  if (tid == KA_THREADS - 1) prefix[a.B] = before;
+  if (tid == WARPS * 32 - 1) prefix[a.B] = before;
   __syncthreads();
+}
+// Quotient of numbers that mostly fit into 32 bits.
+__device__ __forceinline__ int kv8_div(long long x, int d) {
+  return (x >> 31) == 0 ? (int)((unsigned)x / (unsigned)d) : (int)(x / d);
 }
 
 template <int D, int HT, typename T>
-__global__ void __launch_bounds__(KA_THREADS, kv8_attn_per_sm(D, HT))
+__global__ void __launch_bounds__(kv8_attn_warps(D, HT) * 32, 1)
 kv8_attn_kernel(const __grid_constant__ Kv8AttnArgs a) {
   constexpr int KU = D % 64 == 0 ? 16 : 8, KN = D / (4 * KU);                         // K: bytes of a lane's unit, units a row
   constexpr int VU = D % 128 == 0 ? 16 : (D % 64 == 0 ? 8 : 4), VN = D / (8 * VU);    // V: the same
   constexpr int KW = D / 16, VW = D / 32;                                             // words of a row in a lane
+  constexpr int KA_WARPS = kv8_attn_warps(D, HT), KA_THREADS = KA_WARPS * 32;
   constexpr int NT = HT / 8, S = kv8_attn_stages(D), STAGE = 32 * D, BOX = D % 128 == 0 ? 128 : D;
   extern __shared__ uint8_t smem_raw[];  // [warps][S][K tile, V tile] on 1024 bytes, then prefix [B + 1]
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -182,7 +191,7 @@ kv8_attn_kernel(const __grid_constant__ Kv8AttnArgs a) {
   }
   pdl_launch_dependents();
   pdl_wait();
-  kv8_prefix(a, prefix, warp_sums);  // its barriers show the mbarriers, too
+  kv8_prefix<KA_WARPS>(a, prefix, warp_sums);  // its barriers show the mbarriers, too
   // sequences without a token to see have no steps: their zeros are written here
   for (int b = blockIdx.x; b < a.B; b += gridDim.x)
     if (prefix[b + 1] == prefix[b])
@@ -204,7 +213,7 @@ kv8_attn_kernel(const __grid_constant__ Kv8AttnArgs a) {
     }
     const int cost = prefix[b + 1] - prefix[b];
     const long long seq0 = (long long)prefix[b] * rows_per_seq;
-    joined = seq0 + ((block0 - seq0) / cost + 1) * cost >= block1;
+    joined = seq0 + (long long)(kv8_div(block0 - seq0, cost) + 1) * cost >= block1;
   }
   if (lane < HT) sh_ml[wid][lane] = make_float2(KA_NONE, 0.f);
   uint8_t* queue = smem + wid * S * STAGE;
@@ -218,7 +227,7 @@ kv8_attn_kernel(const __grid_constant__ Kv8AttnArgs a) {
     while (prefix[b + 1] == prefix[b] || (long long)prefix[b + 1] * rows_per_seq <= u) ++b;
     const int cost = prefix[b + 1] - prefix[b], steps = cost - KA_ROW;
     const long long seq0 = (long long)prefix[b] * rows_per_seq;
-    const int row = (int)((u - seq0) / cost);
+    const int row = kv8_div(u - seq0, cost);
     const long long row0 = seq0 + (long long)row * cost;  // its beginning counts first, then its steps
     const int s0 = (int)max(0ll, u - row0 - KA_ROW), s1 = (int)min((long long)steps, u1 - row0 - KA_ROW);
     const int kvh = row / a.tiles, h0 = (row % a.tiles) * HT, heads = min(HT, a.G - h0);
@@ -514,70 +523,90 @@ kv8_attn_kernel(const __grid_constant__ Kv8AttnArgs a) {
 template <int D, int HT, typename T>
 __global__ void __launch_bounds__(KA_JOIN)
 kv8_attn_join_kernel(const __grid_constant__ Kv8AttnArgs a) {
-  constexpr int E = D / 32, WARPS = KA_JOIN / 32;  // a lane's dimensions
+  constexpr int KA_WARPS = kv8_attn_warps(D, HT), E = D / 32, WARPS = KA_JOIN / 32, AHEAD = 8;  // E: a lane's dimensions
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   __shared__ float sh_o[WARPS][D];
   __shared__ float2 sh_ml[WARPS];
+  __shared__ SharedRow sh_rows[KA_WARPS];
   pdl_launch_dependents();
   pdl_wait();
-  int begun[KA_WARPS], n = 0;
+  if (threadIdx.x < KA_WARPS * 2) reinterpret_cast<int4*>(sh_rows)[threadIdx.x] = reinterpret_cast<const int4*>(a.rows + blockIdx.x * KA_WARPS)[threadIdx.x];
+  __syncthreads();
+  int n = 0;
 #pragma unroll
-  for (int i = 0; i < KA_WARPS; ++i) begun[i] = a.rows[blockIdx.x * KA_WARPS + i].seq;
-#pragma unroll
-  for (int i = 0; i < KA_WARPS; ++i) n += begun[i] >= 0;
+  for (int i = 0; i < KA_WARPS; ++i) n += sh_rows[i].seq >= 0;
   if (n == 0) return;
-  const int team = WARPS / n;  // warps a row: 16, 8, 5 or 4
-  const int mine = wid / team, rank = wid % team;
-  int c0 = -1, k = 0;
-#pragma unroll
-  for (int i = 0; i < KA_WARPS; ++i)
-    if (begun[i] >= 0 && k++ == mine) c0 = blockIdx.x * KA_WARPS + i;
-  int runs = 1, heads = 0;
-  if (c0 >= 0) {
-    const SharedRow r = a.rows[c0];
-    heads = r.heads;
-    // warps whose parts count: c0 .. 4 joined0 - 1, the first of each joined block, and what follows those
-    const int j0 = r.joined0 * KA_WARPS, j1 = max(r.joined0, r.joined1) * KA_WARPS;
-    const int n0 = max(0, j0 - c0), n1 = n0 + max(0, (j1 - max(j0, c0)) / KA_WARPS);
-    const bool any = j1 > j0 && j0 >= c0;
+  const int tile = min(HT, a.G), runs = max(1, WARPS / (n * tile));  // warps a head
+  for (int x = wid; x < n * tile * runs; x += WARPS) {
+    const int h = x / runs % tile;
+    int c0 = -1, k = x / runs / tile;
+    for (int i = 0; i < KA_WARPS; ++i)
+      if (sh_rows[i].seq >= 0 && k-- == 0) c0 = i;
+    const SharedRow r = sh_rows[c0];
+    if (h >= r.heads) continue;
+    c0 += blockIdx.x * KA_WARPS;
+    // parts that count: the warps c0 .. j0 - 1, the first one of each joined block up to j1, and the warps from there on
+    const int j0 = r.joined0 * KA_WARPS, j1 = r.joined1 * KA_WARPS;
+    const bool any = j1 > j0;
+    const int n0 = any ? j0 - c0 : 0, n1 = any ? n0 + r.joined1 - r.joined0 : 0;
     const int parts = any ? n1 + max(0, r.last - j1 + 1) : r.last - c0 + 1;
-    auto at = [&](int p, int h) {
+    const int len = (parts + runs - 1) / runs, p0 = (x % runs) * len, p1 = min(parts, p0 + len);
+    auto at = [&](int p) {
       const int w = !any || p < n0 ? c0 + p : (p < n1 ? j0 + (p - n0) * KA_WARPS : j1 + (p - n1));
       return ((size_t)2 * w + (p == 0 ? 1 : 0)) * HT + h;
     };
-    runs = max(1, team / heads);
-    const int len = (parts + runs - 1) / runs;
-    for (int x = rank; x < heads * runs; x += team) {
-      const int h = x / runs, p0 = (x % runs) * len, p1 = min(parts, p0 + len);
-      float m = KA_NONE, l = 0.f, o[E];
+    float m = KA_NONE, l = 0.f, o[E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = 0.f;
-      for (int p = p0 + lane; p < p1; p += 32) m = fmaxf(m, a.part_ml[at(p, h)].x);
-      m = warp_max(m);
-#pragma unroll 8
-      for (int p = p0; p < p1; ++p) {
-        const float2 ml = a.part_ml[at(p, h)];
-        const float f = fast_exp2(ml.x - m);
-        l = fmaf(ml.y, f, l);
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+    for (int p = p0; p < p1; p += AHEAD) {  // AHEAD parts under way at once
+      float2 ml[AHEAD];
+      float y[AHEAD][E], top = m;
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = fmaf(a.part[at(p, h) * D + lane + 32 * e], f, o[e]);
+      for (int i = 0; i < AHEAD; ++i) {
+        ml[i] = make_float2(KA_NONE, 0.f);
+        if (p + i < p1) {
+          const size_t q = at(p + i);
+          ml[i] = a.part_ml[q];
+#pragma unroll
+          for (int e = 0; e < E; ++e) y[i][e] = a.part[q * D + lane + 32 * e];
+        }
       }
-      if (runs == 1) {
-        const float inv = l != 0.f ? 1.f / l : 0.f;
-        T* out = reinterpret_cast<T*>(a.out) + ((size_t)r.seq * a.Hk * a.G + r.head + h) * D;
 #pragma unroll
-        for (int e = 0; e < E; ++e) store1(out + lane + 32 * e, o[e] * inv);
-      } else {
+      for (int i = 0; i < AHEAD; ++i) top = fmaxf(top, ml[i].x);
+      const float down = fast_exp2(m - top);
+      m = top;
+      l *= down;
 #pragma unroll
-        for (int e = 0; e < E; ++e) sh_o[wid][lane + 32 * e] = o[e];
-        if (lane == 0) sh_ml[wid] = make_float2(m, l);
-      }
+      for (int e = 0; e < E; ++e) o[e] *= down;
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i)
+        if (p + i < p1) {
+          const float f = fast_exp2(ml[i].x - top);
+          l = fmaf(ml[i].y, f, l);
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[e] = fmaf(y[i][e], f, o[e]);
+        }
+    }
+    if (runs == 1) {
+      const float inv = l != 0.f ? 1.f / l : 0.f;
+      T* out = reinterpret_cast<T*>(a.out) + ((size_t)r.seq * a.Hk * a.G + r.head + h) * D;
+#pragma unroll
+      for (int e = 0; e < E; ++e) store1(out + lane + 32 * e, o[e] * inv);
+    } else {  // then no warp takes a second run
+#pragma unroll
+      for (int e = 0; e < E; ++e) sh_o[wid][lane + 32 * e] = o[e];
+      if (lane == 0) sh_ml[wid] = make_float2(m, l);
     }
   }
+  if (runs == 1) return;
   __syncthreads();
-  if (c0 < 0 || runs == 1 || rank >= heads) return;
-  const SharedRow r = a.rows[c0];
-  const int w0 = mine * team + rank * runs;  // the warps that had head `rank`
+  if (wid >= n * tile) return;
+  const int h = wid % tile, w0 = wid * runs;  // the warps that had this head
+  int c0 = -1, k = wid / tile;
+  for (int i = 0; i < KA_WARPS; ++i)
+    if (sh_rows[i].seq >= 0 && k-- == 0) c0 = i;
+  const SharedRow r = sh_rows[c0];
+  if (h >= r.heads) return;
   float mx = KA_NONE, den = 0.f, o[E];
   for (int w = w0; w < w0 + runs; ++w) mx = fmaxf(mx, sh_ml[w].x);
 #pragma unroll
@@ -589,17 +618,17 @@ kv8_attn_join_kernel(const __grid_constant__ Kv8AttnArgs a) {
     for (int e = 0; e < E; ++e) o[e] = fmaf(sh_o[w][lane + 32 * e], f, o[e]);
   }
   const float inv = den != 0.f ? 1.f / den : 0.f;
-  T* out = reinterpret_cast<T*>(a.out) + ((size_t)r.seq * a.Hk * a.G + r.head + rank) * D;
+  T* out = reinterpret_cast<T*>(a.out) + ((size_t)r.seq * a.Hk * a.G + r.head + h) * D;
 #pragma unroll
   for (int e = 0; e < E; ++e) store1(out + lane + 32 * e, o[e] * inv);
 }
 
 inline int kv8_head_tile(int D, int G) { return G <= 8 || D > 128 ? 8 : 16; }
-inline int kv8_attn_blocks(int D, int HT) { return trlb_host::sm_count() * kv8_attn_per_sm(D, HT); }
 
 template <int D, int HT, typename T>
 int kv8_attn_launch(Kv8AttnArgs& a, const void* k, const void* v, cudaStream_t st) {
-  const size_t queues = (size_t)KA_WARPS * kv8_attn_stages(D) * 32 * D + 1024, smem = queues + (size_t)(a.B + 1) * 4;
+  constexpr int WARPS = kv8_attn_warps(D, HT);
+  const size_t queues = (size_t)WARPS * kv8_attn_stages(D) * 32 * D + 1024, smem = queues + (size_t)(a.B + 1) * 4;
   static bool ready[64] = {};  // per device; a second thread that sets it at once sets the same
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -614,10 +643,10 @@ int kv8_attn_launch(Kv8AttnArgs& a, const void* k, const void* v, cudaStream_t s
   if (trlb_host::make_tmap_3d_u8(&a.k, k, D, page, tiles, box, KA_STEP, kv8_attn_swizzle(D)) ||
       trlb_host::make_tmap_3d_u8(&a.v, v, D, page, tiles, box, KA_STEP, kv8_attn_swizzle(D)))
     return -6;
-  const int blocks = kv8_attn_blocks(D, HT);
-  a.part_ml = reinterpret_cast<float2*>(a.part + (size_t)2 * blocks * KA_WARPS * HT * D);  // each on 16 bytes
-  a.rows = reinterpret_cast<SharedRow*>(a.part_ml + (size_t)2 * blocks * KA_WARPS * HT);
-  e = trlb_host::launch_kernel(kv8_attn_kernel<D, HT, T>, dim3(blocks), dim3(KA_THREADS), smem, st, trlb_host::pdl_enabled(), a);
+  const int blocks = trlb_host::sm_count();
+  a.part_ml = reinterpret_cast<float2*>(a.part + (size_t)2 * blocks * WARPS * HT * D);  // each on 16 bytes
+  a.rows = reinterpret_cast<SharedRow*>(a.part_ml + (size_t)2 * blocks * WARPS * HT);
+  e = trlb_host::launch_kernel(kv8_attn_kernel<D, HT, T>, dim3(blocks), dim3(WARPS * 32), smem, st, trlb_host::pdl_enabled(), a);
   if (e != cudaSuccess) return (int)e;
   // it waits for the attention kernel by itself, so it may always be set up under that kernel's end
   return (int)trlb_host::launch_kernel(kv8_attn_join_kernel<D, HT, T>, dim3(blocks), dim3(KA_JOIN), 0, st, true, a);
@@ -642,7 +671,7 @@ using namespace trlb;
 // fp32 words of scratch that a call needs: parts of rows that several blocks share
 TRLB_API long long trlb_kv8_attn_scratch(int Hq, int Hk, int D) {
   const int ht = kv8_head_tile(D, Hq / Hk);
-  return (2ll * ht * (D + 2) + sizeof(SharedRow) / 4) * KA_WARPS * kv8_attn_blocks(D, ht);
+  return (2ll * ht * (D + 2) + sizeof(SharedRow) / 4) * kv8_attn_warps(D, ht) * trlb_host::sm_count();
 }
 
 // q [B, Hq, D] bf16 (dtype 0) or fp16 (1) with strides in elements (multiples of 4, rows 8 bytes aligned); out dense.

@@ -1194,8 +1194,8 @@ def kv8_decode_attn(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens
     if q.dtype not in (torch.bfloat16, torch.float16) or q.dim() != 3 or q.shape[2] != dim or q.shape[1] % heads or q.shape[1] == 0:
         raise ValueError(f"q has to be bf16 or fp16 [sequences, a multiple of {heads} heads, {dim}], not {q.dtype} {tuple(q.shape)}")
     B, Hq, _ = q.shape
-    if B > 8192:
-        raise ValueError("at most 8192 sequences a call")
+    if B > 4096:
+        raise ValueError("at most 4096 sequences a call")
     if q.stride(2) != 1 or q.stride(0) % 4 or q.stride(1) % 4 or q.data_ptr() % 8:
         q = q.contiguous()
     _same_device(k_cache.device, q=q, seq_lens=seq_lens, slots=slots, out=out)
