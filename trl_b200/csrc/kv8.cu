@@ -9,6 +9,7 @@
 // max(scale, 2^e(a)) otherwise; in the second case the rows that stand before are brought to the new scale.  Rows behind
 // the last token are left as they are.
 #include <cuda_fp16.h>
+#include <type_traits>
 
 #include "kv8.cuh"
 
@@ -319,25 +320,32 @@ int kv8_append_launch(const Kv8Source<T>& src, const Kv8Cache& c, const int* tab
 
 using namespace trlb;
 
-// dtype: 0 bf16, 1 fp16, 2 fp32.  Rows of D dense elements, 16 bytes aligned.  cu null: one token per sequence (tokens == n).
-TRLB_API int trlb_kv8_append(const void* k, const void* v, int dtype, long long k_tok, long long k_head, long long v_tok,
-                             long long v_head, void* k_codes, void* v_codes, float* k_scale, float* v_scale, int pages,
-                             int heads, int page_size, int dim, const int* table, int table_rows, int max_blocks,
-                             const int* starts, const int* cu, const int* slots, int n, int tokens, int max_new, int* status,
-                             cudaStream_t st) {
-  if (n == 0 || tokens == 0) return 0;
-  if (dim <= 0 || dim > 256 || dim % 16 || heads <= 0 || heads > 65535 || page_size <= 0) return -1;
-  if (max_new < 1 || (cu == nullptr && tokens != n)) return -2;
-  Kv8Cache c{{(uint8_t*)k_codes, (uint8_t*)v_codes}, {k_scale, v_scale}, pages, heads, page_size, dim};
-  if (dtype == 0)
-    return kv8_append_launch(Kv8Source<__nv_bfloat16>{{(const __nv_bfloat16*)k, (const __nv_bfloat16*)v}, {k_tok, v_tok}, {k_head, v_head}},
-                             c, table, table_rows, max_blocks, starts, cu, slots, n, tokens, max_new, status, st);
-  if (dtype == 1)
-    return kv8_append_launch(Kv8Source<__half>{{(const __half*)k, (const __half*)v}, {k_tok, v_tok}, {k_head, v_head}}, c, table,
-                             table_rows, max_blocks, starts, cu, slots, n, tokens, max_new, status, st);
-  if (dtype == 2)
-    return kv8_append_launch(Kv8Source<float>{{(const float*)k, (const float*)v}, {k_tok, v_tok}, {k_head, v_head}}, c, table,
-                             table_rows, max_blocks, starts, cu, slots, n, tokens, max_new, status, st);
+// dtype: 0 bf16, 1 fp16, 2 fp32.  Rows of dim dense elements on 16 bytes.  cu null: one token per sequence (tokens == n).
+struct Kv8AppendCall {
+  const void *k, *v;
+  void *k_codes, *v_codes;
+  float *k_scale, *v_scale;
+  const int *table, *starts, *cu, *slots;
+  int* status;
+  cudaStream_t stream;
+  long long k_tok, k_head, v_tok, v_head;  // strides in elements
+  int dtype, pages, heads, page_size, dim, table_rows, max_blocks, n, tokens, max_new;
+};
+TRLB_API int trlb_kv8_append(const Kv8AppendCall* call) {
+  const Kv8AppendCall a = *call;
+  if (a.n == 0 || a.tokens == 0) return 0;
+  if (a.dim <= 0 || a.dim > 256 || a.dim % 16 || a.heads <= 0 || a.heads > 65535 || a.page_size <= 0) return -1;
+  if (a.max_new < 1 || (a.cu == nullptr && a.tokens != a.n)) return -2;
+  Kv8Cache c{{(uint8_t*)a.k_codes, (uint8_t*)a.v_codes}, {a.k_scale, a.v_scale}, a.pages, a.heads, a.page_size, a.dim};
+  auto go = [&](auto* type) {
+    using T = std::remove_pointer_t<decltype(type)>;
+    const Kv8Source<T> src{{(const T*)a.k, (const T*)a.v}, {a.k_tok, a.v_tok}, {a.k_head, a.v_head}};
+    return kv8_append_launch(src, c, a.table, a.table_rows, a.max_blocks, a.starts, a.cu, a.slots, a.n, a.tokens, a.max_new,
+                             a.status, a.stream);
+  };
+  if (a.dtype == 0) return go((__nv_bfloat16*)nullptr);
+  if (a.dtype == 1) return go((__half*)nullptr);
+  if (a.dtype == 2) return go((float*)nullptr);
   return -4;
 }
 

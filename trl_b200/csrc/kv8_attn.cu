@@ -85,7 +85,7 @@ __device__ __forceinline__ int place(int c) { return D % 128 == 0 ? (c >> 1) | (
 __device__ __forceinline__ uint32_t pack_out(float a, float b, __nv_bfloat16) { return pack_bf16(a, b); }
 __device__ __forceinline__ uint32_t pack_out(float a, float b, __half) { return pack_f16(a, b); }
 
-struct SharedRow {
+struct alignas(16) SharedRow {
   int seq, head, heads;  // seq < 0: none
   int last;              // warp of the last step
   int joined0, joined1;  // blocks whose warps' parts are one, at the first warp's place
@@ -669,27 +669,38 @@ int kv8_attn_pick(Kv8AttnArgs& a, const void* k, const void* v, int D, cudaStrea
 using namespace trlb;
 
 // fp32 words of scratch that a call needs: parts of rows that several blocks share
-TRLB_API long long trlb_kv8_attn_scratch(int Hq, int Hk, int D) {
+TRLB_API long long trlb_kv8_attn_scratch(int device, int Hq, int Hk, int D) {
+  (void)device;
   const int ht = kv8_head_tile(D, Hq / Hk);
   return (2ll * ht * (D + 2) + sizeof(SharedRow) / 4) * kv8_attn_warps(D, ht) * trlb_host::sm_count();
 }
 
-// q [B, Hq, D] bf16 (dtype 0) or fp16 (1) with strides in elements (multiples of 4, rows 8 bytes aligned); out dense.
-// page_size a power of two, 16 or more.  window 0: everything.  Rows with seq_len < 0 get zeros.
-TRLB_API int trlb_kv8_decode_attn(const void* q, int dtype, long long q_row, long long q_head, const void* k_codes,
-                                  const void* v_codes, const float* k_scale, const float* v_scale, int pages, int page_size,
-                                  const int* table, int table_rows, int max_blocks, const int* seq_lens, const int* slots,
-                                  int B, int Hq, int Hk, int D, float scale, int window, float* part, void* out, int* status,
-                                  cudaStream_t st) {
-  if (B == 0) return 0;
-  if (Hk <= 0 || Hq <= 0 || Hq % Hk || B > KA_MAX_SEQS || window < 0) return -2;
-  if (page_size < KA_STEP || (page_size & (page_size - 1))) return -3;
+// q [B, Hq, D] bf16 (dtype 0) or fp16 (1) with strides in elements (multiples of 4, rows 8 bytes aligned); out dense, on 16
+// bytes.  page_size a power of two, 16 or more.  window 0: everything.  Rows with seq_len < 0 get zeros.
+struct Kv8AttnCall {
+  const void *q, *k_codes, *v_codes;
+  const float *k_scale, *v_scale;
+  const int *table, *seq_lens, *slots;
+  float* part;
+  void* out;
+  int* status;
+  cudaStream_t stream;
+  long long q_row, q_head;
+  int dtype, pages, page_size, table_rows, max_blocks, B, Hq, Hk, D, window, part_words;
+  float scale;
+};
+TRLB_API int trlb_kv8_decode_attn(const Kv8AttnCall* call) {
+  const Kv8AttnCall c = *call;
+  if (c.B == 0) return 0;
+  if (c.Hk <= 0 || c.Hq <= 0 || c.Hq % c.Hk || c.B > KA_MAX_SEQS || c.window < 0) return -2;
+  if (c.page_size < KA_STEP || (c.page_size & (c.page_size - 1))) return -3;
+  if ((long long)c.pages * c.Hk > 2147483647ll) return -5;
+  if (c.part_words < trlb_kv8_attn_scratch(0, c.Hq, c.Hk, c.D)) return -7;
   int shift = 0;
-  while ((1 << shift) < page_size) ++shift;
-  if ((long long)pages * Hk > 2147483647ll) return -5;
-  Kv8AttnArgs a{{}, {}, q, q_row, q_head, k_scale, v_scale, table, seq_lens, slots,
-                out, part, nullptr, nullptr, status, pages, Hk, Hq / Hk, 1, shift, table_rows, max_blocks, B, window, 1, scale};
-  if (dtype == 0) return kv8_attn_pick<__nv_bfloat16>(a, k_codes, v_codes, D, st);
-  if (dtype == 1) return kv8_attn_pick<__half>(a, k_codes, v_codes, D, st);
+  while ((1 << shift) < c.page_size) ++shift;
+  Kv8AttnArgs a{{}, {}, c.q, c.q_row, c.q_head, c.k_scale, c.v_scale, c.table, c.seq_lens, c.slots, c.out, c.part, nullptr,
+                nullptr, c.status, c.pages, c.Hk, c.Hq / c.Hk, 1, shift, c.table_rows, c.max_blocks, c.B, c.window, 1, c.scale};
+  if (c.dtype == 0) return kv8_attn_pick<__nv_bfloat16>(a, c.k_codes, c.v_codes, c.D, c.stream);
+  if (c.dtype == 1) return kv8_attn_pick<__half>(a, c.k_codes, c.v_codes, c.D, c.stream);
   return -4;
 }

@@ -1,26 +1,29 @@
 // Sampling with temperature, top-k, top-p and min-p from one random word per row.
 //
 //   z = logit / max(temperature, 1e-6); NaN counts as -inf, +inf as the largest finite value
-//   top-k keeps z >= the k-th largest (equals of the k-th too); 0 keeps all
+//   top-k keeps what is at least the k-th largest logit (equals of the k-th too); 0 keeps all
 //   top-p keeps, most likely first and the lower column first among equals, each token before which at most
 //         top_p of the mass of what top-k kept stands
 //   min-p keeps z >= max z + log(min_p)
 //   token = argmax over what is kept of z - log(-log u), u = (hash(word of the row, column) + 1/2) / 2^32; of z where
 //   temperature is 0; its log-probability is that in the distribution over what is kept
 //
-// All filters are one border: the last token kept, in the order "larger z, then lower column".  A row is read by the blocks
-// of a cluster.  What bounds it is the row's bytes, which stay in the second-level cache after the first pass, and the
-// latency of the few exchanges between the blocks; so the border is found in as few passes as the row allows:
-//   1. the maximum;
-//   2. a histogram of max z - z in steps of 1/64 and the mass; from counts alone the bins bound the mass above each of them
-//      from both sides, which brackets the border;
-//   3. the tokens of the bracket (and of all bins above, where they are few) are listed and sorted by one block, which finds
-//      the border exactly.  Where the list holds every kept token it draws the token, too;
-//   4. otherwise a last pass over the row sums what is kept and draws.
-// A bracket with too many tokens for the list is cut again by histograms over the keys' bits.
-// Counts are integers and sums are taken in a fixed order, so results do not depend on timing.
+// All filters are one border: the last token kept, in the order "larger logit, then lower column".  A row is read by the blocks
+// of a cluster.  What bounds it is the work per logit (the row's bytes stay in the second-level cache after the first pass) and
+// the latency of the few exchanges between the blocks; so logits are compared undivided, and the border is found in as few
+// passes as the row allows:
+//   1. the maximum and the mass, each thread with a running maximum of its own;
+//   2. candidates for the kept tokens: with top-k what is not below the k-th largest of the threads' maxima (k logits are at
+//      least that large), with top-p alone what is not lighter than (1 - top_p) mass / V (lighter ones together are less than
+//      what top-p leaves out).  Where one block's list holds them, it finds the border there and draws: done.
+//   3. otherwise a histogram of the distances to the maximum.  From counts alone the bins bound the mass above each of them from
+//      both sides, which brackets the border; the tokens of the bracket are listed, and the exact mass above it says which of
+//      them is the last.  A bracket with too many tokens for the list is cut again by histograms over the logits' bits.
+//   4. a last pass over the row draws among what is kept.
+// Counts and the sums over lists are integers, other sums are taken in a fixed order: results do not depend on timing.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
+#include <cstddef>
 
 #include "common.cuh"
 
@@ -28,11 +31,15 @@ namespace cg = cooperative_groups;
 
 namespace trlb {
 
-constexpr int SF_THREADS = 1024, SF_WARPS = SF_THREADS / 32;
-constexpr int SF_BINS = 2048;      // histogram bins; bin SF_BINS holds what lies further below
-constexpr int SF_LIST = 4096;      // tokens that the list holds
-constexpr float SF_STEP = 64.f;    // bins per unit of z
+constexpr int SF_THREADS = 512, SF_WARPS = SF_THREADS / 32;  // two blocks an SM
+constexpr int SF_EACH = 4;         // bins of a thread: SF_BINS / SF_THREADS
+constexpr int SF_BINS = 2048;      // histogram bins; the last one holds all that lies further below
+constexpr int SF_LIST = 8192;      // tokens that the list holds
+constexpr int SF_CUT = 2048;       // and the cut around the border; more are sorted in the list itself
+constexpr int SF_BATCH = 16;       // logits that a thread loads at once
 constexpr float SF_MAX = 3.4028234663852886e38f;
+constexpr float SF_LOG2E = 1.4426950408889634f;
+constexpr double SF_UNIT = 17592186044416.;  // 2^44: weights in sums over lists are whole multiples of 1 / SF_UNIT
 
 struct SampleArgs {
   const void* logits;
@@ -53,17 +60,21 @@ __device__ __forceinline__ uint32_t sf_hash(uint32_t x) {
   x ^= x >> 16; x *= 0x7feb352dU; x ^= x >> 15; x *= 0x846ca68bU; x ^= x >> 16;
   return x;
 }
+// The random bits of a column: u = (h + 1/2) / 2^32.
+__device__ __forceinline__ uint32_t sf_bits(uint32_t word, uint32_t col) {
+  return sf_hash(sf_hash(word ^ sf_hash(col * 0x85EBCA6BU + 0x165667B1U)) + col);
+}
 // -log(-log u): both halves of (0, 1) in the form that keeps their precision
-__device__ __forceinline__ float sf_gumbel(uint32_t word, uint32_t col) {
-  const uint32_t h = sf_hash(sf_hash(word ^ sf_hash(col * 0x85EBCA6BU + 0x165667B1U)) + col);
+__device__ __noinline__ float sf_gumbel(uint32_t h) {
   float e;
   if (h & 0x80000000u) e = -log1pf(-((float)(~h) + 0.5f) * 2.3283064365386963e-10f);
   else e = -logf(((float)h + 0.5f) * 2.3283064365386963e-10f);
   return -logf(e);
 }
+__device__ __forceinline__ float sf_quotient(float x, float t) { return fminf(__fdiv_rn(x, t), SF_MAX); }
 // Orders floats as unsigned integers.
-__device__ __forceinline__ uint32_t sf_key(float z) {
-  const uint32_t u = __float_as_uint(z);
+__device__ __forceinline__ uint32_t sf_key(float x) {
+  const uint32_t u = __float_as_uint(x);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float sf_unkey(uint32_t k) {
@@ -94,50 +105,78 @@ __device__ __forceinline__ void sf_unpack<__half>(uint4 u, float* x) {
   }
 }
 
-// NaN counts as -inf; + 0 makes one zero of both, so that their bits are equal, too
-__device__ __forceinline__ float sf_z(float x, float T) {
-  const float z = __fdiv_rn(x, T);
-  return z != z ? -INFINITY : fminf(z, SF_MAX) + 0.f;
-}
-
 struct SfShared {
   unsigned hist[SF_BINS];
-  unsigned long long list[SF_LIST];  // ~key << 32 | column: ascending is "larger z, then lower column"
+  unsigned long long list[SF_LIST];   // ~key << 32 | column: ascending is "larger logit, then lower column"
+  unsigned long long cut[SF_CUT];     // the part of the list around the border
   double red[3][SF_WARPS];
-  double mass;                       // this block's share of a sum
+  unsigned long long sum[SF_WARPS];
+  unsigned long long weights[SF_THREADS];
+  double mass, first_mass;            // this block's shares of sums
+  double kept;                        // mass down to the border, 0: unknown
   float fmax;
-  unsigned kmin, kmax, list_n;
-  int bin_lo, bin_hi;                // the bracket, its tokens and those above it: the same in every block
+  unsigned kmin, kmax, list_n, cut_n;
+  int bin_lo, bin_hi;                 // the bracket, its tokens and those above it: the same in every block
   unsigned above, upto;
-  float border_z;                    // written by the first block, read by all
+  float border;                       // written by the first block, read by all
   int border_col;
-  float best;                        // this block's draw
+  float best;                         // this block's draw
   int best_col;
   float best_z;
 };
+// the table is read four bins at a time
+static_assert(offsetof(SfShared, hist) % 16 == 0, "bins on 16 bytes");
 
+// A block's columns of a row.
 template <typename T>
 struct SfRow {
   const T* x;
-  int v0, v1;       // this block's columns
+  int v0, v1;
   bool vec;
-  float temperature;
-  // f(z, column) over the block's columns
+  float cap;  // logits from here on are equals: their quotients by the temperature are not finite
+  // NaN -> -inf (fmaxf drops it); one zero of both
+  __device__ __forceinline__ float clean(float y) const { return fminf(fmaxf(y, -INFINITY), cap) + 0.f; }
+  // f(logit, column) over the block's columns, until stop() says so
+  template <typename F, typename G>
+  __device__ __forceinline__ void each(F f, G stop) const {
+    constexpr int N = 16 / sizeof(T);
+    int i = v0 + threadIdx.x;
+    if (vec) {
+      constexpr int U = SF_BATCH / N;
+      const int n1 = v1 / N;  // v0 is a multiple of N
+#pragma unroll 1
+      for (int at = v0 / N + threadIdx.x; at < n1; at += U * SF_THREADS) {
+        if (stop()) return;
+        uint4 u[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+          if (at + j * SF_THREADS < n1) u[j] = reinterpret_cast<const uint4*>(x)[at + j * SF_THREADS];
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+          if (at + j * SF_THREADS >= n1) break;
+          float y[N];
+          sf_unpack<T>(u[j], y);
+#pragma unroll
+          for (int k = 0; k < N; ++k) f(clean(y[k]), (at + j * SF_THREADS) * N + k);
+        }
+      }
+      i = n1 * N + threadIdx.x;
+    }
+#pragma unroll 1
+    for (; i < v1; i += SF_THREADS) {
+      if (stop()) return;
+      f(clean(sf_load(x, i)), i);
+    }
+  }
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
-    constexpr int N = 16 / sizeof(T);
-    if (vec) {
-      const int n0 = v0 / N, n1 = v1 / N;  // v0 is a multiple of N
-      for (int i = n0 + threadIdx.x; i < n1; i += SF_THREADS) {
-        float y[N];
-        sf_unpack<T>(reinterpret_cast<const uint4*>(x)[i], y);
-#pragma unroll
-        for (int k = 0; k < N; ++k) f(sf_z(y[k], temperature), i * N + k);
-      }
-      for (int i = n1 * N + threadIdx.x; i < v1; i += SF_THREADS) f(sf_z(sf_load(x, i), temperature), i);
-    } else {
-      for (int i = v0 + threadIdx.x; i < v1; i += SF_THREADS) f(sf_z(sf_load(x, i), temperature), i);
-    }
+    each(f, [] { return false; });
+  }
+  // The same, small instead of fast: for what rows hardly ever need.
+  template <typename F>
+  __device__ __forceinline__ void each_slowly(F f) const {
+#pragma unroll 1
+    for (int i = v0 + threadIdx.x; i < v1; i += SF_THREADS) f(clean(sf_load(x, i)), i);
   }
 };
 
@@ -149,6 +188,16 @@ __device__ __forceinline__ double sf_block_sum(double v, SfShared& s) {
   __syncthreads();
   double all = 0.;
   for (int w = 0; w < SF_WARPS; ++w) all += s.red[0][w];
+  return all;
+}
+__device__ __forceinline__ unsigned long long sf_block_count(unsigned long long v, SfShared& s) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) s.sum[threadIdx.x >> 5] = v;
+  __syncthreads();
+  unsigned long long all = 0;
+  for (int w = 0; w < SF_WARPS; ++w) all += s.sum[w];
   return all;
 }
 // Inclusive prefixes over the threads of a block.
@@ -172,25 +221,25 @@ __device__ __forceinline__ void sf_block_prefix(double (&v)[N], SfShared& s) {
     for (int n = 0; n < N; ++n) v[n] += s.red[n][w];
 }
 
-// Sorts the first n entries of the list ascending (n <= SF_LIST).
-__device__ void sf_sort(SfShared& s, int n) {
+// Sorts n entries ascending; `at` has room for the next power of two.
+__device__ void sf_sort(unsigned long long* at, int n) {
   int size = 2;
   while (size < n) size <<= 1;
-  for (int i = n + threadIdx.x; i < size; i += SF_THREADS) s.list[i] = ~0ull;
+  for (int i = n + threadIdx.x; i < size; i += SF_THREADS) at[i] = ~0ull;
   __syncthreads();
   for (int k = 2; k <= size; k <<= 1)
     for (int j = k >> 1; j > 0; j >>= 1) {
       for (int i = threadIdx.x; i < size / 2; i += SF_THREADS) {
         const int a = 2 * i - (i & (j - 1)), b = a + j;
-        const unsigned long long x = s.list[a], y = s.list[b];
-        if ((x > y) == ((a & k) == 0)) { s.list[a] = y; s.list[b] = x; }
+        const unsigned long long x = at[a], y = at[b];
+        if ((x > y) == ((a & k) == 0)) { at[a] = y; at[b] = x; }
       }
       __syncthreads();
     }
 }
-__device__ __forceinline__ float sf_list_z(unsigned long long e) { return sf_unkey(~(unsigned)(e >> 32)); }
+__device__ __forceinline__ float sf_entry_x(unsigned long long e) { return sf_unkey(~(unsigned)(e >> 32)); }
 
-// Draw and log-probability from the blocks' (or threads') parts: the larger key, then the lower column.
+// The better of two draws: the larger key, then the lower column; col < 0: none.
 __device__ __forceinline__ void sf_better(float& best, int& col, float& z, float ob, int oc, float oz) {
   if (oc >= 0 && (col < 0 || ob > best || (ob == best && oc < col))) { best = ob; col = oc; z = oz; }
 }
@@ -218,15 +267,29 @@ struct SfSampler {
   const SampleArgs& a;
   SfRow<T> r;
   int C, rank, row, tid;
-  float zmax;
+  float temperature, c;   // c: of a logit's distance to the maximum, the exponent of 2
+  float xmax, zmax;
+  float step;             // bins of the linear histogram per unit of the logits
   uint32_t word;
   bool greedy;
   SfShared* lead;
 
   __device__ __forceinline__ SfShared* of(int c) { return cluster.map_shared_rank(&s, c); }
-  __device__ __forceinline__ float weight(float z) const { return expf(z - zmax); }
-  __device__ __forceinline__ float key_of(float z, int col) const { return greedy ? z : z + sf_gumbel(word, (uint32_t)col); }
-  __device__ __forceinline__ int linear_bin(float z) const { return (int)fminf((zmax - z) * SF_STEP, (float)(SF_BINS - 1)); }
+  // What a pass needs of a row, by value: it stays in registers where the members of this object do not.
+  struct Pass {
+    SfRow<T> r;
+    float xmax, c, step;
+    __device__ __forceinline__ float weight(float x) const { return exp2f((x - xmax) * c); }
+    __device__ __forceinline__ int linear_bin(float x) const { return (int)fminf((xmax - x) * step, (float)(SF_BINS - 1)); }
+  };
+  __device__ __forceinline__ Pass pass() const { return {r, xmax, c, step}; }
+  __device__ __forceinline__ float weight(float x) const { return exp2f((x - xmax) * c); }
+  __device__ __forceinline__ float quotient(float x) const { return sf_quotient(x, temperature); }
+  // Bins that reach down to `from`, where that is not too far.
+  __device__ __forceinline__ void set_step(float from) {
+    const float far = (xmax - from) / temperature;
+    step = (far < 31.f ? (float)(SF_BINS - 2) / fmaxf(far, 1e-3f) : 64.f) / temperature;
+  }
 
   // Sum of a block-wide value over the cluster, in the order of the blocks.  Ends with a barrier.
   __device__ double cluster_sum(double v) {
@@ -234,7 +297,7 @@ struct SfSampler {
     if (tid == 0) s.mass = v;
     cluster.sync();
     double all = 0.;
-    for (int c = 0; c < C; ++c) all += of(c)->mass;
+    for (int b = 0; b < C; ++b) all += of(b)->mass;
     cluster.sync();
     return all;
   }
@@ -242,127 +305,291 @@ struct SfSampler {
     for (int i = tid; i < SF_BINS; i += SF_THREADS) s.hist[i] = 0;
     __syncthreads();
   }
-  // This thread's two bins of the whole row.
-  __device__ void merged_bins(unsigned (&n)[2]) {
+  // This thread's bins of the whole row.
+  __device__ void merged_bins(unsigned (&n)[SF_EACH]) {
     cluster.sync();
-    n[0] = n[1] = 0;
-    for (int c = 0; c < C; ++c) {
-      n[0] += of(c)->hist[2 * tid];
-      n[1] += of(c)->hist[2 * tid + 1];
+#pragma unroll
+    for (int i = 0; i < SF_EACH; ++i) n[i] = 0;
+    for (int b = 0; b < C; ++b) {
+      const uint4 x = reinterpret_cast<const uint4*>(of(b)->hist)[tid];
+      n[0] += x.x;
+      n[1] += x.y;
+      n[2] += x.z;
+      n[3] += x.w;
     }
     cluster.sync();
   }
+  // Those of this block.
+  __device__ void own_bins(unsigned (&n)[SF_EACH]) {
+    __syncthreads();
+    const uint4 x = reinterpret_cast<const uint4*>(s.hist)[tid];
+    n[0] = x.x;
+    n[1] = x.y;
+    n[2] = x.z;
+    n[3] = x.w;
+    __syncthreads();
+  }
   // The bin of the k-th token of the histogram.
-  __device__ void bracket_count(const unsigned (&n)[2], unsigned k) {
-    double v[1] = {(double)n[0] + n[1]};
+  __device__ __noinline__ void bracket_count(const unsigned (&n)[SF_EACH], unsigned k) {
+    const unsigned own = n[0] + n[1] + n[2] + n[3];
+    double v[1] = {(double)own};
     sf_block_prefix(v, s);
-    const unsigned upto = (unsigned)v[0], below = upto - n[0] - n[1];
-    if (below < k && k <= upto) {
-      const bool first = k <= below + n[0];
-      s.bin_lo = s.bin_hi = 2 * tid + (first ? 0 : 1);
-      s.above = below + (first ? 0 : n[0]);
-      s.upto = below + n[0] + (first ? 0 : n[1]);
+    unsigned below = (unsigned)v[0] - own;
+#pragma unroll
+    for (int i = 0; i < SF_EACH; ++i) {
+      if (below < k && k <= below + n[i]) {
+        s.bin_lo = s.bin_hi = SF_EACH * tid + i;
+        s.above = below;
+        s.upto = below + n[i];
+      }
+      below += n[i];
     }
     __syncthreads();
   }
   // Bins between which the mass passes `goal`: the first whose upper bound of the mass up to it does, to the first whose
   // lower bound does.  hi / lo: bounds of a token's weight in this thread's bins; mass: what stands above the histogram.
-  __device__ void bracket_mass(const unsigned (&n)[2], const float (&hi)[2], const float (&lo)[2], double mass, double goal) {
+  __device__ __noinline__ void bracket_mass(const unsigned (&n)[SF_EACH], const float (&hi)[SF_EACH], const float (&lo)[SF_EACH], double mass, double goal) {
     if (tid == 0) {
       s.bin_lo = s.bin_hi = SF_BINS - 1;
       s.above = s.upto = 0;
     }
-    double v[3] = {(double)n[0] + n[1], (n[0] * (double)hi[0] + n[1] * (double)hi[1]) * 1.00001,
-                   (n[0] * (double)lo[0] + n[1] * (double)lo[1]) * 0.99999};
-    const double own_hi = v[1], own_lo = v[2];
-    sf_block_prefix(v, s);
-    const unsigned below = (unsigned)v[0] - n[0] - n[1];
-    double up = mass + (v[1] - own_hi), low = mass + (v[2] - own_lo);  // bounds before this thread's bins
-    unsigned cnt = below;
+    double v[3] = {0., 0., 0.};
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const double up1 = up + n[i] * (double)hi[i] * 1.00001, low1 = low + n[i] * (double)lo[i] * 0.99999;
-      if (up1 > goal) atomicMin(&s.bin_lo, 2 * tid + i);
-      if (low1 > goal) atomicMin(&s.bin_hi, 2 * tid + i);
-      up = up1;
-      low = low1;
+    for (int i = 0; i < SF_EACH; ++i) {
+      v[0] += n[i];
+      v[1] += n[i] * (double)hi[i] * 1.00001;
+      v[2] += n[i] * (double)lo[i] * 0.99999;
+    }
+    const double own[3] = {v[0], v[1], v[2]};
+    sf_block_prefix(v, s);
+    unsigned cnt = (unsigned)(v[0] - own[0]);
+    double up = mass + (v[1] - own[1]), low = mass + (v[2] - own[2]);  // bounds before this thread's bins
+#pragma unroll
+    for (int i = 0; i < SF_EACH; ++i) {
+      up += n[i] * (double)hi[i] * 1.00001;
+      low += n[i] * (double)lo[i] * 0.99999;
+      if (up > goal) atomicMin(&s.bin_lo, SF_EACH * tid + i);
+      if (low > goal) atomicMin(&s.bin_hi, SF_EACH * tid + i);
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (2 * tid + i == s.bin_lo) s.above = cnt;
+    for (int i = 0; i < SF_EACH; ++i) {
+      if (SF_EACH * tid + i == s.bin_lo) s.above = cnt;
       cnt += n[i];
-      if (2 * tid + i == s.bin_hi) s.upto = cnt;
-      s.hist[2 * tid + i] = cnt;  // from here on: tokens up to and with a bin
+      if (SF_EACH * tid + i == s.bin_hi) s.upto = cnt;
+      s.hist[SF_EACH * tid + i] = cnt;  // from here on: tokens up to and with a bin
     }
     __syncthreads();
   }
-  // Lists the row's tokens that `in` takes in the first block, sorted; returns their number (to all blocks).
+  // Bounds of a weight in this thread's bins of the linear histogram.
+  __device__ void linear_bounds(float (&hi)[SF_EACH], float (&lo)[SF_EACH]) const {
+#pragma unroll
+    for (int i = 0; i < SF_EACH; ++i) {
+      const int bin = SF_EACH * tid + i;
+      hi[i] = exp2f(-(float)bin / step * c);
+      lo[i] = bin == SF_BINS - 1 ? 0.f : exp2f(-(float)(bin + 1) / step * c);
+    }
+  }
+  // Bounds of a weight in this thread's bins of the histogram of keys from `top` down over `span`.
+  __device__ void key_bounds(float (&hi)[SF_EACH], float (&lo)[SF_EACH], unsigned top, unsigned span, int shift) const {
+#pragma unroll
+    for (int i = 0; i < SF_EACH; ++i) {
+      const unsigned bin = (unsigned)(SF_EACH * tid + i);
+      hi[i] = lo[i] = 0.f;
+      if (bin <= span >> shift) {
+        hi[i] = weight(sf_unkey(top - (bin << shift)));
+        lo[i] = weight(sf_unkey(top - min((bin << shift) + ((1u << shift) - 1u), span)));
+      }
+    }
+  }
+  // Lists the row's tokens that `in` takes in the first block, in no order; returns their number, 0 where the list is too short.
   template <typename F>
-  __device__ int gather(F in) {
+  __device__ __forceinline__ int gather(F in) {
     if (tid == 0) s.list_n = 0;
     __syncthreads();
-    r.each([&](float z, int col) {
-      if (in(z)) {
-        const unsigned i = atomicAdd(&s.list_n, 1u);
-        if (i < SF_LIST) s.list[i] = (unsigned long long)(~sf_key(z)) << 32 | (unsigned)col;
-      }
-    });
+    {
+      SfShared& sh = s;
+      const SfRow<T> q = r;
+      q.each(
+          [&](float x, int col) {
+            if (in(x)) {
+              const unsigned i = atomicAdd(&sh.list_n, 1u);
+              if (i < SF_LIST) sh.list[i] = (unsigned long long)(~sf_key(x)) << 32 | (unsigned)col;
+            }
+          },
+          [&] { return *reinterpret_cast<volatile unsigned*>(&sh.list_n) > SF_LIST; });
+    }
+    return collect();
+  }
+  // The blocks' lists in the first one.
+  __device__ __noinline__ int collect() {
     cluster.sync();
     int n = 0;
-    for (int c = 0; c < C; ++c) {
-      const int m = min((int)of(c)->list_n, SF_LIST - n);
-      if (rank == 0 && c > 0) {
-        const unsigned long long* from = of(c)->list;
-        for (int i = tid; i < m; i += SF_THREADS) s.list[n + i] = from[i];
-      }
-      n += m;
-    }
+    for (int b = 0; b < C; ++b) n += (int)of(b)->list_n;
+    if (n > SF_LIST) return 0;
     if (rank == 0) {
+      int at = (int)s.list_n;
+      for (int b = 1; b < C; ++b) {
+        const int m = (int)of(b)->list_n;
+        const unsigned long long* from = of(b)->list;
+        for (int i = tid; i < m; i += SF_THREADS) s.list[at + i] = from[i];
+        at += m;
+      }
       __syncthreads();
-      sf_sort(s, n);
     }
     return n;
   }
-  // The sorted list's last entry before which at most `goal` of mass stands, `mass` of it above the list.
-  __device__ int last_within(int n, double mass, double goal) {
-    constexpr int E = SF_LIST / SF_THREADS;
-    double v[1] = {0.}, w[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int i = tid * E + e;
-      w[e] = i < n ? (double)weight(sf_list_z(s.list[i])) : 0.;
-      v[0] += w[e];
+
+  // ---- the first block alone: borders in its list of n tokens -----------------------------------------------------------
+  __device__ __forceinline__ unsigned long long whole(double w) const { return (unsigned long long)(w * SF_UNIT + 0.5); }
+  // The border among n <= SF_THREADS entries in no order, `above` tokens and `mass` above them, a thread an entry: it counts and
+  // weighs the entries before its own.
+  __device__ __noinline__ void small_border(const unsigned long long* at, int n, bool by_mass, double goal, unsigned above, double mass) {
+    const unsigned long long mine = tid < n ? at[tid] : 0;
+    const unsigned long long own = tid < n && by_mass ? whole((double)weight(sf_entry_x(mine))) : 0;
+    if (tid == 0) s.bin_lo = -1;
+    if (tid < n) s.weights[tid] = own;
+    __syncthreads();
+    int rank_here = 0;
+    unsigned long long before = 0;
+    if (tid < n) {
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) {
+        if (at[j] < mine) {
+          ++rank_here;
+          before += s.weights[j];
+        }
+      }
+      if (by_mass) {
+        if (mass + (double)before / SF_UNIT <= goal) atomicMax(&s.bin_lo, rank_here);
+      } else if (above + rank_here + 1 == (unsigned)goal) {
+        s.border = sf_entry_x(mine);
+        s.border_col = 0x7fffffff;
+        s.kept = 0.;
+      }
     }
+    __syncthreads();
+    if (by_mass && tid < n && rank_here == max(0, s.bin_lo)) {
+      s.border = sf_entry_x(mine);
+      s.border_col = (int)(unsigned)mine;
+      s.kept = mass + (double)(before + own) / SF_UNIT;
+    }
+    __syncthreads();
+  }
+  // The border among n entries that are sorted.
+  __device__ __noinline__ void sorted_border(const unsigned long long* at, int n, bool by_mass, double goal, unsigned above, double mass) {
+    if (!by_mass) {
+      if (tid == 0) {
+        s.border = sf_entry_x(at[(unsigned)goal - above - 1]);
+        s.border_col = 0x7fffffff;
+        s.kept = 0.;
+      }
+      __syncthreads();
+      return;
+    }
+    constexpr int E = SF_LIST / SF_THREADS;
+    double v[1] = {0.};
+    for (int e = 0; e < E; ++e) v[0] += tid * E + e < n ? (double)weight(sf_entry_x(at[tid * E + e])) : 0.;
     const double own = v[0];
     sf_block_prefix(v, s);
     if (tid == 0) s.bin_lo = 0;
     __syncthreads();
     double before = mass + (v[0] - own);
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int i = tid * E + e;
-      if (i < n && before <= goal) atomicMax(&s.bin_lo, i);
-      before += w[e];
+    for (int e = 0; e < E && tid * E + e < n; ++e) {
+      if (before <= goal) atomicMax(&s.bin_lo, tid * E + e);
+      before += (double)weight(sf_entry_x(at[tid * E + e]));
     }
     __syncthreads();
-    return s.bin_lo;
+    const int last = s.bin_lo;
+    before = mass + (v[0] - own);
+    for (int e = 0; e < E && tid * E + e < n; ++e) {
+      before += (double)weight(sf_entry_x(at[tid * E + e]));
+      if (tid * E + e == last) {
+        s.kept = before;
+        s.border = sf_entry_x(at[last]);
+        s.border_col = (int)(unsigned)at[last];
+      }
+    }
+    __syncthreads();
   }
-  // Sums and draws over the first n list entries with z >= floor.  First block only.
-  __device__ void finish_list(int n, float floor) {
-    double mass = 0.;
+  // The border in the list of n tokens, `above` of them and `mass` above it: the last token before which at most `goal` of mass
+  // stands (by_mass), or the goal-th token and its equals.  Leaves s.border, s.border_col and s.kept (0: unknown).
+  __device__ __noinline__ void list_border(int n, bool by_mass, double goal, unsigned above, double mass) {
+    if (n <= SF_THREADS) {
+      small_border(s.list, n, by_mass, goal, above, mass);
+      return;
+    }
+    unsigned lo = 0xffffffffu, hi = 0u;
+    for (int i = tid; i < n; i += SF_THREADS) {
+      const unsigned k = ~(unsigned)(s.list[i] >> 32);
+      lo = min(lo, k);
+      hi = max(hi, k);
+    }
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    if (tid == 0) { s.kmin = 0xffffffffu; s.kmax = 0u; s.cut_n = 0; }
+    clear_hist();
+    if ((tid & 31) == 0) { atomicMin(&s.kmin, lo); atomicMax(&s.kmax, hi); }
+    __syncthreads();
+    lo = s.kmin;
+    hi = s.kmax;
+    int shift = 0;
+    while (((hi - lo) >> shift) >= SF_BINS) ++shift;
+    for (int i = tid; i < n; i += SF_THREADS) atomicAdd(&s.hist[(hi - ~(unsigned)(s.list[i] >> 32)) >> shift], 1u);
+    unsigned cnt[SF_EACH];
+    own_bins(cnt);
+    if (by_mass) {
+      float wh[SF_EACH], wl[SF_EACH];
+      key_bounds(wh, wl, hi, hi - lo, shift);
+      bracket_mass(cnt, wh, wl, mass, goal);
+    } else {
+      bracket_count(cnt, (unsigned)goal - above);
+    }
+    const unsigned b0 = (unsigned)s.bin_lo, b1 = (unsigned)s.bin_hi, a0 = s.above, around = s.upto - s.above;
+    __syncthreads();
+    if (around > SF_CUT) {  // (nearly) equals: in place
+      sf_sort(s.list, n);
+      sorted_border(s.list, n, by_mass, goal, above, mass);
+      return;
+    }
+    unsigned long long before = 0;
+    for (int i = tid; i < n; i += SF_THREADS) {
+      const unsigned long long e = s.list[i];
+      const unsigned bin = (hi - ~(unsigned)(e >> 32)) >> shift;
+      if (bin >= b0 && bin <= b1) s.cut[atomicAdd(&s.cut_n, 1u)] = e;
+      else if (bin < b0 && by_mass) before += whole((double)weight(sf_entry_x(e)));
+    }
+    if (by_mass) mass += (double)sf_block_count(before, s) / SF_UNIT;
+    __syncthreads();
+    const int m = (int)s.cut_n;
+    above += a0;
+    if (m <= SF_THREADS) {
+      small_border(s.cut, m, by_mass, goal, above, mass);
+    } else {
+      sf_sort(s.cut, m);
+      sorted_border(s.cut, m, by_mass, goal, above, mass);
+    }
+  }
+  static __device__ __forceinline__ bool within(float x, int col, float border, int border_col) {
+    return x > border || (x == border && col <= border_col);
+  }
+  // Sums and draws over the list's tokens down to the border and at least `floor`.
+  __device__ __noinline__ void finish_list(int n, float border, int border_col, float floor) {
+    unsigned long long sum = 0;
     float best = -INFINITY, best_z = 0.f;
     int col = -1;
     for (int i = tid; i < n; i += SF_THREADS) {
       const unsigned long long e = s.list[i];
-      const float z = sf_list_z(e);
-      if (z < floor) continue;
-      mass += (double)weight(z);
-      sf_better(best, col, best_z, key_of(z, (int)(unsigned)e), (int)(unsigned)e, z);
+      const float x = sf_entry_x(e);
+      const int at = (int)(unsigned)e;
+      if (x < floor || !within(x, at, border, border_col)) continue;
+      const float z = quotient(x);
+      sum += whole((double)expf(z - zmax));
+      sf_better(best, col, best_z, greedy ? z : z + sf_gumbel(sf_bits(word, (uint32_t)at)), at, z);
     }
-    mass = sf_block_sum(mass, s);
+    sum = sf_block_count(sum, s);
     sf_block_best(best, col, best_z, s);
-    write(best_z, col, mass);
+    write(best_z, col, (double)sum / SF_UNIT);
   }
   __device__ void write(float z, int col, double mass) {
     if (tid == 0) {
@@ -371,40 +598,51 @@ struct SfSampler {
     }
   }
 
-  // The border of top-k (by_mass false: goal is k) or top-p (goal is p) among the tokens with z >= floor.  Returns the number
-  // of entries of the first block's list if that holds every token down to the border's bin, else 0 and the border.
-  __device__ int search(bool by_mass, double goal, float floor, float& border_z, int& border_col, double& total) {
+  // ---- all blocks ----------------------------------------------------------------------------------------------------
+  // What the first block found, for every block.
+  __device__ __noinline__ void share_border(float& border, int& border_col, double& kept) {
+    cluster.sync();
+    border = lead->border;
+    border_col = lead->border_col;
+    kept = lead->kept;
+    cluster.sync();
+  }
+  // The border of top-k (by_mass false: goal is a number of tokens) or top-p (goal is a mass) among the tokens that are at least
+  // `floor`; with floor_mass the goal is that share of their mass.  Returns the number of entries of the first block's list if
+  // that holds every token down to the border's bin (and sets goal), else 0 and the border; kept: the mass down to it, if known.
+  __device__ __noinline__ int search(bool by_mass, double& goal, bool floor_mass, float floor, float& border, int& border_col, double& kept) {
+    kept = 0.;
+    set_step(floor);
     clear_hist();
     float part = 0.f;
-    r.each([&](float z, int) {
-      if (z >= floor && z > -INFINITY) {
-        atomicAdd(&s.hist[linear_bin(z)], 1u);
-        part += weight(z);
-      }
-    });
-    total = cluster_sum((double)part);
-    unsigned n[2];
+    const Pass q = pass();
+    {
+      unsigned* hist = s.hist;
+      const float from = fmaxf(floor, -SF_MAX);
+      q.r.each([&](float x, int) {
+        if (x >= from) {
+          atomicAdd(&hist[q.linear_bin(x)], 1u);
+          if (floor_mass) part += q.weight(x);
+        }
+      });
+    }
+    if (floor_mass) goal *= cluster_sum((double)part);
+    unsigned n[SF_EACH];
     merged_bins(n);
-    double limit = 0.;
+    const double limit = goal;
     if (by_mass) {
-      limit = fmax(0., goal * total);
-      float hi[2], lo[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int bin = 2 * tid + i;
-        hi[i] = expf(-(float)bin / SF_STEP);
-        lo[i] = bin == SF_BINS - 1 ? 0.f : expf(-(float)(bin + 1) / SF_STEP);
-      }
+      float hi[SF_EACH], lo[SF_EACH];
+      linear_bounds(hi, lo);
       bracket_mass(n, hi, lo, 0., limit);
     } else {
-      double all[1] = {(double)n[0] + n[1]};
+      double all[1] = {(double)n[0] + n[1] + n[2] + n[3]};
       sf_block_prefix(all, s);
       if (tid == SF_THREADS - 1) s.upto = (unsigned)all[0];
       __syncthreads();
       const unsigned finite = s.upto;
       __syncthreads();
       if (goal > (double)finite) {  // fewer tokens than k: all are kept
-        border_z = -INFINITY;
+        border = -INFINITY;
         border_col = 0x7fffffff;
         return 0;
       }
@@ -413,22 +651,36 @@ struct SfSampler {
     const int b0 = s.bin_lo, b1 = s.bin_hi;
     unsigned above = s.above, upto = s.upto;
     __syncthreads();
-    if (upto <= SF_LIST)
-      return gather([&](float z) { return z >= floor && z > -INFINITY && linear_bin(z) <= b1; });
-    auto member = [&](float z) {
-      if (!(z >= floor && z > -INFINITY)) return false;
-      const int b = linear_bin(z);
-      return b >= b0 && b <= b1;
+    const float from = fmaxf(floor, -SF_MAX);
+    if (upto <= SF_LIST) return gather([&](float x) { return x >= from && q.linear_bin(x) <= b1; });
+    auto member = [&](float x) {
+      const int b = q.linear_bin(x);
+      return x >= from && b >= b0 && b <= b1;
     };
+    auto over = [&](float x) { return x >= -SF_MAX && q.linear_bin(x) < b0; };
+    double mass = 0.;
+    part = 0.f;
+    if (upto - above <= SF_LIST) {
+      const int m = gather([&](float x) {
+        const int b = q.linear_bin(x);
+        if (by_mass && b < b0) part += q.weight(x);
+        return x >= from && b >= b0 && b <= b1;
+      });
+      if (by_mass) mass = cluster_sum((double)part);
+      if (rank == 0) {
+        list_border(m, by_mass, limit, above, mass);
+      }
+      share_border(border, border_col, kept);
+      return 0;
+    }
     // keys of the bracket, and the mass above it
     unsigned kmin = 0xffffffffu, kmax = 0u;
-    part = 0.f;
-    r.each([&](float z, int) {
-      if (member(z)) {
-        kmin = min(kmin, sf_key(z));
-        kmax = max(kmax, sf_key(z));
-      } else if (z > -INFINITY && linear_bin(z) < b0) {
-        part += weight(z);
+    r.each_slowly([&](float x, int) {
+      if (member(x)) {
+        kmin = min(kmin, sf_key(x));
+        kmax = max(kmax, sf_key(x));
+      } else if (over(x)) {
+        part += weight(x);
       }
     });
     kmin = __reduce_min_sync(0xffffffffu, kmin);
@@ -436,45 +688,36 @@ struct SfSampler {
     if (tid == 0) { s.kmin = 0xffffffffu; s.kmax = 0u; }
     __syncthreads();
     if ((tid & 31) == 0) { atomicMin(&s.kmin, kmin); atomicMax(&s.kmax, kmax); }
-    double mass = cluster_sum((double)part);  // its barriers show kmin and kmax, too
-    for (int c = 0; c < C; ++c) {
-      kmin = min(kmin, of(c)->kmin);
-      kmax = max(kmax, of(c)->kmax);
+    mass = cluster_sum((double)part);  // its barriers show kmin and kmax, too
+    for (int b = 0; b < C; ++b) {
+      kmin = min(kmin, of(b)->kmin);
+      kmax = max(kmax, of(b)->kmax);
     }
     cluster.sync();
-    // all tokens with keys in [kmin, kmax] are the bracket's: the bins are intervals of z.  Each turn leaves an interval of
-    // one bin's width, so there are three at most.
+    // All tokens with keys in [kmin, kmax] are the bracket's: the bins are intervals of the logits.  Each turn leaves an
+    // interval of one bin's width, so there are three at most.
     while (upto - above > SF_LIST && kmin < kmax) {
       int shift = 0;
       while (((kmax - kmin) >> shift) >= SF_BINS) ++shift;
       const unsigned top = kmax, span = kmax - kmin;
       clear_hist();
-      r.each([&](float z, int) {
-        const unsigned k = sf_key(z);
+      r.each_slowly([&](float x, int) {
+        const unsigned k = sf_key(x);
         if (k >= kmin && k <= top) atomicAdd(&s.hist[(top - k) >> shift], 1u);
       });
       merged_bins(n);
       unsigned c0, c1, a0, a1;  // the bracket's bins; tokens of the interval above it, and up to its end
       if (by_mass) {
-        float hi[2], lo[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const unsigned bin = (unsigned)(2 * tid + i);
-          hi[i] = lo[i] = 0.f;
-          if (bin <= span >> shift) {
-            hi[i] = weight(sf_unkey(top - (bin << shift)));
-            const unsigned down = (bin << shift) + ((1u << shift) - 1u);
-            lo[i] = weight(sf_unkey(top - min(down, span)));
-          }
-        }
+        float hi[SF_EACH], lo[SF_EACH];
+        key_bounds(hi, lo, top, span, shift);
         bracket_mass(n, hi, lo, mass, limit);
         c0 = (unsigned)s.bin_lo, c1 = (unsigned)s.bin_hi, a0 = s.above, a1 = s.upto;
         __syncthreads();
         auto between = [&](unsigned from, unsigned to) {  // exact mass of a run of bins
           float sum = 0.f;
-          r.each([&](float z, int) {
-            const unsigned k = sf_key(z);
-            if (k >= kmin && k <= top && (top - k) >> shift >= from && (top - k) >> shift <= to) sum += weight(z);
+          r.each_slowly([&](float x, int) {
+            const unsigned k = sf_key(x);
+            if (k >= kmin && k <= top && (top - k) >> shift >= from && (top - k) >> shift <= to) sum += weight(x);
           });
           return cluster_sum((double)sum);
         };
@@ -503,38 +746,29 @@ struct SfSampler {
       above += a0;
     }
     if (upto - above <= SF_LIST) {
-      const int m = gather([&](float z) { const unsigned k = sf_key(z); return k >= kmin && k <= kmax; });
+      const int m = gather([&](float x) { const unsigned k = sf_key(x); return k >= kmin && k <= kmax; });
       if (rank == 0) {
-        int at;
-        if (by_mass) at = last_within(m, mass, limit);
-        else at = (int)((unsigned)goal - above) - 1;
-        if (tid == 0) {
-          s.border_z = sf_list_z(s.list[at]);
-          s.border_col = by_mass ? (int)(unsigned)s.list[at] : 0x7fffffff;
-        }
+        list_border(m, by_mass, limit, above, mass);
       }
-      cluster.sync();
-      border_z = lead->border_z;
-      border_col = lead->border_col;
-      cluster.sync();
+      share_border(border, border_col, kept);
       return 0;
     }
     // more equals than the list holds
-    border_z = sf_unkey(kmax);
+    border = sf_unkey(kmax);
     border_col = 0x7fffffff;
     if (by_mass) {
-      const double w = (double)weight(border_z), equals = (double)(upto - above);
+      const double w = (double)weight(border), equals = (double)(upto - above);
       const double fit = w > 0. ? ::floor((limit - mass) / w) + 1. : equals;  // how many of them are kept
       if (fit < equals) border_col = column_of(kmax, (unsigned)fmax(1., fit));
     }
     return 0;
   }
   // The column of the n-th token (in the order of the columns, from 1) whose key is `key`.
-  __device__ int column_of(unsigned key, unsigned n) {
+  __device__ __noinline__ int column_of(unsigned key, unsigned n) {
     int width = (a.V + SF_BINS - 1) / SF_BINS;
     clear_hist();
-    r.each([&](float z, int col) { if (sf_key(z) == key) atomicAdd(&s.hist[col / width], 1u); });
-    unsigned m[2];
+    r.each_slowly([&](float x, int col) { if (sf_key(x) == key) atomicAdd(&s.hist[col / width], 1u); });
+    unsigned m[SF_EACH];
     merged_bins(m);
     bracket_count(m, n);
     const int bin = s.bin_lo;
@@ -544,8 +778,8 @@ struct SfSampler {
       const int lo = bin * width, hi = min(a.V, lo + width);
       unsigned count = before;
       int found = hi - 1;
-      for (int c = lo; c < hi; ++c)
-        if (sf_key(sf_z(sf_load(r.x, c), r.temperature)) == key && ++count == n) { found = c; break; }
+      for (int i = lo; i < hi; ++i)
+        if (sf_key(r.clean(sf_load(r.x, i))) == key && ++count == n) { found = i; break; }
       s.border_col = found;
     }
     cluster.sync();
@@ -558,75 +792,176 @@ struct SfSampler {
     const float top_p = a.top_p ? a.top_p[row] : a.top_p_all, min_p = a.min_p ? a.min_p[row] : a.min_p_all;
     const int top_k = a.top_k ? a.top_k[row] : a.top_k_all;
     const bool by_k = top_k > 0 && top_k < a.V, by_p = top_p < 1.f;
-    float mx = -INFINITY;
-    r.each([&](float z, int) { mx = fmaxf(mx, z); });
-    mx = warp_max(mx);
+    // ---- the maximum, and the mass relative to each thread's own ----
+    float mine = -INFINITY, part = 0.f;
+    {
+      const SfRow<T> q = r;
+      const float k = c;
+      q.each([&](float x, int) {
+        if (x > mine) {  // rare after the first few
+          part *= exp2f((mine - x) * k);  // 0 at first: exp2(-inf)
+          mine = x;
+        }
+        if (x >= -SF_MAX) part += exp2f((x - mine) * k);
+      });
+    }
+    float mx = warp_max(mine);
     if ((tid & 31) == 0) s.red[0][tid >> 5] = mx;
     __syncthreads();
+    mx = (float)s.red[0][0];
+    for (int w = 1; w < SF_WARPS; ++w) mx = fmaxf(mx, (float)s.red[0][w]);
+    const double sum = sf_block_sum(mine == -INFINITY ? 0. : (double)(part * exp2f((mine - mx) * c)), s);
     if (tid == 0) {
-      for (int w = 0; w < SF_WARPS; ++w) mx = fmaxf(mx, (float)s.red[0][w]);
       s.fmax = mx;
+      s.first_mass = sum;
     }
     cluster.sync();
-    zmax = -INFINITY;
-    for (int c = 0; c < C; ++c) zmax = fmaxf(zmax, of(c)->fmax);
-    if (zmax == -INFINITY) {  // nothing to draw from
+    xmax = -INFINITY;
+    for (int b = 0; b < C; ++b) xmax = fmaxf(xmax, of(b)->fmax);
+    if (xmax == -INFINITY) {  // nothing to draw from
       if (rank == 0 && tid == 0) { a.tok[row] = 0; a.logp[row] = -INFINITY; }
       return;
     }
-    float floor = -INFINITY;  // min-p, as the smallest value that it keeps
-    if (min_p > 0.f) floor = fminf(zmax, __double2float_ru((double)zmax + log((double)min_p)));
-    float bz = -INFINITY;
-    int bc = 0x7fffffff;
+    zmax = quotient(xmax);
     double total = 0.;
+    for (int b = 0; b < C; ++b)
+      if (of(b)->fmax > -INFINITY) total += of(b)->first_mass * (double)exp2f((of(b)->fmax - xmax) * c);
+    float floor = -INFINITY;  // min-p, as the smallest logit that it keeps
+    if (min_p > 0.f) {
+      const double least = (double)zmax + log((double)min_p);
+      floor = fminf(xmax, (float)(least * (double)temperature));
+      // the quotients, rounded, decide: at most a few logits around the product are on its wrong side
+      for (int i = 0; i < 8 && (double)quotient(nextafterf(floor, -INFINITY)) >= least; ++i) floor = nextafterf(floor, -INFINITY);
+      for (int i = 0; i < 8 && (double)quotient(floor) < least && floor < xmax; ++i) floor = nextafterf(floor, INFINITY);
+      floor = fminf(floor, xmax);
+    }
+    float border = -INFINITY;
+    int border_col = 0x7fffffff;
+    double kept = 0.;
     if (by_k) {
-      const int n = search(false, (double)top_k, -INFINITY, bz, bc, total);
+      int n = 0;
+      if (top_k <= C * SF_THREADS) {
+        // the bin of the k-th largest of the threads' maxima: at least k tokens lie in it or above
+        step = 64.f / temperature;
+        clear_hist();
+        if (mine > -INFINITY) atomicAdd(&s.hist[pass().linear_bin(mine)], 1u);
+        unsigned h[SF_EACH];
+        merged_bins(h);
+        if (tid == 0) s.bin_lo = SF_BINS;
+        __syncthreads();
+        bracket_count(h, (unsigned)top_k);
+        const int last = s.bin_lo;
+        __syncthreads();
+        if (last < SF_BINS - 1) {
+          const float from = fmaxf(-SF_MAX, xmax - (float)(last + 1) / step * 1.000001f);  // a little below the bin's end
+          n = gather([&](float x) { return x >= from; });
+        }
+      }
+      double goal = (double)top_k;
+      if (n == 0) n = search(false, goal, false, -INFINITY, border, border_col, kept);
       if (n > 0) {
         if (rank == 0) {
-          const float zk = sf_list_z(s.list[top_k - 1]);
-          double count = 0.;  // the k-th and its equals
-          for (int i = tid; i < n; i += SF_THREADS) count += sf_list_z(s.list[i]) >= zk;
-          int kept = (int)sf_block_sum(count, s);
+          list_border(n, false, (double)top_k, 0, 0.);
+          border = s.border;
           if (by_p) {
-            double mass = 0.;
-            for (int i = tid; i < kept; i += SF_THREADS) mass += (double)weight(sf_list_z(s.list[i]));
-            mass = sf_block_sum(mass, s);
-            kept = last_within(kept, 0., fmax(0., (double)top_p * mass)) + 1;
+            // of the k-th and its equals, which move to the front
+            __syncthreads();
+            if (tid == 0) s.list_n = 0;
+            constexpr int E = SF_LIST / SF_THREADS;
+            unsigned long long e[E], w = 0;
+#pragma unroll
+            for (int i = 0; i < E; ++i) e[i] = tid + i * SF_THREADS < n ? s.list[tid + i * SF_THREADS] : ~0ull;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < E; ++i)
+              if (tid + i * SF_THREADS < n && sf_entry_x(e[i]) >= border) {
+                w += whole((double)weight(sf_entry_x(e[i])));
+                s.list[atomicAdd(&s.list_n, 1u)] = e[i];
+              }
+            const double mass = (double)sf_block_count(w, s) / SF_UNIT;
+            n = (int)s.list_n;
+            list_border(n, true, fmax(0., (double)top_p * mass), 0, 0.);
           }
-          finish_list(kept, floor);
+          finish_list(n, s.border, s.border_col, floor);
         }
         return;
       }
     }
     if (by_p) {
-      const int n = search(true, (double)top_p, bz, bz, bc, total);
+      int n = 0;
+      double goal = fmax(0., (double)top_p * total);
+      float from = border;
+      if (by_k) {
+        goal = fmax(0., (double)top_p);
+      } else {
+        // lighter tokens than this together have less than what top-p leaves out; a little is added for the sums' rounding
+        const double least = (1. - (double)top_p - 2e-5) * total / a.V;
+        if (least > 0.) from = fmaxf(-SF_MAX, xmax + ((float)log(least) - 1e-3f) * temperature);
+        // weights are at most 1: at least `goal` tokens are kept, and with many of them come more than the list holds
+        if (least > 0. && goal < SF_LIST / 16) n = gather([&](float x) { return x >= from; });
+      }
+      if (n == 0) n = search(true, goal, by_k, from, border, border_col, kept);
       if (n > 0) {
-        if (rank == 0) finish_list(last_within(n, 0., fmax(0., (double)top_p * total)) + 1, floor);
+        if (rank == 0) {
+          list_border(n, true, goal, 0, 0.);
+          finish_list(n, s.border, s.border_col, floor);
+        }
         return;
       }
     }
-    if (floor > bz) { bz = floor; bc = 0x7fffffff; }
-    float part = 0.f, best = -INFINITY, best_z = 0.f;
-    int col = -1;
-    r.each([&](float z, int c) {
-      if (z == -INFINITY || z < bz || (z == bz && c > bc)) return;
-      part += weight(z);
-      const float k = key_of(z, c);
-      if (col < 0 || k > best || (k == best && c < col)) { best = k; col = c; best_z = z; }
-    });
-    const double mass = cluster_sum((double)part);
-    sf_block_best(best, col, best_z, s);
-    if (tid == 0) { s.best = best; s.best_col = col; s.best_z = best_z; }
-    cluster.sync();
-    if (rank == 0) {
-      for (int c = 1; c < C; ++c) sf_better(best, col, best_z, of(c)->best, of(c)->best_col, of(c)->best_z);
-      write(best_z, col, mass);
+    const bool all = border == -INFINITY && floor == -INFINITY;  // then the mass is known
+    if (floor > border) { border = floor; border_col = 0x7fffffff; kept = 0.; }
+    // ---- what is kept: its mass, and the draw ----
+    double mass = all ? total : kept;
+    if (mass == 0.) {
+      part = 0.f;
+      const Pass q = pass();
+      const float last = border;
+      const int last_col = border_col;
+      q.r.each([&](float x, int col) {
+        if (within(x, col, last, last_col) && x >= -SF_MAX) part += q.weight(x);
+      });
+      mass = cluster_sum((double)part);
     }
+    // The largest z - log(-log u) of n tokens is lse + a Gumbel variate, which is below lse - 3 once in 10^8 rows.  A token
+    // reaches K = lse - 3 only if -log u <= exp(z - K), and -log u >= 1 - u: most are out after their random bits.
+    float best = -INFINITY, best_z = 0.f;
+    int col = -1;
+    for (int turn = 0; turn < 2 && col < 0; ++turn) {
+      const Pass q = pass();
+      const float reach = turn == 1 ? INFINITY : (float)(4294967296. * 20.0855369 * 1.001 / mass), last = fmaxf(border, -SF_MAX), t = temperature;
+      const int last_col = border == -INFINITY ? 0x7fffffff : border_col;
+      const uint32_t w = word;
+      const bool most = greedy;
+      float top = -INFINITY, top_z = 0.f;
+      int at = -1;
+      q.r.each([&](float x, int i) {
+        if (!within(x, i, last, last_col)) return;
+        float z = x, k = x;
+        if (!most) {
+          const uint32_t h = sf_bits(w, (uint32_t)i);
+          if ((float)(~h) > reach * q.weight(x)) return;
+          z = sf_quotient(x, t);
+          k = z + sf_gumbel(h);
+        }
+        if (at < 0 || k > top || (k == top && i < at)) { top = k; at = i; top_z = z; }
+      });
+      best = top;
+      best_z = top_z;
+      col = at;
+      if (greedy && col >= 0) best_z = quotient(best_z);
+      sf_block_best(best, col, best_z, s);
+      if (tid == 0) { s.best = best; s.best_col = col; s.best_z = best_z; }
+      cluster.sync();
+      for (int b = 0; b < C; ++b) sf_better(best, col, best_z, of(b)->best, of(b)->best_col, of(b)->best_z);
+      cluster.sync();
+    }
+    if (rank == 0) write(best_z, col, mass);
   }
 };
 
 template <typename T>
-__global__ void __launch_bounds__(SF_THREADS, 1)
+__global__ void __launch_bounds__(SF_THREADS, 2)
 sample_filtered_kernel(const __grid_constant__ SampleArgs a) {
   extern __shared__ __align__(16) unsigned char raw[];
   cg::cluster_group cluster = cg::this_cluster();
@@ -641,7 +976,9 @@ sample_filtered_kernel(const __grid_constant__ SampleArgs a) {
   f.r.v1 = rank == C - 1 ? a.V : min(a.V / N * N, (rank + 1) * per);
   f.r.vec = (reinterpret_cast<uintptr_t>(f.r.x) & 15) == 0;
   const float temp = a.temperature ? a.temperature[row] : a.temperature_all;
-  f.r.temperature = fmaxf(temp, 1e-6f);
+  f.temperature = fminf(fmaxf(temp, 1e-6f), 1e37f);
+  f.c = SF_LOG2E / f.temperature;
+  f.r.cap = SF_MAX * fminf(f.temperature, 1.f);
   f.greedy = !(temp > 0.f);
   f.word = a.words ? a.words[row] : a.seed ^ sf_hash((a.step_ptr ? (uint32_t)*a.step_ptr : 0u) * 0x9E3779B9U + (uint32_t)row);
   f.C = C;
@@ -655,9 +992,9 @@ sample_filtered_kernel(const __grid_constant__ SampleArgs a) {
 
 template <typename T>
 int sample_filtered_launch(const SampleArgs& a, int B, cudaStream_t st) {
-  // blocks a row: as many as give every SM one, up to the 8 of a portable cluster
+  // blocks a row: up to two an SM, and up to the 8 of a portable cluster
   int C = 1;
-  while (C < 8 && 2 * C * B <= trlb_host::sm_count()) C *= 2;
+  while (C < 8 && C * B <= trlb_host::sm_count()) C *= 2;
   const size_t smem = sizeof(SfShared);
   cudaError_t e = cudaFuncSetAttribute(sample_filtered_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return (int)e;
@@ -681,18 +1018,31 @@ int sample_filtered_launch(const SampleArgs& a, int B, cudaStream_t st) {
 
 using namespace trlb;
 
-// dtype: 0 bf16, 1 fp16, 2 fp32.  Per-row parameters may be null, then the scalar beside them holds for every row.
-// words null: the random word of a row is made of seed, *step_ptr and the row, as trlb_sample makes it.
-TRLB_API int trlb_sample_filtered(const void* logits, int dtype, long long row_stride, int B, int V, const float* temperature,
-                                  float temperature_all, const int* top_k, int top_k_all, const float* top_p, float top_p_all,
-                                  const float* min_p, float min_p_all, const unsigned* words, unsigned seed,
-                                  const int* step_ptr, int* tok, float* logp, cudaStream_t st) {
-  if (B == 0) return 0;
-  if (V < 1 || B < 0 || B > (1 << 27)) return -1;
-  SampleArgs a{logits, row_stride, V, temperature, top_p, min_p, top_k, temperature_all, top_p_all, min_p_all, top_k_all, words,
-               seed, step_ptr, tok, logp};
-  if (dtype == 0) return sample_filtered_launch<__nv_bfloat16>(a, B, st);
-  if (dtype == 1) return sample_filtered_launch<__half>(a, B, st);
-  if (dtype == 2) return sample_filtered_launch<float>(a, B, st);
+// dtype: 0 bf16, 1 fp16, 2 fp32.  Per-row parameters may be null, then the number for all rows holds.  words null: the random
+// word of a row is made of seed, *step_ptr and the row, as trlb_sample makes it.
+struct SampleCall {
+  const void* logits;
+  const float* temperature;
+  const int* top_k;
+  const float *top_p, *min_p;
+  const uint32_t* words;
+  const int* step_ptr;
+  int* tok;
+  float* logp;
+  cudaStream_t stream;
+  long long row_stride;
+  int dtype, B, V, top_k_all, unused;
+  uint32_t seed;
+  float temperature_all, top_p_all, min_p_all;
+};
+TRLB_API int trlb_sample_filtered(const SampleCall* call) {
+  const SampleCall c = *call;
+  if (c.B == 0) return 0;
+  if (c.V < 1 || c.B < 0 || c.B > (1 << 27)) return -1;
+  SampleArgs a{c.logits, c.row_stride, c.V, c.temperature, c.top_p, c.min_p, c.top_k, c.temperature_all, c.top_p_all, c.min_p_all,
+               c.top_k_all, c.words, c.seed, c.step_ptr, c.tok, c.logp};
+  if (c.dtype == 0) return sample_filtered_launch<__nv_bfloat16>(a, c.B, c.stream);
+  if (c.dtype == 1) return sample_filtered_launch<__half>(a, c.B, c.stream);
+  if (c.dtype == 2) return sample_filtered_launch<float>(a, c.B, c.stream);
   return -2;
 }

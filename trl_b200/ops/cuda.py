@@ -9,6 +9,7 @@ from __future__ import annotations
 import os
 
 import ctypes
+import struct
 from ctypes import c_float, c_int, c_longlong, c_void_p
 
 import torch
@@ -1095,172 +1096,242 @@ def allreduce_add_rmsnorm(arena, byte_offset, buf_elems, res, w, eps, sync, out=
 # 8-bit paged cache (csrc/kv8.cu, csrc/kv8_attn.cu) and filtered sampling (csrc/sample_filtered.cu)
 # -------------------------------------------------------------------------------------------
 _KV8_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_TYPES = {"p": c_void_p, "i": c_int, "l": c_longlong, "f": c_float, "u": ctypes.c_uint, "s": ctypes.c_char_p}
+_bound: dict = {}
 
 
-def _same_device(dev, **tensors):
+def _fn(name, types, result=c_int):
+    """An entry of the kernel library whose argument types are set once, so that calls pass plain numbers.  Entries that take
+    some twenty arguments read them from one packed structure ("s"): these operators run in decode loops, where converting
+    the arguments one by one would take longer than the kernel."""
+    f = _bound.get(name)
+    if f is None:
+        f = getattr(lib(), name)
+        f.argtypes, f.restype = [_TYPES[c] for c in types], result
+        _bound[name] = f
+    return f
+
+
+_raw_stream, _device_now = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _launch(index, fn, what, *args):
+    """``fn(*args)`` with the device ``index`` current."""
+    if _device_now() == index:
+        rc = fn(*args)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args)
+    _chk(rc, what)
+
+
+def _status_ptr(index):
+    s = _status.get(index)
+    return (status_buffer(torch.device("cuda", index)) if s is None else s).data_ptr()
+
+
+def _same_device(index, **tensors):
     for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, expected {dev}")
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"{name} is on {t.device}, not where the other tensors are")
 
 
 def _want_i32(t, name):
-    if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
+    if t.dtype != torch.int32 or not t.is_contiguous():
         raise ValueError(f"{name} has to be a contiguous int32 tensor")
-    return t
 
 
 def _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table):
-    """(pages, heads, page size, head dim) of a cache as :func:`functional.kv8_alloc` makes it."""
-    pages, heads, page, dim = k_cache.shape
-    if v_cache.shape != k_cache.shape or k_cache.dtype != torch.float8_e4m3fn or v_cache.dtype != torch.float8_e4m3fn:
+    """(pages, heads, page size, head dim, device) of a cache as :func:`functional.kv8_alloc` makes it."""
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape or k_cache.dtype != torch.float8_e4m3fn or v_cache.dtype != torch.float8_e4m3fn:
         raise ValueError("the codes of keys and values are float8_e4m3fn tensors [pages, heads, page size, head dim] of one shape")
+    pages, heads, page, dim = shape
     if page < 16 or page & (page - 1) or dim not in (64, 96, 128, 256):
         raise ValueError(f"page sizes are powers of two from 16 on and head dims 64, 96, 128 or 256, not {page} and {dim}")
-    for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if s.shape != (pages, heads) or s.dtype != torch.float32:
-            raise ValueError(f"{name} has to be fp32 [pages, heads] = [{pages}, {heads}]")
-    if not all(t.is_contiguous() and t.data_ptr() % 16 == 0 for t in (k_cache, v_cache)) or not (k_scale.is_contiguous() and v_scale.is_contiguous()):
+    if k_scale.shape != shape[:2] or v_scale.shape != shape[:2] or k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+        raise ValueError(f"k_scale and v_scale have to be fp32 [pages, heads] = [{pages}, {heads}]")
+    if (k_cache.data_ptr() | v_cache.data_ptr()) & 15 or not (k_cache.is_contiguous() and v_cache.is_contiguous()
+                                                              and k_scale.is_contiguous() and v_scale.is_contiguous()):
         raise ValueError("the tensors of an 8-bit cache have to be contiguous, the codes on 16 bytes")
     if block_table.dim() != 2:
         raise ValueError("block_table has to be [rows, blocks]")
     _want_i32(block_table, "block_table")
-    _same_device(k_cache.device, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, block_table=block_table)
-    return pages, heads, page, dim
+    index = k_cache.get_device()
+    if not index == v_cache.get_device() == k_scale.get_device() == v_scale.get_device() == block_table.get_device():
+        raise ValueError("the tensors of an 8-bit cache and the block table have to be on one device")
+    return pages, heads, page, dim, index
 
 
 def _kv8_rows(t, name, heads, dim):
     """[tokens, heads, dim] with dense rows on 16 bytes."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim:
-        raise ValueError(f"{name} has to be [tokens, {heads}, {dim}], not {tuple(t.shape)}")
-    per = 16 // t.element_size()
-    if t.stride(2) != 1 or t.stride(0) % per or t.stride(1) % per or t.data_ptr() % 16:
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim:
+        raise ValueError(f"{name} has to be [tokens, {heads}, {dim}], not {tuple(shape)}")
+    a, b, c = t.stride()
+    mask = 16 // t.element_size() - 1
+    if c != 1 or (a | b) & mask or t.data_ptr() & 15:
         t = t.contiguous()
     return t
 
 
+_KV8_APPEND = struct.Struct("12P4q10i")
+
+
 def kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, starts, *, cu_seqlens=None, slots=None, max_new=None):
     """See :func:`functional.kv8_append`."""
-    pages, heads, page, dim = _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table)
-    if k.dtype != v.dtype or k.dtype not in _KV8_DTYPES or k.shape != v.shape:
+    pages, heads, page, dim, index = _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table)
+    dtype = _KV8_DTYPES.get(k.dtype)
+    if dtype is None or k.dtype != v.dtype or k.shape != v.shape:
         raise ValueError("k and v have to be bf16, fp16 or fp32 tensors of one type and shape")
     k, v = _kv8_rows(k, "k", heads, dim), _kv8_rows(v, "v", heads, dim)
     tokens, n = k.shape[0], starts.shape[0]
-    _same_device(k_cache.device, k=k, v=v, starts=starts, cu_seqlens=cu_seqlens, slots=slots)
-    _want_i32(starts, "starts"), _want_i32(cu_seqlens, "cu_seqlens"), _want_i32(slots, "slots")
-    if cu_seqlens is None and tokens != n:
-        raise ValueError(f"without cu_seqlens every sequence has one new token: {tokens} tokens for {n} sequences")
-    if cu_seqlens is not None and cu_seqlens.shape != (n + 1,):
-        raise ValueError(f"cu_seqlens has to be [{n + 1}]")
-    if slots is not None and slots.shape != (n,):
-        raise ValueError(f"slots has to be [{n}]")
-    if slots is None and n > block_table.shape[0]:
-        raise ValueError(f"{n} sequences for a block table of {block_table.shape[0]} rows")
+    rows, blocks = block_table.shape
+    _want_i32(starts, "starts")
+    if not index == k.get_device() == v.get_device() == starts.get_device():
+        raise ValueError("k, v and starts have to be where the cache is")
+    if cu_seqlens is None:
+        if tokens != n:
+            raise ValueError(f"without cu_seqlens every sequence has one new token: {tokens} tokens for {n} sequences")
+    else:
+        _want_i32(cu_seqlens, "cu_seqlens")
+        _same_device(index, cu_seqlens=cu_seqlens)
+        if cu_seqlens.shape != (n + 1,):
+            raise ValueError(f"cu_seqlens has to be [{n + 1}]")
+    if slots is None:
+        if n > rows:
+            raise ValueError(f"{n} sequences for a block table of {rows} rows")
+    else:
+        _want_i32(slots, "slots")
+        _same_device(index, slots=slots)
+        if slots.shape != (n,):
+            raise ValueError(f"slots has to be [{n}]")
     max_new = tokens if max_new is None else int(max_new)
     if tokens == 0 or n == 0:
         return
     if max_new < 1:
         raise ValueError("max_new is the largest number of new tokens of a sequence: at least 1")
-    with torch.cuda.device(k_cache.device):
-        _chk(lib().trlb_kv8_append(_p(k), _p(v), c_int(_KV8_DTYPES[k.dtype]), c_longlong(k.stride(0)), c_longlong(k.stride(1)),
-                                   c_longlong(v.stride(0)), c_longlong(v.stride(1)), _p(k_cache), _p(v_cache), _p(k_scale),
-                                   _p(v_scale), c_int(pages), c_int(heads), c_int(page), c_int(dim), _p(block_table),
-                                   c_int(block_table.shape[0]), c_int(block_table.shape[1]), _p(starts), _p(cu_seqlens),
-                                   _p(slots), c_int(n), c_int(tokens), c_int(min(max_new, tokens)),
-                                   _p(status_buffer(k_cache.device)), _s()), "kv8_append")
+    k_tok, k_head, _ = k.stride()
+    v_tok, v_head, _ = v.stride()
+    call = _KV8_APPEND.pack(k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+                            v_scale.data_ptr(), block_table.data_ptr(), starts.data_ptr(), _ptr(cu_seqlens), _ptr(slots),
+                            _status_ptr(index), _raw_stream(index), k_tok, k_head, v_tok, v_head, dtype, pages, heads, page,
+                            dim, rows, blocks, n, tokens, min(max_new, tokens))
+    _launch(index, _fn("trlb_kv8_append", "s"), "kv8_append", call)
 
 
 def kv8_rope_append(qkv, bias, q_norm, k_norm, norm_eps, seq_lens, slot_ids, block_table, q_out, k_cache, v_cache, k_scale,
                     v_scale, Hq, theta, pos_delta=None):
     """:func:`rope_kv_write` (``qkv`` bf16) or :func:`rope_kv_write_f32` (``qkv`` fp32 sums, cleared) into an 8-bit cache."""
-    pages, heads, page, dim = _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table)
+    pages, heads, page, dim, index = _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table)
     B = qkv.shape[0]
     f32 = qkv.dtype == torch.float32
     if dim > 128 or (not f32 and qkv.dtype != torch.bfloat16) or qkv.stride(1) != 1 or qkv.shape[1] != (Hq + 2 * heads) * dim:
         raise ValueError("qkv has to be dense rows of bf16 or fp32 for heads of at most 128 values")
     if not f32 and bias is not None:
         raise ValueError("a bias belongs to fp32 sums: a bf16 row has it already")
-    with torch.cuda.device(k_cache.device):
-        _chk(lib().trlb_kv8_rope_append(_p(qkv), c_int(int(f32)), c_longlong(qkv.stride(0)), _p(bias), _p(q_norm), _p(k_norm),
-                                        c_float(norm_eps), _p(seq_lens), _p(slot_ids), _p(block_table),
-                                        c_int(block_table.shape[0]), c_int(block_table.shape[1]), _p(q_out), _p(k_cache),
-                                        _p(v_cache), _p(k_scale), _p(v_scale), c_int(pages), c_int(heads), c_int(page),
-                                        c_int(dim), c_int(B), c_int(Hq), c_float(theta), _p(pos_delta),
-                                        _p(status_buffer(k_cache.device)), _s()), "kv8_rope_append")
+    _launch(index, _fn("trlb_kv8_rope_append", "pilpppfpppiipppppiiiiiifppp"), "kv8_rope_append", qkv.data_ptr(), int(f32),
+            qkv.stride(0), _ptr(bias), _ptr(q_norm), _ptr(k_norm), norm_eps, seq_lens.data_ptr(), _ptr(slot_ids),
+            block_table.data_ptr(), *block_table.shape, q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            k_scale.data_ptr(), v_scale.data_ptr(), pages, heads, page, dim, B, Hq, theta, _ptr(pos_delta), _status_ptr(index),
+            _raw_stream(index))
+
+
+_KV8_ATTN = struct.Struct("12P2q11if")
 
 
 def kv8_decode_attn(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, scale, *, slots=None, window=None, out=None):
     """See :func:`functional.kv8_decode_attn`."""
-    pages, heads, page, dim = _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table)
-    if q.dtype not in (torch.bfloat16, torch.float16) or q.dim() != 3 or q.shape[2] != dim or q.shape[1] % heads or q.shape[1] == 0:
-        raise ValueError(f"q has to be bf16 or fp16 [sequences, a multiple of {heads} heads, {dim}], not {q.dtype} {tuple(q.shape)}")
-    B, Hq, _ = q.shape
+    pages, heads, page, dim, index = _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table)
+    shape = q.shape
+    if len(shape) != 3 or q.dtype not in (torch.bfloat16, torch.float16) or shape[2] != dim or shape[1] % heads or shape[1] == 0:
+        raise ValueError(f"q has to be bf16 or fp16 [sequences, a multiple of {heads} heads, {dim}], not {q.dtype} {tuple(shape)}")
+    B, Hq, _ = shape
     if B > 4096:
         raise ValueError("at most 4096 sequences a call")
-    if q.stride(2) != 1 or q.stride(0) % 4 or q.stride(1) % 4 or q.data_ptr() % 8:
+    a, b, c = q.stride()
+    if c != 1 or (a | b) & 3 or q.data_ptr() & 7:
         q = q.contiguous()
-    _same_device(k_cache.device, q=q, seq_lens=seq_lens, slots=slots, out=out)
-    _want_i32(seq_lens, "seq_lens"), _want_i32(slots, "slots")
-    if slots is None and B > min(block_table.shape[0], seq_lens.shape[0]):
-        raise ValueError(f"{B} sequences for {block_table.shape[0]} rows of the block table and {seq_lens.shape[0]} lengths")
-    if slots is not None and (slots.shape != (B,) or seq_lens.shape[0] < block_table.shape[0]):
-        raise ValueError(f"slots has to be [{B}], with a length for every row of the block table")
+        a, b, c = q.stride()
+    rows, blocks = block_table.shape
+    _want_i32(seq_lens, "seq_lens")
+    if not index == q.get_device() == seq_lens.get_device():
+        raise ValueError("q and seq_lens have to be where the cache is")
+    if slots is None:
+        if B > min(rows, seq_lens.shape[0]):
+            raise ValueError(f"{B} sequences for {rows} rows of the block table and {seq_lens.shape[0]} lengths")
+    else:
+        _want_i32(slots, "slots")
+        _same_device(index, slots=slots)
+        if slots.shape != (B,) or seq_lens.shape[0] < rows:
+            raise ValueError(f"slots has to be [{B}], with a length for every row of the block table")
     if window is not None and window < 1:
         raise ValueError("a window sees at least the newest token")
     if out is None:
-        out = torch.empty(B, Hq, dim, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
-        raise ValueError("out has to be contiguous, of the shape and type of q")
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    elif out.shape != shape or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() & 15 or out.get_device() != index:
+        raise ValueError("out has to be contiguous, on 16 bytes, of the shape, type and device of q")
     if B == 0:
         return out
-    L = lib()
-    L.trlb_kv8_attn_scratch.restype = c_longlong
-    with torch.cuda.device(q.device):
-        # scratch of this call alone: calls on other streams, and graphs, have their own
-        part = torch.empty(L.trlb_kv8_attn_scratch(c_int(Hq), c_int(heads), c_int(dim)), dtype=torch.float32, device=q.device)
-        _chk(L.trlb_kv8_decode_attn(_p(q), c_int(_KV8_DTYPES[q.dtype]), c_longlong(q.stride(0)), c_longlong(q.stride(1)),
-                                    _p(k_cache), _p(v_cache), _p(k_scale), _p(v_scale), c_int(pages), c_int(page),
-                                    _p(block_table), c_int(block_table.shape[0]), c_int(block_table.shape[1]), _p(seq_lens),
-                                    _p(slots), c_int(B), c_int(Hq), c_int(heads), c_int(dim), c_float(scale),
-                                    c_int(min(window or 0, 2**31 - 1)), _p(part), _p(out), _p(status_buffer(q.device)), _s()),
-             "kv8_decode_attn")
+    # scratch of this call alone: calls on other streams, and graphs, have their own
+    part = torch.empty(_fn("trlb_kv8_attn_scratch", "iiii", c_longlong)(index, Hq, heads, dim), dtype=torch.float32, device=q.device)
+    call = _KV8_ATTN.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                          block_table.data_ptr(), seq_lens.data_ptr(), _ptr(slots), part.data_ptr(), out.data_ptr(),
+                          _status_ptr(index), _raw_stream(index), a, b, _KV8_DTYPES[q.dtype], pages, page, rows, blocks, B, Hq,
+                          heads, dim, min(window or 0, 2**31 - 1), part.numel(), scale)
+    _launch(index, _fn("trlb_kv8_decode_attn", "s"), "kv8_decode_attn", call)
     return out
 
 
-def _per_row(x, name, B, dtype, device):
+def _per_row(x, name, B, dtype, index):
     """(tensor or None, number): a sampling parameter that is one number for all rows or one per row."""
-    if torch.is_tensor(x):
-        if x.shape != (B,):
-            raise ValueError(f"{name} has to be a number or a tensor [{B}], not {tuple(x.shape)}")
-        _same_device(device, **{name: x})
-        return x.to(dtype).contiguous(), 0
-    return None, x
+    if not isinstance(x, torch.Tensor):
+        return None, x
+    if x.shape != (B,):
+        raise ValueError(f"{name} has to be a number or a tensor [{B}], not {tuple(x.shape)}")
+    if x.get_device() != index:
+        raise ValueError(f"{name} is on {x.device}, not where the logits are")
+    return (x if x.dtype == dtype and x.is_contiguous() else x.to(dtype).contiguous()), 0
+
+
+_SAMPLE_FILTERED = struct.Struct("10Pq5iI3f")
 
 
 def sample_filtered(logits, rng=None, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, seed=0, step_ptr=None, out_tok=None,
                     out_logp=None):
     """See :func:`functional.sample_filtered`.  Without ``rng`` the rows' random words are made of ``seed``, ``step_ptr`` and
     the row, as :func:`sample_tokens` makes them."""
-    if logits.dim() != 2 or logits.dtype not in _KV8_DTYPES or logits.shape[1] < 1:
-        raise ValueError(f"logits have to be bf16, fp16 or fp32 [rows, vocabulary], not {logits.dtype} {tuple(logits.shape)}")
-    B, V = logits.shape
-    dev = logits.device
-    if logits.stride(1) != 1 and V > 1:
+    shape = logits.shape
+    dtype = _KV8_DTYPES.get(logits.dtype)
+    if len(shape) != 2 or dtype is None or shape[1] < 1:
+        raise ValueError(f"logits have to be bf16, fp16 or fp32 [rows, vocabulary], not {logits.dtype} {tuple(shape)}")
+    B, V = shape
+    index = logits.get_device()
+    stride, one = logits.stride()
+    if one != 1 and V > 1:
         logits = logits.contiguous()
+        stride = V
     if rng is not None:
         if rng.shape != (B,) or rng.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"rng has to be an int32 or int64 tensor [{B}]: the low 32 bits of each are used")
-        rng = rng.to(torch.int32).contiguous()
-    _same_device(dev, rng=rng, step_ptr=step_ptr, out_tok=out_tok, out_logp=out_logp)
-    (t, t0), (k, k0) = _per_row(temperature, "temperature", B, torch.float32, dev), _per_row(top_k, "top_k", B, torch.int32, dev)
-    (p, p0), (m, m0) = _per_row(top_p, "top_p", B, torch.float32, dev), _per_row(min_p, "min_p", B, torch.float32, dev)
-    tok = torch.empty(B, dtype=torch.int32, device=dev) if out_tok is None else out_tok
-    logp = torch.empty(B, dtype=torch.float32, device=dev) if out_logp is None else out_logp
-    for name, x, dt in (("out_tok", tok, torch.int32), ("out_logp", logp, torch.float32)):
-        if x.shape != (B,) or x.dtype != dt or not x.is_contiguous():
+        if rng.dtype != torch.int32 or not rng.is_contiguous():
+            rng = rng.to(torch.int32).contiguous()
+    (t, t0), (k, k0) = _per_row(temperature, "temperature", B, torch.float32, index), _per_row(top_k, "top_k", B, torch.int32, index)
+    (p, p0), (m, m0) = _per_row(top_p, "top_p", B, torch.float32, index), _per_row(min_p, "min_p", B, torch.float32, index)
+    tok = torch.empty(B, dtype=torch.int32, device=logits.device) if out_tok is None else out_tok
+    logp = torch.empty(B, dtype=torch.float32, device=logits.device) if out_logp is None else out_logp
+    for name, x, dt in (("out_tok", out_tok, torch.int32), ("out_logp", out_logp, torch.float32)):
+        if x is not None and (x.shape != (B,) or x.dtype != dt or not x.is_contiguous()):
             raise ValueError(f"{name} has to be a contiguous {dt} tensor [{B}]")
-    with torch.cuda.device(dev):
-        _chk(lib().trlb_sample_filtered(_p(logits), c_int(_KV8_DTYPES[logits.dtype]), c_longlong(logits.stride(0)), c_int(B),
-                                        c_int(V), _p(t), c_float(t0), _p(k), c_int(min(int(k0), 2**31 - 1)), _p(p), c_float(p0),
-                                        _p(m), c_float(m0), _p(rng), ctypes.c_uint(seed & 0xFFFFFFFF), _p(step_ptr), _p(tok),
-                                        _p(logp), _s()), "sample_filtered")
+    _same_device(index, rng=rng, step_ptr=step_ptr, out_tok=out_tok, out_logp=out_logp)
+    if B == 0:
+        return tok, logp
+    call = _SAMPLE_FILTERED.pack(logits.data_ptr(), _ptr(t), _ptr(k), _ptr(p), _ptr(m), _ptr(rng), _ptr(step_ptr),
+                                 tok.data_ptr(), logp.data_ptr(), _raw_stream(index), stride, dtype, B, V,
+                                 max(-1, min(int(k0), 2**31 - 1)), 0, seed & 0xFFFFFFFF, t0, p0, m0)
+    _launch(index, _fn("trlb_sample_filtered", "s"), "sample_filtered", call)
     return tok, logp

@@ -17,10 +17,16 @@ import torch.nn.functional as F
 from ..oracle import ops as _ref
 
 
-def _cuda():
-    from . import cuda as _c
+_CUDA = None
 
-    return _c
+
+def _cuda():
+    global _CUDA
+    if _CUDA is None:
+        from . import cuda as _c
+
+        _CUDA = _c
+    return _CUDA
 
 
 def _use_kernel(x: torch.Tensor) -> bool:
