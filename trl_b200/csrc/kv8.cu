@@ -56,12 +56,16 @@ __device__ __forceinline__ void kv8_again(uint8_t* codes, int bytes, float ratio
   }
 }
 
+// Eight values as they stand in memory, and as floats.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]);
-template <>
-__device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&x)[8]) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+struct Raw8 { uint4 u[sizeof(T) / 2]; };
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, Raw8<T>& r) {
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(T) / 2); ++i) r.u[i] = reinterpret_cast<const uint4*>(p)[i];
+}
+__device__ __forceinline__ void floats8(const Raw8<__nv_bfloat16>& r, float (&x)[8]) {
+  const uint32_t w[4] = {r.u[0].x, r.u[0].y, r.u[0].z, r.u[0].w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 f = unpack_bf16(w[i]);
@@ -69,10 +73,8 @@ __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, flo
     x[2 * i + 1] = f.y;
   }
 }
-template <>
-__device__ __forceinline__ void load8<__half>(const __half* p, float (&x)[8]) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+__device__ __forceinline__ void floats8(const Raw8<__half>& r, float (&x)[8]) {
+  const uint32_t w[4] = {r.u[0].x, r.u[0].y, r.u[0].z, r.u[0].w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
@@ -80,11 +82,43 @@ __device__ __forceinline__ void load8<__half>(const __half* p, float (&x)[8]) {
     x[2 * i + 1] = f.y;
   }
 }
+__device__ __forceinline__ void floats8(const Raw8<float>& r, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    x[4 * i] = __uint_as_float(r.u[i].x);
+    x[4 * i + 1] = __uint_as_float(r.u[i].y);
+    x[4 * i + 2] = __uint_as_float(r.u[i].z);
+    x[4 * i + 3] = __uint_as_float(r.u[i].w);
+  }
+}
+// Largest magnitude of some values as the type's bits (ordered like the magnitudes; infinities and NaN are at least `special`).
+template <typename T>
+struct Bits;
 template <>
-__device__ __forceinline__ void load8<float>(const float* p, float (&x)[8]) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-  x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+struct Bits<__nv_bfloat16> {
+  static constexpr uint32_t special = 0x7f80u;
+  static __device__ __forceinline__ float value(uint32_t b) { return __uint_as_float(b << 16); }
+};
+template <>
+struct Bits<__half> {
+  static constexpr uint32_t special = 0x7c00u;
+  static __device__ __forceinline__ float value(uint32_t b) { return __half2float(__ushort_as_half((unsigned short)b)); }
+};
+template <>
+struct Bits<float> {
+  static constexpr uint32_t special = 0x7f800000u;
+  static __device__ __forceinline__ float value(uint32_t b) { return __uint_as_float(b); }
+};
+template <typename T>
+__device__ __forceinline__ uint32_t largest8(const Raw8<T>& r) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(T) / 2); ++i) {
+    const uint32_t w[4] = {r.u[i].x, r.u[i].y, r.u[i].z, r.u[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m = sizeof(T) == 2 ? __vmaxu2(m, w[j] & 0x7fff7fffu) : max(m, w[j] & 0x7fffffffu);
+  }
+  return sizeof(T) == 2 ? max(m & 0xffffu, m >> 16) : m;
 }
 __device__ __forceinline__ float as_float(float x) { return x; }
 __device__ __forceinline__ float as_float(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -96,15 +130,20 @@ struct Kv8Source {
   long long tok[2], head[2];   // strides in elements
 };
 
-// One block per (sequence, page it touches, head, keys or values).  The new rows of the page are read once to find the
-// largest magnitude and once more (from cache) to be written.
-template <typename T>
-__global__ void __launch_bounds__(256)
+// The new rows of pages, read once into registers: their largest magnitude decides the scale, then they are written.  A group
+// of threads (a warp for pages of up to 2048 values, else the block) takes one page and ITEMS of its 2 x heads tiles (head, keys
+// or values), whose loads are all under way together.  Bound by the bytes: 2 or 4 read and 1 written a value.
+template <typename T, int VECS, int ITEMS, bool WARP>
+__global__ void __launch_bounds__(256, sizeof(T) == 4 || VECS == 16 ? 2 : 4)
 kv8_append_pages_kernel(Kv8Source<T> src, Kv8Cache c, const int* __restrict__ table, int table_rows, int max_blocks,
-                        const int* __restrict__ starts, const int* __restrict__ cu, const int* __restrict__ slots,
+                        const int* __restrict__ starts, const int* __restrict__ cu, const int* __restrict__ slots, int n,
                         int tokens, int pages_per_seq, int* status) {
-  const int seq = blockIdx.x / pages_per_seq, nth = blockIdx.x % pages_per_seq;
-  const int head = blockIdx.y, which = blockIdx.z;
+  constexpr int GROUP = WARP ? 32 : 256, GROUPS = 256 / GROUP;
+  const int in = threadIdx.x % GROUP, wid = threadIdx.x >> 5;
+  const long long item = (long long)blockIdx.x * GROUPS + threadIdx.x / GROUP;
+  __shared__ uint32_t part[ITEMS][8];
+  const int seq = (int)(item / pages_per_seq), nth = (int)(item % pages_per_seq);
+  if (seq >= n) return;  // whole groups leave, here and below
   const int start = starts[seq];
   const int t0 = cu[seq], t1 = min(cu[seq + 1], tokens);
   if (start < 0 || t0 < 0 || t1 <= t0) return;
@@ -116,37 +155,88 @@ kv8_append_pages_kernel(Kv8Source<T> src, Kv8Cache c, const int* __restrict__ ta
   if (p1 <= p0) return;
   const int blk = kv8_page_of(table, table_rows, max_blocks, slots ? slots[seq] : seq, index, c.pages, status, SITE_KV8_APPEND);
   if (blk < 0) return;
-  const int row0 = p0 - index * bs, rows = p1 - p0;
-  const T* x = src.x[which] + (long long)(t0 + (p0 - start)) * src.tok[which] + (long long)head * src.head[which];
-  uint8_t* page = c.codes[which] + ((size_t)blk * c.heads + head) * bs * D;
-  float* scale = c.scale[which] + (size_t)blk * c.heads + head;
-  const int vecs = D / 8, n = rows * vecs;
-  float amax = 0.f;
-  for (int i = threadIdx.x; i < n; i += blockDim.x) {
-    float v[8];
-    load8<T>(x + (long long)(i / vecs) * src.tok[which] + (i % vecs) * 8, v);
+  const int row0 = p0 - index * bs, vecs = D / 8, count = (p1 - p0) * vecs, first = blockIdx.y * ITEMS;
+  Raw8<T> raw[ITEMS][VECS];
+  uint32_t top[ITEMS];
+  float old[ITEMS];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) amax = fmaxf(amax, kv8_magnitude(v[k]));
-  }
-  __shared__ float part[8];
-  amax = warp_max(amax);
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = amax;
-  const float old = row0 > 0 ? *scale : 0.f;
-  __syncthreads();
+  for (int j = 0; j < VECS; ++j) {
+    const int i = in + j * GROUP;
+    const long long row = t0 + (p0 - start) + i / vecs;
+    const int col = (i % vecs) * 8;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) amax = fmaxf(amax, part[w]);
-  const float now = fmaxf(old, kv8_pow2(kv8_exponent(amax)));
-  if (row0 > 0 && now > old) kv8_again(page, row0 * D, old / now, threadIdx.x, blockDim.x);
-  const float inv = 1.f / now;
-  for (int i = threadIdx.x; i < n; i += blockDim.x) {
-    float v[8];
-    load8<T>(x + (long long)(i / vecs) * src.tok[which] + (i % vecs) * 8, v);
-    uint2 u;
-    u.x = kv8_encode2(v[0], v[1], inv) | (kv8_encode2(v[2], v[3], inv) << 16);
-    u.y = kv8_encode2(v[4], v[5], inv) | (kv8_encode2(v[6], v[7], inv) << 16);
-    reinterpret_cast<uint2*>(page + row0 * D)[i] = u;
+    for (int k = 0; k < ITEMS; ++k) {
+      const int tile = first + k, which = tile & 1;
+      if (i < count && tile < 2 * c.heads)
+        load8<T>(src.x[which] + row * src.tok[which] + (long long)(tile >> 1) * src.head[which] + col, raw[k][j]);
+    }
   }
-  if (threadIdx.x == 0) *scale = now;
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    const int tile = first + k;
+    old[k] = row0 > 0 && tile < 2 * c.heads ? c.scale[tile & 1][(size_t)blk * c.heads + (tile >> 1)] : 0.f;
+    top[k] = 0;
+#pragma unroll
+    for (int j = 0; j < VECS; ++j)
+      if (in + j * GROUP < count && tile < 2 * c.heads) top[k] = max(top[k], largest8<T>(raw[k][j]));
+    top[k] = __reduce_max_sync(0xffffffffu, top[k]);
+    if (!WARP && (threadIdx.x & 31) == 0) part[k][wid] = top[k];
+  }
+  if (!WARP) __syncthreads();
+  else __syncwarp();  // every lane has read the old scales
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    const int tile = first + k, which = tile & 1;
+    if (tile >= 2 * c.heads) break;
+    if (!WARP)
+#pragma unroll
+      for (int w = 0; w < 8; ++w) top[k] = max(top[k], part[k][w]);
+    float amax = Bits<T>::value(top[k]);
+    const bool special = top[k] >= Bits<T>::special;  // an infinity or NaN among them: rare, so the scale is found again without
+    if (special) {
+      amax = 0.f;
+#pragma unroll
+      for (int j = 0; j < VECS; ++j) {
+        float v[8];
+        floats8(raw[k][j], v);
+        if (in + j * GROUP < count)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) amax = fmaxf(amax, kv8_magnitude(v[e]));
+      }
+      amax = warp_max(amax);
+      if (!WARP) {
+        __shared__ float again[8];
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) again[wid] = amax;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 8; ++w) amax = fmaxf(amax, again[w]);
+      }
+    }
+    const size_t at = (size_t)blk * c.heads + (tile >> 1);
+    uint8_t* page = c.codes[which] + at * bs * D;
+    const float now = fmaxf(old[k], kv8_pow2(kv8_exponent(amax)));
+    if (row0 > 0 && now > old[k]) kv8_again(page, row0 * D, old[k] / now, in, GROUP);
+    const float inv = 1.f / now;
+#pragma unroll
+    for (int j = 0; j < VECS; ++j) {
+      const int i = in + j * GROUP;
+      if (i < count) {
+        float v[8];
+        floats8(raw[k][j], v);
+        uint2 u;
+        if (special) {
+          u.x = kv8_encode2(v[0], v[1], inv) | (kv8_encode2(v[2], v[3], inv) << 16);
+          u.y = kv8_encode2(v[4], v[5], inv) | (kv8_encode2(v[6], v[7], inv) << 16);
+        } else {
+          u.x = kv8_encode2_finite(v[0], v[1], inv) | (kv8_encode2_finite(v[2], v[3], inv) << 16);
+          u.y = kv8_encode2_finite(v[4], v[5], inv) | (kv8_encode2_finite(v[6], v[7], inv) << 16);
+        }
+        reinterpret_cast<uint2*>(page + row0 * D)[i] = u;
+      }
+    }
+    if (in == 0) c.scale[which][at] = now;
+  }
 }
 
 // One warp per (sequence, head, keys or values): the row of one token.
@@ -311,9 +401,24 @@ int kv8_append_launch(const Kv8Source<T>& src, const Kv8Cache& c, const int* tab
   }
   const long long per = (max_new - 1) / c.page_size + 2;  // a piece may begin inside a page
   if (per * n > 2147483647ll) return -3;
-  kv8_append_pages_kernel<T><<<dim3((unsigned)(per * n), c.heads, 2), 256, 0, st>>>(
-      src, c, table, table_rows, max_blocks, starts, cu, slots, tokens, (int)per, status);
-  return (int)cudaGetLastError();
+  auto go = [&](auto vecs, auto items, auto warp) {
+    constexpr int V = decltype(vecs)::value, I = decltype(items)::value;
+    constexpr bool W = decltype(warp)::value;
+    const unsigned groups = W ? 8 : 1;
+    kv8_append_pages_kernel<T, V, I, W><<<dim3((unsigned)((per * n + groups - 1) / groups), (2 * c.heads + I - 1) / I), 256, 0, st>>>(
+        src, c, table, table_rows, max_blocks, starts, cu, slots, n, tokens, (int)per, status);
+    return (int)cudaGetLastError();
+  };
+  // 8 vectors of 16 bytes a thread, where a tile allows it: two tiles of 64 rows of 128 bf16 values, say
+  using std::integral_constant;
+  const int values = c.page_size * c.dim;
+  if (values <= 1024) return go(integral_constant<int, 4>(), integral_constant<int, 2>(), std::true_type());
+  if (values <= 2048) return go(integral_constant<int, 8>(), integral_constant<int, 1>(), std::true_type());
+  if (values <= 4096) return go(integral_constant<int, 2>(), integral_constant<int, 4>(), std::false_type());
+  if (values <= 8192) return go(integral_constant<int, 4>(), integral_constant<int, 2>(), std::false_type());
+  if (values <= 16384) return go(integral_constant<int, 8>(), integral_constant<int, 1>(), std::false_type());
+  if (values <= 32768) return go(integral_constant<int, 16>(), integral_constant<int, 1>(), std::false_type());
+  return -6;
 }
 
 }  // namespace trlb

@@ -33,6 +33,12 @@ __device__ __forceinline__ uint32_t kv8_encode2(float a, float b, float inv_scal
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(yb), "f"(ya));
   return r;
 }
+// The same of finite values.
+__device__ __forceinline__ uint32_t kv8_encode2_finite(float a, float b, float inv_scale) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b * inv_scale), "f"(a * inv_scale));
+  return r;
+}
 // Two codes (low byte first) as a pair of fp16, exact: fp16 has every e4m3 value.
 __device__ __forceinline__ uint32_t kv8_decode2(uint32_t codes) {
   uint32_t r;

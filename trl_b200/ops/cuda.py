@@ -1151,8 +1151,8 @@ def _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table):
     if len(shape) != 4 or v_cache.shape != shape or k_cache.dtype != torch.float8_e4m3fn or v_cache.dtype != torch.float8_e4m3fn:
         raise ValueError("the codes of keys and values are float8_e4m3fn tensors [pages, heads, page size, head dim] of one shape")
     pages, heads, page, dim = shape
-    if page < 16 or page & (page - 1) or dim not in (64, 96, 128, 256):
-        raise ValueError(f"page sizes are powers of two from 16 on and head dims 64, 96, 128 or 256, not {page} and {dim}")
+    if page < 16 or page > 128 or page & (page - 1) or dim not in (64, 96, 128, 256):
+        raise ValueError(f"page sizes are 16, 32, 64 or 128 and head dims 64, 96, 128 or 256, not {page} and {dim}")
     if k_scale.shape != shape[:2] or v_scale.shape != shape[:2] or k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
         raise ValueError(f"k_scale and v_scale have to be fp32 [pages, heads] = [{pages}, {heads}]")
     if (k_cache.data_ptr() | v_cache.data_ptr()) & 15 or not (k_cache.is_contiguous() and v_cache.is_contiguous()

@@ -171,8 +171,8 @@ def load_balancing_loss(router_probs, topk_idx, num_experts, top_k, token_mask=N
 def kv8_alloc(num_blocks, kv_heads, block_size, head_dim, device=None):
     """An 8-bit paged cache: ``(k_cache, v_cache, k_scale, v_scale)``.  The codes are e4m3 [blocks, heads, block size, head
     dim]; an entry stands for its code times the scale [blocks, heads] of its page and head, a power of two."""
-    if block_size < 16 or block_size & (block_size - 1) or head_dim not in (64, 96, 128, 256):
-        raise ValueError(f"page sizes are powers of two from 16 on and head dims 64, 96, 128 or 256, not {block_size} and {head_dim}")
+    if block_size not in (16, 32, 64, 128) or head_dim not in (64, 96, 128, 256):
+        raise ValueError(f"page sizes are 16, 32, 64 or 128 and head dims 64, 96, 128 or 256, not {block_size} and {head_dim}")
     codes = [torch.zeros(num_blocks, kv_heads, block_size, head_dim, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
              for _ in range(2)]
     return (*codes, *[torch.ones(num_blocks, kv_heads, dtype=torch.float32, device=device) for _ in range(2)])
