@@ -20,6 +20,8 @@
 //      both sides, which brackets the border; the tokens of the bracket are listed, and the exact mass above it says which of
 //      them is the last.  A bracket with too many tokens for the list is cut again by histograms over the logits' bits.
 //   4. a last pass over the row draws among what is kept.
+// A row that fits into the shared memory of a cluster is read once and stays there for all of it (SfSampler::fast); the few rows
+// that need what fast() leaves out, and larger ones, are read again for each pass (SfSampler::run).
 // Counts and the sums over lists are integers, other sums are taken in a fixed order: results do not depend on timing.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
@@ -34,8 +36,10 @@ namespace trlb {
 constexpr int SF_THREADS = 512, SF_WARPS = SF_THREADS / 32;  // two blocks an SM
 constexpr int SF_EACH = 4;         // bins of a thread: SF_BINS / SF_THREADS
 constexpr int SF_BINS = 2048;      // histogram bins; the last one holds all that lies further below
-constexpr int SF_LIST = 8192;      // tokens that the list holds
-constexpr int SF_CUT = 2048;       // and the cut around the border; more are sorted in the list itself
+constexpr int SF_LIST = 4096;      // tokens that the list holds
+constexpr int SF_CUT = 1024;       // and the cut around the border; more are sorted in the list itself
+constexpr int SF_HELD = 4096;      // 16-byte vectors of a row in a block's shared memory, at most: with it two blocks an SM
+constexpr float SF_FINE = 1024.f;  // parts of a bin in which the histogram adds up where in the bin its tokens lie
 constexpr int SF_BATCH = 16;       // logits that a thread loads at once
 constexpr float SF_MAX = 3.4028234663852886e38f;
 constexpr float SF_LOG2E = 1.4426950408889634f;
@@ -105,14 +109,53 @@ __device__ __forceinline__ void sf_unpack<__half>(uint4 u, float* x) {
   }
 }
 
+template <typename T>
+__device__ __forceinline__ T sf_lowest();
+template <>
+__device__ __forceinline__ float sf_lowest<float>() { return -INFINITY; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 sf_lowest<__nv_bfloat16>() { return __ushort_as_bfloat16((unsigned short)0xff80); }
+template <>
+__device__ __forceinline__ __half sf_lowest<__half>() { return __ushort_as_half((unsigned short)0xfc00); }
+// NaN -> -inf (a maximum drops it), nothing above cap, one zero of both.
+__device__ __forceinline__ float sf_clean1(float y, float cap) { return fminf(fmaxf(y, -INFINITY), cap) + 0.f; }
+template <typename T>
+__device__ __forceinline__ void sf_clean(uint4& u, float cap);
+template <>
+__device__ __forceinline__ void sf_clean<float>(uint4& u, float cap) {
+  u.x = __float_as_uint(sf_clean1(__uint_as_float(u.x), cap));
+  u.y = __float_as_uint(sf_clean1(__uint_as_float(u.y), cap));
+  u.z = __float_as_uint(sf_clean1(__uint_as_float(u.z), cap));
+  u.w = __float_as_uint(sf_clean1(__uint_as_float(u.w), cap));
+}
+template <>
+__device__ __forceinline__ void sf_clean<__nv_bfloat16>(uint4& u, float cap) {
+  const __nv_bfloat162 lo = __bfloat162bfloat162(sf_lowest<__nv_bfloat16>()), hi = __bfloat162bfloat162(__float2bfloat16_rz(cap)),
+                       zero = __bfloat162bfloat162(__float2bfloat16(0.f));
+  __nv_bfloat162* p = reinterpret_cast<__nv_bfloat162*>(&u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) p[i] = __hadd2(__hmin2(__hmax2(p[i], lo), hi), zero);
+}
+template <>
+__device__ __forceinline__ void sf_clean<__half>(uint4& u, float cap) {
+  const __half2 lo = __half2half2(sf_lowest<__half>()), hi = __half2half2(__float2half_rz(fminf(cap, 65504.f))),
+                zero = __half2half2(__float2half(0.f));
+  __half2* p = reinterpret_cast<__half2*>(&u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) p[i] = __hadd2(__hmin2(__hmax2(p[i], lo), hi), zero);
+}
+
 struct SfShared {
   unsigned hist[SF_BINS];
+  union {
+    unsigned where[SF_BINS];          // sums of the tokens' places in their bins
+    unsigned cumul[SF_BINS];          // tokens up to and with a bin
+    unsigned long long cut[SF_CUT];   // the part of the list around the border
+  };
   unsigned long long list[SF_LIST];   // ~key << 32 | column: ascending is "larger logit, then lower column"
-  unsigned long long cut[SF_CUT];     // the part of the list around the border
   double red[3][SF_WARPS];
   unsigned long long sum[SF_WARPS];
-  unsigned long long weights[SF_THREADS];
-  double mass, first_mass;            // this block's shares of sums
+  double mass, first_mass, sums[2];   // this block's shares of sums
   double kept;                        // mass down to the border, 0: unknown
   float fmax;
   unsigned kmin, kmax, list_n, cut_n;
@@ -123,9 +166,11 @@ struct SfShared {
   float best;                         // this block's draw
   int best_col;
   float best_z;
+  float bests[8], best_zs[8];          // the first block: all blocks' draws
+  int best_cols[8];
 };
-// the table is read four bins at a time
-static_assert(offsetof(SfShared, hist) % 16 == 0, "bins on 16 bytes");
+// the tables are read four bins at a time
+static_assert(offsetof(SfShared, hist) % 16 == 0 && offsetof(SfShared, where) % 16 == 0, "bins on 16 bytes");
 
 // A block's columns of a row.
 template <typename T>
@@ -134,8 +179,7 @@ struct SfRow {
   int v0, v1;
   bool vec;
   float cap;  // logits from here on are equals: their quotients by the temperature are not finite
-  // NaN -> -inf (fmaxf drops it); one zero of both
-  __device__ __forceinline__ float clean(float y) const { return fminf(fmaxf(y, -INFINITY), cap) + 0.f; }
+  __device__ __forceinline__ float clean(float y) const { return sf_clean1(y, cap); }
   // f(logit, column) over the block's columns, until stop() says so
   template <typename F, typename G>
   __device__ __forceinline__ void each(F f, G stop) const {
@@ -221,21 +265,31 @@ __device__ __forceinline__ void sf_block_prefix(double (&v)[N], SfShared& s) {
     for (int n = 0; n < N; ++n) v[n] += s.red[n][w];
 }
 
-// Sorts n entries ascending; `at` has room for the next power of two.
-__device__ void sf_sort(unsigned long long* at, int n) {
+// Sorts n entries ascending; `at` has room for the next power of two.  As many warps as it takes pairs for work on it: the
+// others wait once, at the end.
+__device__ __noinline__ void sf_sort(unsigned long long* at, int n) {
   int size = 2;
   while (size < n) size <<= 1;
-  for (int i = n + threadIdx.x; i < size; i += SF_THREADS) at[i] = ~0ull;
+  const int workers = min(SF_THREADS, max(32, size / 2));
   __syncthreads();
-  for (int k = 2; k <= size; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      for (int i = threadIdx.x; i < size / 2; i += SF_THREADS) {
-        const int a = 2 * i - (i & (j - 1)), b = a + j;
-        const unsigned long long x = at[a], y = at[b];
-        if ((x > y) == ((a & k) == 0)) { at[a] = y; at[b] = x; }
+  if (threadIdx.x < workers) {
+    auto meet = [&] {
+      if (workers == 32) __syncwarp();
+      else asm volatile("bar.sync 1, %0;" ::"r"(workers) : "memory");
+    };
+    for (int i = n + threadIdx.x; i < size; i += workers) at[i] = ~0ull;
+    meet();
+    for (int k = 2; k <= size; k <<= 1)
+      for (int j = k >> 1; j > 0; j >>= 1) {
+        for (int i = threadIdx.x; i < size / 2; i += workers) {
+          const int a = 2 * i - (i & (j - 1)), b = a + j;
+          const unsigned long long x = at[a], y = at[b];
+          if ((x > y) == ((a & k) == 0)) { at[a] = y; at[b] = x; }
+        }
+        meet();
       }
-      __syncthreads();
-    }
+  }
+  __syncthreads();
 }
 __device__ __forceinline__ float sf_entry_x(unsigned long long e) { return sf_unkey(~(unsigned)(e >> 32)); }
 
@@ -291,13 +345,30 @@ struct SfSampler {
     step = (far < 31.f ? (float)(SF_BINS - 2) / fmaxf(far, 1e-3f) : 64.f) / temperature;
   }
 
+  // Sum and maximum over the blocks of a value that each of them left in its shared memory: a lane reads a block's, so that the
+  // reads are under way together; the tree of the shuffles adds them in one order.
+  template <typename F>
+  __device__ __forceinline__ double sum_of(F value) {
+    const int lane = tid & 31;
+    double v = lane < C ? value(*of(lane)) : 0.;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return __shfl_sync(0xffffffffu, v, 0);
+  }
+  template <typename F>
+  __device__ __forceinline__ float max_of(F value) {
+    const int lane = tid & 31;
+    float v = lane < C ? value(*of(lane)) : -INFINITY;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return __shfl_sync(0xffffffffu, v, 0);
+  }
   // Sum of a block-wide value over the cluster, in the order of the blocks.  Ends with a barrier.
   __device__ double cluster_sum(double v) {
     v = sf_block_sum(v, s);
     if (tid == 0) s.mass = v;
     cluster.sync();
-    double all = 0.;
-    for (int b = 0; b < C; ++b) all += of(b)->mass;
+    const double all = sum_of([](const SfShared& o) { return o.mass; });
     cluster.sync();
     return all;
   }
@@ -305,19 +376,28 @@ struct SfSampler {
     for (int i = tid; i < SF_BINS; i += SF_THREADS) s.hist[i] = 0;
     __syncthreads();
   }
-  // This thread's bins of the whole row.
-  __device__ void merged_bins(unsigned (&n)[SF_EACH]) {
+  // This thread's bins of the whole row.  The table may be written again behind the next barrier.
+  __device__ __noinline__ void merged_bins(unsigned (&n)[SF_EACH]) {
     cluster.sync();
+    merge([](const SfShared& o) { return o.hist; }, n);
+  }
+  template <typename F>
+  __device__ __forceinline__ void merge(F table, unsigned (&n)[SF_EACH]) {
+    uint4 x[8];
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+      x[b] = make_uint4(0, 0, 0, 0);
+      if (b < C) x[b] = reinterpret_cast<const uint4*>(table(*of(b)))[tid];
+    }
 #pragma unroll
     for (int i = 0; i < SF_EACH; ++i) n[i] = 0;
-    for (int b = 0; b < C; ++b) {
-      const uint4 x = reinterpret_cast<const uint4*>(of(b)->hist)[tid];
-      n[0] += x.x;
-      n[1] += x.y;
-      n[2] += x.z;
-      n[3] += x.w;
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+      n[0] += x[b].x;
+      n[1] += x[b].y;
+      n[2] += x[b].z;
+      n[3] += x[b].w;
     }
-    cluster.sync();
   }
   // Those of this block.
   __device__ void own_bins(unsigned (&n)[SF_EACH]) {
@@ -347,29 +427,50 @@ struct SfSampler {
     __syncthreads();
   }
   // Bins between which the mass passes `goal`: the first whose upper bound of the mass up to it does, to the first whose
-  // lower bound does.  hi / lo: bounds of a token's weight in this thread's bins; mass: what stands above the histogram.
-  __device__ __noinline__ void bracket_mass(const unsigned (&n)[SF_EACH], const float (&hi)[SF_EACH], const float (&lo)[SF_EACH], double mass, double goal) {
+  // lower bound does.  hi / lo: bounds of the mass in this thread's bins; mass: what stands above the histogram.  With `keep`
+  // s.cumul has the tokens up to and with each bin.
+  __device__ __noinline__ void bracket_mass(const unsigned (&n)[SF_EACH], const float (&hi)[SF_EACH], const float (&lo)[SF_EACH], double mass, double goal, bool keep) {
     if (tid == 0) {
       s.bin_lo = s.bin_hi = SF_BINS - 1;
       s.above = s.upto = 0;
     }
-    double v[3] = {0., 0., 0.};
+    // 32 bits do: the bounds are apart by more than some tens of roundings
+    const int lane = tid & 31, wid = tid >> 5;
+    float v[2] = {hi[0] + hi[1] + hi[2] + hi[3], lo[0] + lo[1] + lo[2] + lo[3]};
+    unsigned cnt = n[0] + n[1] + n[2] + n[3];
+    const float own[2] = {v[0], v[1]};
+    const unsigned own_n = cnt;
 #pragma unroll
-    for (int i = 0; i < SF_EACH; ++i) {
-      v[0] += n[i];
-      v[1] += n[i] * (double)hi[i] * 1.00001;
-      v[2] += n[i] * (double)lo[i] * 0.99999;
+    for (int o = 1; o < 32; o <<= 1) {
+      const float x = __shfl_up_sync(0xffffffffu, v[0], o), y = __shfl_up_sync(0xffffffffu, v[1], o);
+      const unsigned z = __shfl_up_sync(0xffffffffu, cnt, o);
+      if (lane >= o) { v[0] += x; v[1] += y; cnt += z; }
     }
-    const double own[3] = {v[0], v[1], v[2]};
-    sf_block_prefix(v, s);
-    unsigned cnt = (unsigned)(v[0] - own[0]);
-    double up = mass + (v[1] - own[1]), low = mass + (v[2] - own[2]);  // bounds before this thread's bins
+    __syncthreads();
+    if (lane == 31) { s.red[0][wid] = v[0]; s.red[1][wid] = v[1]; s.red[2][wid] = cnt; }
+    __syncthreads();
+    float up = (float)mass, low = (float)mass;
+    unsigned before = 0;
+#pragma unroll
+    for (int w = 0; w < SF_WARPS; ++w)
+      if (w < wid) { up += (float)s.red[0][w]; low += (float)s.red[1][w]; before += (unsigned)s.red[2][w]; }
+    up += v[0] - own[0];  // bounds before this thread's bins
+    low += v[1] - own[1];
+    cnt += before - own_n;
+    const float limit = (float)goal;
+    int first_up = SF_BINS - 1, first_low = SF_BINS - 1;
 #pragma unroll
     for (int i = 0; i < SF_EACH; ++i) {
-      up += n[i] * (double)hi[i] * 1.00001;
-      low += n[i] * (double)lo[i] * 0.99999;
-      if (up > goal) atomicMin(&s.bin_lo, SF_EACH * tid + i);
-      if (low > goal) atomicMin(&s.bin_hi, SF_EACH * tid + i);
+      up += hi[i];
+      low += lo[i];
+      if (up * 1.00001f > limit) first_up = min(first_up, SF_EACH * tid + i);
+      if (low * 0.99999f > limit) first_low = min(first_low, SF_EACH * tid + i);
+    }
+    first_up = __reduce_min_sync(0xffffffffu, first_up);
+    first_low = __reduce_min_sync(0xffffffffu, first_low);
+    if ((tid & 31) == 0) {
+      atomicMin(&s.bin_lo, first_up);
+      atomicMin(&s.bin_hi, first_low);
     }
     __syncthreads();
 #pragma unroll
@@ -377,28 +478,40 @@ struct SfSampler {
       if (SF_EACH * tid + i == s.bin_lo) s.above = cnt;
       cnt += n[i];
       if (SF_EACH * tid + i == s.bin_hi) s.upto = cnt;
-      s.hist[SF_EACH * tid + i] = cnt;  // from here on: tokens up to and with a bin
+      if (keep) s.cumul[SF_EACH * tid + i] = cnt;
     }
     __syncthreads();
   }
-  // Bounds of a weight in this thread's bins of the linear histogram.
-  __device__ void linear_bounds(float (&hi)[SF_EACH], float (&lo)[SF_EACH]) const {
+  // Bounds of the mass of this thread's bins of the linear histogram, from counts alone.
+  __device__ void linear_bounds(const unsigned (&n)[SF_EACH], float (&hi)[SF_EACH], float (&lo)[SF_EACH]) const {
 #pragma unroll
     for (int i = 0; i < SF_EACH; ++i) {
       const int bin = SF_EACH * tid + i;
-      hi[i] = exp2f(-(float)bin / step * c);
-      lo[i] = bin == SF_BINS - 1 ? 0.f : exp2f(-(float)(bin + 1) / step * c);
+      hi[i] = (float)n[i] * exp2f(-(float)bin / step * c) * 1.00001f;
+      lo[i] = bin == SF_BINS - 1 ? 0.f : (float)n[i] * exp2f(-(float)(bin + 1) / step * c) * 0.99999f;
     }
   }
-  // Bounds of a weight in this thread's bins of the histogram of keys from `top` down over `span`.
-  __device__ void key_bounds(float (&hi)[SF_EACH], float (&lo)[SF_EACH], unsigned top, unsigned span, int shift) const {
+  // The same with the sums of the places in the bins: a token's weight is exp(-y) of the bin's upper one, y its place times the
+  // bin's width, and 1 - y <= exp(-y) <= 1 - y + y^2 / 2.
+  __device__ void placed_bounds(const unsigned (&n)[SF_EACH], const unsigned (&place)[SF_EACH], float (&hi)[SF_EACH], float (&lo)[SF_EACH]) const {
+    const float width = c * 0.6931471805599453f / step;
+#pragma unroll
+    for (int i = 0; i < SF_EACH; ++i) {
+      const int bin = SF_EACH * tid + i;
+      const float top = exp2f(-(float)bin / step * c), y = (float)place[i] / SF_FINE * width, slack = (float)n[i] * width / SF_FINE;
+      hi[i] = fminf((float)n[i], (float)n[i] - y + slack + 0.5f * width * y) * top * 1.00001f;
+      lo[i] = bin == SF_BINS - 1 ? 0.f : fmaxf((float)n[i] * (1.f - width), (float)n[i] - y - slack) * top * 0.99999f;
+    }
+  }
+  // Bounds of the mass of this thread's bins of the histogram of keys from `top` down over `span`.
+  __device__ void key_bounds(const unsigned (&n)[SF_EACH], float (&hi)[SF_EACH], float (&lo)[SF_EACH], unsigned top, unsigned span, int shift) const {
 #pragma unroll
     for (int i = 0; i < SF_EACH; ++i) {
       const unsigned bin = (unsigned)(SF_EACH * tid + i);
       hi[i] = lo[i] = 0.f;
       if (bin <= span >> shift) {
-        hi[i] = weight(sf_unkey(top - (bin << shift)));
-        lo[i] = weight(sf_unkey(top - min((bin << shift) + ((1u << shift) - 1u), span)));
+        hi[i] = (float)n[i] * weight(sf_unkey(top - (bin << shift))) * 1.00001f;
+        lo[i] = (float)n[i] * weight(sf_unkey(top - min((bin << shift) + ((1u << shift) - 1u), span))) * 0.99999f;
       }
     }
   }
@@ -413,8 +526,7 @@ struct SfSampler {
       q.each(
           [&](float x, int col) {
             if (in(x)) {
-              const unsigned i = atomicAdd(&sh.list_n, 1u);
-              if (i < SF_LIST) sh.list[i] = (unsigned long long)(~sf_key(x)) << 32 | (unsigned)col;
+              append(sh, x, col);
             }
           },
           [&] { return *reinterpret_cast<volatile unsigned*>(&sh.list_n) > SF_LIST; });
@@ -424,16 +536,23 @@ struct SfSampler {
   // The blocks' lists in the first one.
   __device__ __noinline__ int collect() {
     cluster.sync();
-    int n = 0;
-    for (int b = 0; b < C; ++b) n += (int)of(b)->list_n;
+    const int lane = tid & 31, mine = lane < C ? (int)of(lane)->list_n : 0;
+    int upto = mine;  // entries of the blocks up to this lane's
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    const int n = __shfl_sync(0xffffffffu, upto, 7);
     if (n > SF_LIST) return 0;
     if (rank == 0) {
-      int at = (int)s.list_n;
-      for (int b = 1; b < C; ++b) {
-        const int m = (int)of(b)->list_n;
+      // each warp copies part of one other block's list
+      constexpr int W = SF_WARPS / 8;
+      const int b = (tid >> 5) / W, part = (tid >> 5) % W;
+      const int m = __shfl_sync(0xffffffffu, mine, b), at = __shfl_sync(0xffffffffu, upto, b) - m;
+      if (b > 0 && b < C) {
         const unsigned long long* from = of(b)->list;
-        for (int i = tid; i < m; i += SF_THREADS) s.list[at + i] = from[i];
-        at += m;
+        for (int i = part * 32 + lane; i < m; i += W * 32) s.list[at + i] = from[i];
       }
       __syncthreads();
     }
@@ -442,37 +561,32 @@ struct SfSampler {
 
   // ---- the first block alone: borders in its list of n tokens -----------------------------------------------------------
   __device__ __forceinline__ unsigned long long whole(double w) const { return (unsigned long long)(w * SF_UNIT + 0.5); }
-  // The border among n <= SF_THREADS entries in no order, `above` tokens and `mass` above them, a thread an entry: it counts and
-  // weighs the entries before its own.
+  // The border among n <= SF_THREADS sorted entries, a thread an entry; `above` tokens and `mass` above them.
   __device__ __noinline__ void small_border(const unsigned long long* at, int n, bool by_mass, double goal, unsigned above, double mass) {
     const unsigned long long mine = tid < n ? at[tid] : 0;
-    const unsigned long long own = tid < n && by_mass ? whole((double)weight(sf_entry_x(mine))) : 0;
-    if (tid == 0) s.bin_lo = -1;
-    if (tid < n) s.weights[tid] = own;
-    __syncthreads();
-    int rank_here = 0;
-    unsigned long long before = 0;
-    if (tid < n) {
-#pragma unroll 4
-      for (int j = 0; j < n; ++j) {
-        if (at[j] < mine) {
-          ++rank_here;
-          before += s.weights[j];
-        }
+    bool border = !by_mass && tid < n && above + tid + 1 == (unsigned)goal;
+    double kept = 0.;
+    if (by_mass) {
+      const int lane = tid & 31, wid = tid >> 5;
+      const unsigned long long own = tid < n ? whole((double)weight(sf_entry_x(mine))) : 0;
+      unsigned long long upto = own;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
       }
-      if (by_mass) {
-        if (mass + (double)before / SF_UNIT <= goal) atomicMax(&s.bin_lo, rank_here);
-      } else if (above + rank_here + 1 == (unsigned)goal) {
-        s.border = sf_entry_x(mine);
-        s.border_col = 0x7fffffff;
-        s.kept = 0.;
-      }
+      if (lane == 31) s.sum[wid] = upto;
+      __syncthreads();
+      for (int w = 0; w < wid; ++w) upto += s.sum[w];
+      // the last entry before which at most `goal` stands: its successor is behind more
+      const double behind = mass + (double)upto / SF_UNIT;
+      border = tid < n && (tid == 0 || mass + (double)(upto - own) / SF_UNIT <= goal) && (tid == n - 1 || behind > goal);
+      kept = behind;
     }
-    __syncthreads();
-    if (by_mass && tid < n && rank_here == max(0, s.bin_lo)) {
+    if (border) {
       s.border = sf_entry_x(mine);
-      s.border_col = (int)(unsigned)mine;
-      s.kept = mass + (double)(before + own) / SF_UNIT;
+      s.border_col = by_mass ? (int)(unsigned)mine : 0x7fffffff;
+      s.kept = kept;
     }
     __syncthreads();
   }
@@ -516,6 +630,7 @@ struct SfSampler {
   // stands (by_mass), or the goal-th token and its equals.  Leaves s.border, s.border_col and s.kept (0: unknown).
   __device__ __noinline__ void list_border(int n, bool by_mass, double goal, unsigned above, double mass) {
     if (n <= SF_THREADS) {
+      sf_sort(s.list, n);
       small_border(s.list, n, by_mass, goal, above, mass);
       return;
     }
@@ -540,8 +655,8 @@ struct SfSampler {
     own_bins(cnt);
     if (by_mass) {
       float wh[SF_EACH], wl[SF_EACH];
-      key_bounds(wh, wl, hi, hi - lo, shift);
-      bracket_mass(cnt, wh, wl, mass, goal);
+      key_bounds(cnt, wh, wl, hi, hi - lo, shift);
+      bracket_mass(cnt, wh, wl, mass, goal, false);
     } else {
       bracket_count(cnt, (unsigned)goal - above);
     }
@@ -563,12 +678,9 @@ struct SfSampler {
     __syncthreads();
     const int m = (int)s.cut_n;
     above += a0;
-    if (m <= SF_THREADS) {
-      small_border(s.cut, m, by_mass, goal, above, mass);
-    } else {
-      sf_sort(s.cut, m);
-      sorted_border(s.cut, m, by_mass, goal, above, mass);
-    }
+    sf_sort(s.cut, m);
+    if (m <= SF_THREADS) small_border(s.cut, m, by_mass, goal, above, mass);
+    else sorted_border(s.cut, m, by_mass, goal, above, mass);
   }
   static __device__ __forceinline__ bool within(float x, int col, float border, int border_col) {
     return x > border || (x == border && col <= border_col);
@@ -629,11 +741,12 @@ struct SfSampler {
     if (floor_mass) goal *= cluster_sum((double)part);
     unsigned n[SF_EACH];
     merged_bins(n);
+    cluster.sync();
     const double limit = goal;
     if (by_mass) {
       float hi[SF_EACH], lo[SF_EACH];
-      linear_bounds(hi, lo);
-      bracket_mass(n, hi, lo, 0., limit);
+      linear_bounds(n, hi, lo);
+      bracket_mass(n, hi, lo, 0., limit, false);
     } else {
       double all[1] = {(double)n[0] + n[1] + n[2] + n[3]};
       sf_block_prefix(all, s);
@@ -706,11 +819,12 @@ struct SfSampler {
         if (k >= kmin && k <= top) atomicAdd(&s.hist[(top - k) >> shift], 1u);
       });
       merged_bins(n);
+      cluster.sync();
       unsigned c0, c1, a0, a1;  // the bracket's bins; tokens of the interval above it, and up to its end
       if (by_mass) {
         float hi[SF_EACH], lo[SF_EACH];
-        key_bounds(hi, lo, top, span, shift);
-        bracket_mass(n, hi, lo, mass, limit);
+        key_bounds(n, hi, lo, top, span, shift);
+        bracket_mass(n, hi, lo, mass, limit, true);
         c0 = (unsigned)s.bin_lo, c1 = (unsigned)s.bin_hi, a0 = s.above, a1 = s.upto;
         __syncthreads();
         auto between = [&](unsigned from, unsigned to) {  // exact mass of a run of bins
@@ -724,7 +838,7 @@ struct SfSampler {
         if (c0 > 0) mass += between(0, c0 - 1);
         // the bounds leave several bins only where the goal is within their margin of a bin's end
         while (c0 < c1 && a1 - a0 > SF_LIST) {
-          const unsigned mid = (c0 + c1) / 2, am = s.hist[mid];
+          const unsigned mid = (c0 + c1) / 2, am = s.cumul[mid];
           const double here = between(c0, mid);
           if (mass + here <= limit && am < a1) {
             mass += here;
@@ -770,6 +884,7 @@ struct SfSampler {
     r.each_slowly([&](float x, int col) { if (sf_key(x) == key) atomicAdd(&s.hist[col / width], 1u); });
     unsigned m[SF_EACH];
     merged_bins(m);
+    cluster.sync();
     bracket_count(m, n);
     const int bin = s.bin_lo;
     const unsigned before = s.above;
@@ -788,7 +903,311 @@ struct SfSampler {
     return col;
   }
 
-  __device__ void run() {
+  // The draw among the list's tokens down to the border and what the blocks drew above the list; `mass` of all of it.
+  __device__ __noinline__ void finish_blocks(int n, float border, int border_col, double mass) {
+    float best = -INFINITY, best_z = 0.f;
+    int col = -1;
+    for (int i = tid; i < n; i += SF_THREADS) {
+      const unsigned long long e = s.list[i];
+      const float x = sf_entry_x(e);
+      const int at = (int)(unsigned)e;
+      if (!within(x, at, border, border_col)) continue;
+      const float z = quotient(x);
+      sf_better(best, col, best_z, greedy ? x : z + sf_gumbel(sf_bits(word, (uint32_t)at)), at, z);
+    }
+    if (tid < C) sf_better(best, col, best_z, s.bests[tid], s.best_cols[tid], s.best_zs[tid]);
+    sf_block_best(best, col, best_z, s);
+    if (!greedy && (double)best < (double)zmax + log(mass) - 3.) {  // once in 10^8 rows: without the shortcut of the draws
+      SfRow<T> q = r;
+      q.v0 = 0;
+      q.v1 = a.V;
+      best = -INFINITY;
+      col = -1;
+      q.each_slowly([&](float x, int at) {
+        if (x >= -SF_MAX && within(x, at, border, border_col)) {
+          const float z = quotient(x);
+          sf_better(best, col, best_z, z + sf_gumbel(sf_bits(word, (uint32_t)at)), at, z);
+        }
+      });
+      sf_block_best(best, col, best_z, s);
+    }
+    write(best_z, col, mass);
+  }
+
+  // The first block has what it needs of the others, which leave: their places are free for the next row.
+  __device__ __forceinline__ void release(bool draws) {
+    if (draws && rank == 0 && tid < C) {
+      s.bests[tid] = of(tid)->best;
+      s.best_cols[tid] = of(tid)->best_col;
+      s.best_zs[tid] = of(tid)->best_z;
+    }
+    cluster.sync();
+  }
+
+  // The block's columns in shared memory, `vecs` vectors, of which a thread reads what it has written.  False where the row needs
+  // run().
+  __device__ __forceinline__ bool fast(uint4* data, int vecs) {
+    constexpr int N = 16 / sizeof(T);
+    const float top_p = a.top_p ? a.top_p[row] : a.top_p_all, min_p = a.min_p ? a.min_p[row] : a.min_p_all;
+    const int top_k = a.top_k ? a.top_k[row] : a.top_k_all;
+    const bool by_k = top_k > 0 && top_k < a.V, by_p = top_p < 1.f;
+    if (by_k && (top_k > SF_THREADS / 2 || top_k * C > SF_LIST / 2)) return false;  // too many for the lists
+    const int first = r.v0;
+    float mine = -INFINITY;
+    {
+      const SfRow<T> q = r;
+#pragma unroll 4
+      for (int v = tid; v < vecs; v += SF_THREADS) {
+        const int at = first + v * N;
+        uint4 u;
+        if (q.vec && at + N <= q.v1) {
+          u = *reinterpret_cast<const uint4*>(q.x + at);
+        } else {
+          uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+          for (int k = 0; k < N; ++k) {
+            const T y = at + k < q.v1 ? q.x[at + k] : sf_lowest<T>();
+            if constexpr (sizeof(T) == 4) w[k] = __float_as_uint(y);
+            else w[k / 2] |= (uint32_t)*reinterpret_cast<const uint16_t*>(&y) << (16 * (k & 1));
+          }
+          u = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        sf_clean<T>(u, q.cap);
+        float y[N];
+        sf_unpack<T>(u, y);
+#pragma unroll
+        for (int k = 0; k < N; ++k) mine = fmaxf(mine, y[k]);
+        data[v] = u;
+      }
+    }
+    auto each = [&](auto f) {
+#pragma unroll 1
+      for (int v = tid; v < vecs; v += SF_THREADS) {
+        float y[N];
+        sf_unpack<T>(data[v], y);
+#pragma unroll
+        for (int k = 0; k < N; ++k) f(y[k], first + v * N + k);
+      }
+    };
+    SfShared& sh = s;
+    // ---- the maximum of the block, the smallest of its threads' ----
+    const int lane = tid & 31, wid = tid >> 5;
+    const float wmax = warp_max(mine), wmin = -warp_max(mine == -INFINITY ? -INFINITY : -mine);
+    if (lane == 0) { sh.red[0][wid] = wmax; sh.red[1][wid] = wmin; }
+    if (tid == 0) { sh.list_n = 0; sh.bin_lo = SF_BINS; }
+    for (int i = tid; i < SF_BINS; i += SF_THREADS) sh.hist[i] = sh.where[i] = 0;
+    __syncthreads();
+    float bmax = lane < SF_WARPS ? (float)sh.red[0][lane] : -INFINITY, bmin = lane < SF_WARPS ? (float)sh.red[1][lane] : INFINITY;
+    bmax = warp_max(bmax);
+    bmin = -warp_max(-bmin);
+    if (by_k) {
+      // What this block can have among the k largest is not below the k-th largest of its threads' maxima.
+      float from = -SF_MAX;  // all, where fewer than k threads have any
+      const float scale = (float)(SF_BINS - 2) / (bmax - bmin);
+      if (scale < 1e30f) {  // false also where the block has none or all maxima are equal
+        if (mine > -INFINITY) atomicAdd(&sh.hist[(int)fminf((bmax - mine) * scale, (float)(SF_BINS - 1))], 1u);
+        unsigned h[SF_EACH];
+        own_bins(h);
+        bracket_count(h, (unsigned)top_k);
+        if (sh.bin_lo < SF_BINS - 1) from = fmaxf(from, bmax - (float)(sh.bin_lo + 1) / scale * 1.000001f);  // a little below the bin's end
+      }
+      each([&](float x, int col) {
+        if (x >= from) append(sh, x, col);
+      });
+      if (tid == 0) sh.fmax = bmax;
+      const int n = collect();
+      if (n == 0) return false;  // none at all, or too many
+      xmax = max_of([](const SfShared& o) { return o.fmax; });
+      zmax = quotient(xmax);
+      if (n < top_k) return false;
+      release(false);
+      if (rank == 0) top_k_of_list(n, top_k, by_p, top_p, min_p > 0.f ? least_logit(min_p) : -INFINITY);
+      return true;
+    }
+    // ---- the mass relative to the block's maximum; then both for the row ----
+    double total;
+    {
+      const float k = c;
+      float part = 0.f;
+      if (bmax > -INFINITY) each([&](float x, int) { part += exp2f((x - bmax) * k); });
+      const double sum = sf_block_sum((double)part, sh);
+      if (tid == 0) { sh.fmax = bmax; sh.sums[0] = sum; }
+      cluster.sync();
+      xmax = max_of([](const SfShared& o) { return o.fmax; });
+      if (xmax == -INFINITY) return false;
+      zmax = quotient(xmax);
+      total = sum_of([&](const SfShared& o) { return o.fmax > -INFINITY ? o.sums[0] * (double)exp2f((o.fmax - xmax) * c) : 0.; });
+    }
+    const Pass q = pass();
+    const float floor = min_p > 0.f ? least_logit(min_p) : -INFINITY;
+    if (!by_p) {
+      double mass = total;
+      if (floor > -INFINITY) {
+        float part = 0.f;
+        each([&](float x, int) { part += x >= floor ? q.weight(x) : 0.f; });
+        const double sum = sf_block_sum((double)part, sh);
+        if (tid == 0) sh.sums[1] = sum;
+        cluster.sync();
+        mass = sum_of([](const SfShared& o) { return o.sums[1]; });
+      }
+      draw(each, q, mass, floor);
+      cluster.sync();
+      release(true);
+      if (rank == 0) finish_blocks(0, fmaxf(floor, -SF_MAX), 0x7fffffff, mass);
+      return true;
+    }
+    // ---- top-p ----
+    // lighter tokens than this together have less than what top-p leaves out; a little is added for the sums' rounding
+    const double goal = fmax(0., (double)top_p * total), least = (1. - (double)top_p - 2e-5) * total / a.V;
+    if (!(least > 0.)) return false;
+    const float from = fmaxf(-SF_MAX, xmax + (logf((float)least) - 1e-3f) * temperature);
+    // weights are at most 1: at least `goal` tokens are kept, and with many of them come more than the list holds
+    if (goal < SF_LIST / 16) {
+      each([&](float x, int col) {
+        if (x >= from) append(sh, x, col);
+      });
+      const int n = collect();
+      if (n > 0) {
+        release(false);
+        if (rank == 0) {
+          list_border(n, true, goal, 0, 0.);
+          finish_list(n, sh.border, sh.border_col, floor);
+        }
+        return true;
+      }
+      cluster.sync();  // the numbers of the lists have been read
+      if (tid == 0) sh.list_n = 0;
+    }
+    if (floor > -INFINITY) return false;
+    set_step(from);
+    const Pass h = pass();
+    each([&](float x, int) {
+      if (x >= from) {
+        const float y = (h.xmax - x) * h.step;
+        const int bin = (int)fminf(y, (float)(SF_BINS - 1));
+        atomicAdd(&sh.hist[bin], 1u);
+        atomicAdd(&sh.where[bin], (unsigned)fminf((y - (float)bin) * SF_FINE, SF_FINE));
+      }
+    });
+    cluster.sync();
+    if (rank == 0) {  // one block's reads of all tables are faster than those of eight
+      unsigned n[SF_EACH], place[SF_EACH];
+      merge([](const SfShared& o) { return o.hist; }, n);
+      merge([](const SfShared& o) { return o.where; }, place);
+      float hi[SF_EACH], lo[SF_EACH];
+      placed_bounds(n, place, hi, lo);
+      bracket_mass(n, hi, lo, 0., goal, false);
+    }
+    cluster.sync();
+    const int b0 = lead->bin_lo, b1 = lead->bin_hi;
+    const unsigned above = lead->above;
+    if (lead->upto - above > SF_LIST) return false;
+    // above the bracket: the mass, and the draw (at least `goal` is kept); the bracket: listed
+    {
+      const float reach = (float)(4294967296. * 20.0855369 * 1.001 / goal), t = temperature;
+      const uint32_t w = word;
+      const bool most = greedy;
+      float part = 0.f, top = -INFINITY, top_z = 0.f;
+      int at = -1;
+      each([&](float x, int col) {
+        if (x < from) return;
+        const int b = h.linear_bin(x);
+        if (b < b0) {
+          const float wt = h.weight(x);
+          part += wt;
+          consider(x, col, wt, reach, t, w, most, top, at, top_z);
+        } else if (b <= b1) {
+          append(sh, x, col);
+        }
+      });
+      if (most && at >= 0) top_z = quotient(top_z);
+      const double sum = sf_block_sum((double)part, sh);
+      sf_block_best(top, at, top_z, sh);
+      if (tid == 0) {
+        sh.sums[1] = sum;
+        sh.best = top;
+        sh.best_col = at;
+        sh.best_z = top_z;
+      }
+    }
+    const int n = collect();
+    const double mass = sum_of([](const SfShared& o) { return o.sums[1]; });
+    release(true);
+    if (rank == 0) {
+      list_border(n, true, goal, above, mass);
+      finish_blocks(n, sh.border, sh.border_col, sh.kept);
+    }
+    return true;
+  }
+  static __device__ __forceinline__ void append(SfShared& sh, float x, int col) {
+    const unsigned i = atomicAdd(&sh.list_n, 1u);
+    if (i < SF_LIST) sh.list[i] = (unsigned long long)(~sf_key(x)) << 32 | (unsigned)col;
+  }
+  // One token's chance in a draw.  The largest z - log(-log u) of the kept tokens is lse + a Gumbel variate, which is below
+  // lse - 3 once in 10^8 rows.  A token reaches K = lse - 3 only if -log u <= exp(z - K), and -log u >= 1 - u: most are out
+  // after their random bits.
+  static __device__ __forceinline__ void consider(float x, int col, float weight, float reach, float t, uint32_t word, bool most,
+                                                  float& top, int& at, float& top_z) {
+    float z = x, k = x;
+    if (!most) {
+      const uint32_t h = sf_bits(word, (uint32_t)col);
+      if ((float)(~h) > reach * weight) return;
+      z = sf_quotient(x, t);
+      k = z + sf_gumbel(h);
+    }
+    if (at < 0 || k > top || (k == top && col < at)) { top = k; at = col; top_z = z; }
+  }
+  // This block's draw among its tokens of at least `floor`.
+  template <typename E>
+  __device__ __forceinline__ void draw(E each, const Pass& q, double mass, float floor) {
+    const float reach = (float)(4294967296. * 20.0855369 * 1.001 / mass), t = temperature, from = fmaxf(floor, -SF_MAX);
+    const uint32_t w = word;
+    const bool most = greedy;
+    float top = -INFINITY, top_z = 0.f;
+    int at = -1;
+    each([&](float x, int col) {
+      if (x >= from) consider(x, col, q.weight(x), reach, t, w, most, top, at, top_z);
+    });
+    if (most && at >= 0) top_z = quotient(top_z);
+    sf_block_best(top, at, top_z, s);
+    if (tid == 0) { s.best = top; s.best_col = at; s.best_z = top_z; }
+  }
+  // The smallest logit that min-p keeps.
+  __device__ __noinline__ float least_logit(float min_p) const {
+    const double least = (double)zmax + log((double)min_p);
+    float floor = fminf(xmax, (float)(least * (double)temperature));
+    // the quotients, rounded, decide: at most a few logits around the product are on its wrong side
+    for (int i = 0; i < 8 && (double)quotient(nextafterf(floor, -INFINITY)) >= least; ++i) floor = nextafterf(floor, -INFINITY);
+    for (int i = 0; i < 8 && (double)quotient(floor) < least && floor < xmax; ++i) floor = nextafterf(floor, INFINITY);
+    return fminf(floor, xmax);
+  }
+  // The first block: top-k, then top-p, then the draw, in a list that holds the k largest.
+  __device__ __noinline__ void top_k_of_list(int n, int top_k, bool by_p, float top_p, float floor) {
+    list_border(n, false, (double)top_k, 0, 0.);
+    const float border = s.border;
+    if (by_p) {
+      // of the k-th and its equals, which move to the front
+      __syncthreads();
+      if (tid == 0) s.list_n = 0;
+      constexpr int E = SF_LIST / SF_THREADS;
+      unsigned long long e[E], w = 0;
+#pragma unroll
+      for (int i = 0; i < E; ++i) e[i] = tid + i * SF_THREADS < n ? s.list[tid + i * SF_THREADS] : ~0ull;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (tid + i * SF_THREADS < n && sf_entry_x(e[i]) >= border) {
+          w += whole((double)weight(sf_entry_x(e[i])));
+          s.list[atomicAdd(&s.list_n, 1u)] = e[i];
+        }
+      const double mass = (double)sf_block_count(w, s) / SF_UNIT;
+      n = (int)s.list_n;
+      list_border(n, true, fmax(0., (double)top_p * mass), 0, 0.);
+    }
+    finish_list(n, s.border, s.border_col, floor);
+  }
+
+  __device__ __noinline__ void run() {
     const float top_p = a.top_p ? a.top_p[row] : a.top_p_all, min_p = a.min_p ? a.min_p[row] : a.min_p_all;
     const int top_k = a.top_k ? a.top_k[row] : a.top_k_all;
     const bool by_k = top_k > 0 && top_k < a.V, by_p = top_p < 1.f;
@@ -816,25 +1235,14 @@ struct SfSampler {
       s.first_mass = sum;
     }
     cluster.sync();
-    xmax = -INFINITY;
-    for (int b = 0; b < C; ++b) xmax = fmaxf(xmax, of(b)->fmax);
+    xmax = max_of([](const SfShared& o) { return o.fmax; });
     if (xmax == -INFINITY) {  // nothing to draw from
       if (rank == 0 && tid == 0) { a.tok[row] = 0; a.logp[row] = -INFINITY; }
       return;
     }
     zmax = quotient(xmax);
-    double total = 0.;
-    for (int b = 0; b < C; ++b)
-      if (of(b)->fmax > -INFINITY) total += of(b)->first_mass * (double)exp2f((of(b)->fmax - xmax) * c);
-    float floor = -INFINITY;  // min-p, as the smallest logit that it keeps
-    if (min_p > 0.f) {
-      const double least = (double)zmax + log((double)min_p);
-      floor = fminf(xmax, (float)(least * (double)temperature));
-      // the quotients, rounded, decide: at most a few logits around the product are on its wrong side
-      for (int i = 0; i < 8 && (double)quotient(nextafterf(floor, -INFINITY)) >= least; ++i) floor = nextafterf(floor, -INFINITY);
-      for (int i = 0; i < 8 && (double)quotient(floor) < least && floor < xmax; ++i) floor = nextafterf(floor, INFINITY);
-      floor = fminf(floor, xmax);
-    }
+    const double total = sum_of([&](const SfShared& o) { return o.fmax > -INFINITY ? o.first_mass * (double)exp2f((o.fmax - xmax) * c) : 0.; });
+    const float floor = min_p > 0.f ? least_logit(min_p) : -INFINITY;
     float border = -INFINITY;
     int border_col = 0x7fffffff;
     double kept = 0.;
@@ -847,6 +1255,7 @@ struct SfSampler {
         if (mine > -INFINITY) atomicAdd(&s.hist[pass().linear_bin(mine)], 1u);
         unsigned h[SF_EACH];
         merged_bins(h);
+        cluster.sync();
         if (tid == 0) s.bin_lo = SF_BINS;
         __syncthreads();
         bracket_count(h, (unsigned)top_k);
@@ -860,30 +1269,7 @@ struct SfSampler {
       double goal = (double)top_k;
       if (n == 0) n = search(false, goal, false, -INFINITY, border, border_col, kept);
       if (n > 0) {
-        if (rank == 0) {
-          list_border(n, false, (double)top_k, 0, 0.);
-          border = s.border;
-          if (by_p) {
-            // of the k-th and its equals, which move to the front
-            __syncthreads();
-            if (tid == 0) s.list_n = 0;
-            constexpr int E = SF_LIST / SF_THREADS;
-            unsigned long long e[E], w = 0;
-#pragma unroll
-            for (int i = 0; i < E; ++i) e[i] = tid + i * SF_THREADS < n ? s.list[tid + i * SF_THREADS] : ~0ull;
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < E; ++i)
-              if (tid + i * SF_THREADS < n && sf_entry_x(e[i]) >= border) {
-                w += whole((double)weight(sf_entry_x(e[i])));
-                s.list[atomicAdd(&s.list_n, 1u)] = e[i];
-              }
-            const double mass = (double)sf_block_count(w, s) / SF_UNIT;
-            n = (int)s.list_n;
-            list_border(n, true, fmax(0., (double)top_p * mass), 0, 0.);
-          }
-          finish_list(n, s.border, s.border_col, floor);
-        }
+        if (rank == 0) top_k_of_list(n, top_k, by_p, top_p, floor);
         return;
       }
     }
@@ -923,11 +1309,10 @@ struct SfSampler {
       });
       mass = cluster_sum((double)part);
     }
-    // The largest z - log(-log u) of n tokens is lse + a Gumbel variate, which is below lse - 3 once in 10^8 rows.  A token
-    // reaches K = lse - 3 only if -log u <= exp(z - K), and -log u >= 1 - u: most are out after their random bits.
+    const double reached = (double)zmax + log(mass) - 3.;
     float best = -INFINITY, best_z = 0.f;
     int col = -1;
-    for (int turn = 0; turn < 2 && col < 0; ++turn) {
+    for (int turn = 0; turn < 2 && (col < 0 || (!greedy && (double)best < reached)); ++turn) {
       const Pass q = pass();
       const float reach = turn == 1 ? INFINITY : (float)(4294967296. * 20.0855369 * 1.001 / mass), last = fmaxf(border, -SF_MAX), t = temperature;
       const int last_col = border == -INFINITY ? 0x7fffffff : border_col;
@@ -936,15 +1321,7 @@ struct SfSampler {
       float top = -INFINITY, top_z = 0.f;
       int at = -1;
       q.r.each([&](float x, int i) {
-        if (!within(x, i, last, last_col)) return;
-        float z = x, k = x;
-        if (!most) {
-          const uint32_t h = sf_bits(w, (uint32_t)i);
-          if ((float)(~h) > reach * q.weight(x)) return;
-          z = sf_quotient(x, t);
-          k = z + sf_gumbel(h);
-        }
-        if (at < 0 || k > top || (k == top && i < at)) { top = k; at = i; top_z = z; }
+        if (within(x, i, last, last_col)) consider(x, i, q.weight(x), reach, t, w, most, top, at, top_z);
       });
       best = top;
       best_z = top_z;
@@ -960,9 +1337,11 @@ struct SfSampler {
   }
 };
 
+constexpr size_t SF_HEAD = (sizeof(SfShared) + 15) / 16 * 16;
+// vecs: vectors of a row in each block's shared memory, 0: the row is too large for that.
 template <typename T>
 __global__ void __launch_bounds__(SF_THREADS, 2)
-sample_filtered_kernel(const __grid_constant__ SampleArgs a) {
+sample_filtered_kernel(const __grid_constant__ SampleArgs a, int vecs) {
   extern __shared__ __align__(16) unsigned char raw[];
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), row = blockIdx.x / C;
@@ -986,22 +1365,29 @@ sample_filtered_kernel(const __grid_constant__ SampleArgs a) {
   f.row = row;
   f.tid = threadIdx.x;
   f.lead = cluster.map_shared_rank(&f.s, 0);
-  f.run();
-  cluster.sync();  // no block leaves while another may read its shared memory
+  bool done = false;
+  if (vecs > 0) done = f.fast(reinterpret_cast<uint4*>(raw + SF_HEAD), vecs);
+  if (done) return;  // the others may have left already
+  f.run();           // all blocks of a cluster take the same way
+  cluster.sync();    // no block leaves while another may read its shared memory
 }
 
 template <typename T>
 int sample_filtered_launch(const SampleArgs& a, int B, cudaStream_t st) {
-  // blocks a row: up to two an SM, and up to the 8 of a portable cluster
+  // Blocks a row: enough for the row to fit into their shared memory, two blocks an SM, up to the 8 of a portable cluster; more
+  // while there are fewer than two an SM.
+  constexpr long long N = 16 / sizeof(T);
   int C = 1;
-  while (C < 8 && C * B <= trlb_host::sm_count()) C *= 2;
-  const size_t smem = sizeof(SfShared);
-  cudaError_t e = cudaFuncSetAttribute(sample_filtered_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  while (C < 8 && (C * N * SF_HELD < a.V || (long long)C * B <= trlb_host::sm_count())) C *= 2;
+  const long long need = ((a.V + C - 1) / C + N - 1) / N;
+  const int vecs = need <= SF_HELD ? (int)need : 0;
+  cudaError_t e = cudaFuncSetAttribute(sample_filtered_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)(SF_HEAD + SF_HELD * 16));
   if (e != cudaSuccess) return (int)e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(B * C));
   cfg.blockDim = dim3(SF_THREADS);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = SF_HEAD + (size_t)vecs * 16;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1011,7 +1397,7 @@ int sample_filtered_launch(const SampleArgs& a, int B, cudaStream_t st) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = trlb_host::pdl_enabled() ? 2 : 1;
-  return (int)cudaLaunchKernelEx(&cfg, sample_filtered_kernel<T>, a);
+  return (int)cudaLaunchKernelEx(&cfg, sample_filtered_kernel<T>, a, vecs);
 }
 
 }  // namespace trlb
