@@ -163,3 +163,39 @@ def test_sampling_refuses(kw, message):
     a = {"logits": torch.zeros(3, 5), "rng": torch.zeros(3, dtype=torch.int32), **kw}
     with pytest.raises(ValueError, match=message):
         K.sample_filtered(a.pop("logits"), a.pop("rng"), **a)
+
+
+def test_an_engine_refuses_what_the_8_bit_cache_does_not_cover():
+    from trl_b200.generation.generation import RolloutGeneration
+    from trl_b200.rollout.engine import RolloutEngine
+    from trl_b200.rollout.layered_engine import LayeredRolloutEngine
+    from trl_b200.testing import make_tiny_model
+
+    model = make_tiny_model("tiny-qwen2", head_dim=64)
+    with pytest.raises(ValueError, match="kv_cache_dtype='int4'"):
+        RolloutEngine(model, kv_cache_dtype="int4")
+    with pytest.raises(ValueError, match="needs a GPU"):
+        RolloutGeneration(model, kv_cache_dtype="fp8")
+    eng = RolloutEngine.__new__(RolloutEngine)
+    eng.model, eng.cfg, eng.tp, eng.kv8 = model, model.config, 1, True
+    assert eng._check_model(128, None) == 64 and eng._check_model(128, 16) == 16 and not eng.attn_tc
+    with pytest.raises(ValueError, match="16, 32, 64 or 128"):
+        eng._check_model(128, 48)
+    eng.tp = 2
+    with pytest.raises(NotImplementedError, match="tensor parallel"):
+        eng._check_model(128, None)
+    eng = LayeredRolloutEngine.__new__(LayeredRolloutEngine)
+    eng.model, eng.cfg, eng.tp, eng.kv8 = model, model.config, 1, True
+    with pytest.raises(NotImplementedError, match="8-bit cache"):
+        eng._check_model(128, None)
+
+
+def test_a_trainer_on_the_cpu_refuses_an_8_bit_cache(tmp_path):
+    from types import SimpleNamespace
+
+    from trl_b200.trainer.grpo_config import GRPOConfig
+    from trl_b200.trainer.online_base import OnlineTrainer
+
+    args = GRPOConfig(output_dir=str(tmp_path), rollout_kv_cache_dtype="fp8", use_cpu=True)
+    with pytest.raises(ValueError, match="rollout_kv_cache_dtype needs a GPU"):
+        OnlineTrainer._get_rollout(SimpleNamespace(args=args, model=None, _rollout=None))

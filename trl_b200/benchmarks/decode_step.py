@@ -19,6 +19,8 @@ def main():
     ap.add_argument("--batch", type=int, default=64)
     ap.add_argument("--ctx", type=int, default=512)
     ap.add_argument("--steps", type=int, default=4)
+    ap.add_argument("--kv-cache-dtype", default="auto")
+    ap.add_argument("--top-p", type=float, default=1.0)
     a = ap.parse_args()
     from torch.profiler import ProfilerActivity, profile
 
@@ -31,9 +33,9 @@ def main():
     model = CausalLM(cfg, dtype=torch.bfloat16, device="cuda").eval()
     n, new = 8, 64
     plen = a.ctx - new
-    eng = RolloutEngine(model, max_num_seqs=a.batch, max_model_len=a.ctx + 16, poll_every=16)
+    eng = RolloutEngine(model, max_num_seqs=a.batch, max_model_len=a.ctx + 16, poll_every=16, kv_cache_dtype=a.kv_cache_dtype)
     prompts = [torch.randint(2, cfg.vocab_size, (plen,)).tolist() for _ in range(a.batch // n)]
-    sp = SamplingParams(n=n, max_tokens=new, eos_token_id=None, seed=1)
+    sp = SamplingParams(n=n, max_tokens=new, eos_token_id=None, seed=1, top_p=a.top_p)
     eng.generate(prompts, sp)  # fills the cache and captures the graph
 
     def reset(frac=1.0):

@@ -34,7 +34,7 @@ EXACT_MATH = {"grouped_attn.cu", "hgrn2.cu", "hgrn2_chunk_tcgen05.cu", "kv8.cu",
 
 # Parts of the kernel library that can be built alone.  "layered": what every layered decoder needs, and the sources of the
 # mixers and feed-forwards it has.
-PARTS = {"layered": ("decode.cu", "decode_gemm.cu", "mixers.cu", "tensormap.cu")}
+PARTS = {"layered": ("decode.cu", "decode_gemm.cu", "mixers.cu", "sample_filtered.cu", "tensormap.cu")}
 _GROUPED = ("grouped_attn.cu", "grouped_decode_tcgen05.cu", "mixer_attn_tcgen05.cu")
 LAYERED_KINDS = {"latent_attention": ("grouped_attn.cu", "latent_decode_tcgen05.cu", "mixer_attn_tcgen05.cu"),
                  "mlstm": ("mlstm_chunk_tcgen05.cu",), "attention": _GROUPED, "attention_2": _GROUPED,

@@ -76,6 +76,12 @@ __device__ __noinline__ float sf_gumbel(uint32_t h) {
   return -logf(e);
 }
 __device__ __forceinline__ float sf_quotient(float x, float t) { return fminf(__fdiv_rn(x, t), SF_MAX); }
+// The same from the 24-bit numbers and fast logarithms of trlb_sample, so that one seed gives the same draws there and here.
+// (The largest number rounds to 1, whose logarithm would let its token win whatever its logit: it counts as 1 - 2^-25.)
+__device__ __forceinline__ float sf_gumbel_as_sampler(uint32_t h) {
+  const float u = ((float)(h >> 8) + 0.5f) * (1.0f / 16777216.0f);
+  return -__logf(fmaxf(-__logf(u), 2.98023224e-8f));
+}
 // Orders floats as unsigned integers.
 __device__ __forceinline__ uint32_t sf_key(float x) {
   const uint32_t u = __float_as_uint(x);
@@ -325,7 +331,7 @@ struct SfSampler {
   float xmax, zmax;
   float step;             // bins of the linear histogram per unit of the logits
   uint32_t word;
-  bool greedy;
+  bool greedy, as_sampler;  // the latter: random numbers as trlb_sample makes them
   SfShared* lead;
 
   __device__ __forceinline__ SfShared* of(int c) { return cluster.map_shared_rank(&s, c); }
@@ -338,6 +344,7 @@ struct SfSampler {
   };
   __device__ __forceinline__ Pass pass() const { return {r, xmax, c, step}; }
   __device__ __forceinline__ float weight(float x) const { return exp2f((x - xmax) * c); }
+  __device__ __forceinline__ float noise(uint32_t h) const { return as_sampler ? sf_gumbel_as_sampler(h) : sf_gumbel(h); }
   __device__ __forceinline__ float quotient(float x) const { return sf_quotient(x, temperature); }
   // Bins that reach down to `from`, where that is not too far.
   __device__ __forceinline__ void set_step(float from) {
@@ -697,7 +704,7 @@ struct SfSampler {
       if (x < floor || !within(x, at, border, border_col)) continue;
       const float z = quotient(x);
       sum += whole((double)expf(z - zmax));
-      sf_better(best, col, best_z, greedy ? z : z + sf_gumbel(sf_bits(word, (uint32_t)at)), at, z);
+      sf_better(best, col, best_z, greedy ? z : z + noise(sf_bits(word, (uint32_t)at)), at, z);
     }
     sum = sf_block_count(sum, s);
     sf_block_best(best, col, best_z, s);
@@ -913,7 +920,7 @@ struct SfSampler {
       const int at = (int)(unsigned)e;
       if (!within(x, at, border, border_col)) continue;
       const float z = quotient(x);
-      sf_better(best, col, best_z, greedy ? x : z + sf_gumbel(sf_bits(word, (uint32_t)at)), at, z);
+      sf_better(best, col, best_z, greedy ? x : z + noise(sf_bits(word, (uint32_t)at)), at, z);
     }
     if (tid < C) sf_better(best, col, best_z, s.bests[tid], s.best_cols[tid], s.best_zs[tid]);
     sf_block_best(best, col, best_z, s);
@@ -926,7 +933,7 @@ struct SfSampler {
       q.each_slowly([&](float x, int at) {
         if (x >= -SF_MAX && within(x, at, border, border_col)) {
           const float z = quotient(x);
-          sf_better(best, col, best_z, z + sf_gumbel(sf_bits(word, (uint32_t)at)), at, z);
+          sf_better(best, col, best_z, z + noise(sf_bits(word, (uint32_t)at)), at, z);
         }
       });
       sf_block_best(best, col, best_z, s);
@@ -1106,7 +1113,7 @@ struct SfSampler {
     {
       const float reach = (float)(4294967296. * 20.0855369 * 1.001 / goal), t = temperature;
       const uint32_t w = word;
-      const bool most = greedy;
+      const bool most = greedy, as = as_sampler;
       float part = 0.f, top = -INFINITY, top_z = 0.f;
       int at = -1;
       each([&](float x, int col) {
@@ -1115,7 +1122,7 @@ struct SfSampler {
         if (b < b0) {
           const float wt = h.weight(x);
           part += wt;
-          consider(x, col, wt, reach, t, w, most, top, at, top_z);
+          consider(x, col, wt, reach, t, w, most, as, top, at, top_z);
         } else if (b <= b1) {
           append(sh, x, col);
         }
@@ -1147,13 +1154,14 @@ struct SfSampler {
   // lse - 3 once in 10^8 rows.  A token reaches K = lse - 3 only if -log u <= exp(z - K), and -log u >= 1 - u: most are out
   // after their random bits.
   static __device__ __forceinline__ void consider(float x, int col, float weight, float reach, float t, uint32_t word, bool most,
-                                                  float& top, int& at, float& top_z) {
+                                                  bool as_sampler, float& top, int& at, float& top_z) {
     float z = x, k = x;
     if (!most) {
       const uint32_t h = sf_bits(word, (uint32_t)col);
-      if ((float)(~h) > reach * weight) return;
+      // 2^13: what 24 bits and fast logarithms may make of 1 - u, 2^-20 at most
+      if ((float)(~h) > reach * weight + (as_sampler ? 8192.f : 0.f)) return;
       z = sf_quotient(x, t);
-      k = z + sf_gumbel(h);
+      k = z + (as_sampler ? sf_gumbel_as_sampler(h) : sf_gumbel(h));
     }
     if (at < 0 || k > top || (k == top && col < at)) { top = k; at = col; top_z = z; }
   }
@@ -1162,11 +1170,11 @@ struct SfSampler {
   __device__ __forceinline__ void draw(E each, const Pass& q, double mass, float floor) {
     const float reach = (float)(4294967296. * 20.0855369 * 1.001 / mass), t = temperature, from = fmaxf(floor, -SF_MAX);
     const uint32_t w = word;
-    const bool most = greedy;
+    const bool most = greedy, as = as_sampler;
     float top = -INFINITY, top_z = 0.f;
     int at = -1;
     each([&](float x, int col) {
-      if (x >= from) consider(x, col, q.weight(x), reach, t, w, most, top, at, top_z);
+      if (x >= from) consider(x, col, q.weight(x), reach, t, w, most, as, top, at, top_z);
     });
     if (most && at >= 0) top_z = quotient(top_z);
     sf_block_best(top, at, top_z, s);
@@ -1317,11 +1325,11 @@ struct SfSampler {
       const float reach = turn == 1 ? INFINITY : (float)(4294967296. * 20.0855369 * 1.001 / mass), last = fmaxf(border, -SF_MAX), t = temperature;
       const int last_col = border == -INFINITY ? 0x7fffffff : border_col;
       const uint32_t w = word;
-      const bool most = greedy;
+      const bool most = greedy, as = as_sampler;
       float top = -INFINITY, top_z = 0.f;
       int at = -1;
       q.r.each([&](float x, int i) {
-        if (within(x, i, last, last_col)) consider(x, i, q.weight(x), reach, t, w, most, top, at, top_z);
+        if (within(x, i, last, last_col)) consider(x, i, q.weight(x), reach, t, w, most, as, top, at, top_z);
       });
       best = top;
       best_z = top_z;
@@ -1359,6 +1367,7 @@ sample_filtered_kernel(const __grid_constant__ SampleArgs a, int vecs) {
   f.c = SF_LOG2E / f.temperature;
   f.r.cap = SF_MAX * fminf(f.temperature, 1.f);
   f.greedy = !(temp > 0.f);
+  f.as_sampler = a.words == nullptr;
   f.word = a.words ? a.words[row] : a.seed ^ sf_hash((a.step_ptr ? (uint32_t)*a.step_ptr : 0u) * 0x9E3779B9U + (uint32_t)row);
   f.C = C;
   f.rank = rank;

@@ -24,7 +24,7 @@ def extract_logprobs(outputs):
 class RolloutGeneration:
     def __init__(self, model, mode: str = "colocate", tensor_parallel_size: int = 1, max_num_seqs: int = 64,
                  max_model_len: int = 2048, server_base_url=None, server_host="127.0.0.1", server_port=8000,
-                 server_timeout: float = 240.0, **kw):
+                 server_timeout: float = 240.0, kv_cache_dtype: str = "auto", **kw):
         self.model, self.mode = model, mode
         if mode == "server":
             self.client = None
@@ -38,8 +38,10 @@ class RolloutGeneration:
             if model.device.type == "cuda":
                 from ..rollout.engine import make_engine
 
-                self.engine = make_engine(model, max_num_seqs, max_model_len)
+                self.engine = make_engine(model, max_num_seqs, max_model_len, kv_cache_dtype=kv_cache_dtype)
             else:
+                if kv_cache_dtype != "auto":
+                    raise ValueError(f"kv_cache_dtype={kv_cache_dtype!r} needs a GPU: the eager generator caches nothing")
                 from ..rollout.engine import EagerGenerator
 
                 self.engine = EagerGenerator(model)

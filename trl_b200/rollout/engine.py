@@ -99,10 +99,12 @@ class EagerGenerator:
 
 
 class _PrefillKV:
-    """Attention hook used during prefill: append K/V to the paged cache, then varlen attention."""
+    """Attention hook used during prefill: append K/V to the paged cache, then varlen attention.  (With an 8-bit cache the
+    prompt's own attention still reads the unrounded keys and values.)"""
 
-    def __init__(self, engine: "RolloutEngine", tok_slot, tok_pos):
+    def __init__(self, engine: "RolloutEngine", tok_slot, tok_pos, slots=None):
         self.e, self.tok_slot, self.tok_pos = engine, tok_slot, tok_pos
+        self.slots, self.starts = slots, None if slots is None else torch.zeros_like(slots)
 
     def attend(self, layer_idx, q, k, v, ctx):
         from ..ops import cuda as K
@@ -113,8 +115,12 @@ class _PrefillKV:
             kw, vw = k[:, sl].contiguous(), v[:, sl].contiguous()
         else:
             kw, vw = k.contiguous(), v.contiguous()
-        K.kv_write_prefill(kw, vw, self.tok_slot, self.tok_pos, e.block_table, e.block_size,
-                           e.k_cache[layer_idx], e.v_cache[layer_idx], v_transposed=e.attn_tc)
+        if e.kv8:
+            K.kv8_append(kw, vw, *e.cache8(layer_idx), e.block_table, self.starts, cu_seqlens=ctx.cu_seqlens, slots=self.slots,
+                         max_new=ctx.max_seqlen)
+        else:
+            K.kv_write_prefill(kw, vw, self.tok_slot, self.tok_pos, e.block_table, e.block_size,
+                               e.k_cache[layer_idx], e.v_cache[layer_idx], v_transposed=e.attn_tc)
         return K.attention_varlen(q, k, v, ctx.cu_seqlens, ctx.max_seqlen, True)
 
 
@@ -125,7 +131,9 @@ class RolloutEngine:
         """q_buf x paged KV of layer ``li`` -> attn_buf (tcgen05 kernel when the cache layout allows it)."""
         from ..ops import cuda as K
 
-        if self.attn_tc:
+        if self.kv8:
+            K.kv8_decode_attn(self.q_buf, *self.cache8(li), self.block_table, self.seq_lens, scale, out=self.attn_buf)
+        elif self.attn_tc:
             K.paged_decode_attn_tc(self.q_buf, self.k_cache[li], self.v_cache[li], self.seq_lens, None, self.block_table,
                                    scale, self.kv_splits, self.part_o, self.part_ml, self.attn_buf,
                                    groups=self.attn_groups)
@@ -135,7 +143,12 @@ class RolloutEngine:
 
     def __init__(self, model: CausalLM, max_num_seqs: int = 64, max_model_len: int = 2048, block_size: int | None = None,
                  num_blocks: int | None = None, poll_every: int = 16, use_cuda_graph: bool = True, kv_splits: int = 0,
-                 tp: int = 1, tp_rank: int = 0):
+                 tp: int = 1, tp_rank: int = 0, kv_cache_dtype: str = "auto"):
+        """``kv_cache_dtype``: "auto" keeps keys and values in the model's type, "fp8" in 8 bits with a scale per page and head
+        (half the memory, so twice the tokens in the same pages)."""
+        if kv_cache_dtype not in ("auto", "fp8", "fp8_e4m3"):
+            raise ValueError(f"kv_cache_dtype={kv_cache_dtype!r}: the cache is kept in the model's type ('auto') or in 'fp8'")
+        self.kv8 = kv_cache_dtype != "auto"
         # vision-language model: the decoder runs here; image features are spliced into the prefill embeddings
         self.vlm = model if getattr(model, "is_vlm", False) else None
         if self.vlm is not None:
@@ -195,6 +208,13 @@ class RolloutEngine:
                                       f"{cfg.sliding_window} < max_model_len={max_model_len}; use EagerGenerator")
         # head_dim 128 with at most 8 query heads per KV head: tensor-core decode attention, which wants 64-token
         # pages and V transposed inside a page; anything else keeps 16-token pages and the CUDA-core kernel
+        if self.kv8:
+            if self.tp > 1:
+                raise NotImplementedError("an 8-bit cache under tensor parallel decode")
+            if block_size not in (None, 16, 32, 64, 128):
+                raise ValueError(f"pages of an 8-bit cache hold 16, 32, 64 or 128 tokens, not {block_size}")
+            self.attn_tc = False
+            return block_size or 64
         tc_ok = cfg.head_dim == 128 and self.hq_local // self.hk_local <= 8
         if not block_size:
             block_size = 64 if tc_ok else 16
@@ -207,9 +227,15 @@ class RolloutEngine:
         cfg, tp, max_num_seqs, block_size = self.cfg, self.tp, self.max_seqs, self.block_size
         L, Hk, D = cfg.num_hidden_layers, self.hk_local, cfg.head_dim
         dt = torch.bfloat16
-        self.k_cache = [torch.zeros(self.num_blocks, block_size, Hk, D, dtype=dt, device=self.dev) for _ in range(L)]
-        v_shape = (self.num_blocks, Hk, D, block_size) if self.attn_tc else (self.num_blocks, block_size, Hk, D)
-        self.v_cache = [torch.zeros(*v_shape, dtype=dt, device=self.dev) for _ in range(L)]
+        if self.kv8:
+            from ..ops.functional import kv8_alloc
+
+            per_layer = [kv8_alloc(self.num_blocks, Hk, block_size, D, self.dev) for _ in range(L)]
+            self.k_cache, self.v_cache, self.k_scale, self.v_scale = map(list, zip(*per_layer))
+        else:
+            self.k_cache = [torch.zeros(self.num_blocks, block_size, Hk, D, dtype=dt, device=self.dev) for _ in range(L)]
+            v_shape = (self.num_blocks, Hk, D, block_size) if self.attn_tc else (self.num_blocks, block_size, Hk, D)
+            self.v_cache = [torch.zeros(*v_shape, dtype=dt, device=self.dev) for _ in range(L)]
         # enough CTAs for ~4 per SM: the kernel is latency-bound on KV loads, occupancy hides it
         self.kv_splits = kv_splits or max(1, min(8, -(-(4 * 148) // max(1, max_num_seqs * Hk))))
         if self.attn_tc and not kv_splits:  # persistent CTAs, one per SM: split only to give every SM an item
@@ -247,8 +273,14 @@ class RolloutEngine:
 
     def _copy_pages(self, dst: torch.Tensor, src: torch.Tensor):
         for li in range(self.cfg.num_hidden_layers):
-            self.k_cache[li].index_copy_(0, dst, self.k_cache[li].index_select(0, src))
-            self.v_cache[li].index_copy_(0, dst, self.v_cache[li].index_select(0, src))
+            for t in self.cache8(li) if self.kv8 else (self.k_cache[li], self.v_cache[li]):
+                if t.dtype == torch.float8_e4m3fn:
+                    t = t.view(torch.uint8)
+                t.index_copy_(0, dst, t.index_select(0, src))
+
+    def cache8(self, li: int):
+        """Codes and scales of layer ``li``'s 8-bit cache."""
+        return self.k_cache[li], self.v_cache[li], self.k_scale[li], self.v_scale[li]
 
     def _copy_slots(self, dst: torch.Tensor, src: torch.Tensor):
         """Per-slot state a sequence takes over from another one with the same prompt (a paged cache has none)."""
@@ -258,7 +290,7 @@ class RolloutEngine:
 
     def _page_writer(self, tok_slot, ctx: SeqCtx, slots: torch.Tensor):
         """What the model's prompt forward hands its keys and values (or states) to."""
-        return _PrefillKV(self, tok_slot, ctx.positions.to(torch.int32))
+        return _PrefillKV(self, tok_slot, ctx.positions.to(torch.int32), slots)
 
     # ---- weights ------------------------------------------------------------------------------
     def sync_weights(self, model: CausalLM | None = None):
@@ -311,10 +343,15 @@ class RolloutEngine:
             else:
                 h = K.rmsnorm_infer(x, l.input_layernorm, eps)
             K.decode_gemm(h, l.qkv_proj, y32=self._acc_qkv)
-            K.rope_kv_write_f32(self._acc_qkv, l.qkv_bias, l.q_norm if cfg.qk_norm else None,
-                                l.k_norm if cfg.qk_norm else None, eps, self.seq_lens, None, self.block_table,
-                                self.block_size, self.q_buf, self.k_cache[li], self.v_cache[li], cfg.num_attention_heads,
-                                cfg.num_key_value_heads, cfg.head_dim, cfg.rope_theta, v_transposed=self.attn_tc, pos_delta=self.rope_delta)
+            norms = (l.q_norm, l.k_norm) if cfg.qk_norm else (None, None)
+            if self.kv8:
+                K.kv8_rope_append(self._acc_qkv, l.qkv_bias, *norms, eps, self.seq_lens, None, self.block_table, self.q_buf,
+                                  *self.cache8(li), cfg.num_attention_heads, cfg.rope_theta, pos_delta=self.rope_delta)
+            else:
+                K.rope_kv_write_f32(self._acc_qkv, l.qkv_bias, *norms, eps, self.seq_lens, None, self.block_table,
+                                    self.block_size, self.q_buf, self.k_cache[li], self.v_cache[li], cfg.num_attention_heads,
+                                    cfg.num_key_value_heads, cfg.head_dim, cfg.rope_theta, v_transposed=self.attn_tc,
+                                    pos_delta=self.rope_delta)
             self._decode_attention(li, scale)
             K.decode_gemm(self.attn_buf.view(self.max_seqs, -1), l.o_proj, y32=self._acc_o)
             h = K.add_rmsnorm_f32_infer(x, self._acc_o, l.post_attention_layernorm, eps)
@@ -358,9 +395,13 @@ class RolloutEngine:
                 qn = K.rmsnorm_infer(qkv[:, :qs].reshape(-1, cfg.head_dim).contiguous(), l.q_norm, eps)
                 kn = K.rmsnorm_infer(qkv[:, qs:qs + ks].reshape(-1, cfg.head_dim).contiguous(), l.k_norm, eps)
                 qkv = torch.cat([qn.view(-1, qs), kn.view(-1, ks), qkv[:, qs + ks:]], dim=1)
-            K.rope_kv_write(qkv, self.seq_lens, None, self.block_table, self.block_size, self.q_buf, self.k_cache[li],
-                            self.v_cache[li], cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim,
-                            cfg.rope_theta, v_transposed=self.attn_tc, pos_delta=self.rope_delta)
+            if self.kv8:
+                K.kv8_rope_append(qkv, None, None, None, eps, self.seq_lens, None, self.block_table, self.q_buf, *self.cache8(li),
+                                  cfg.num_attention_heads, cfg.rope_theta, pos_delta=self.rope_delta)
+            else:
+                K.rope_kv_write(qkv, self.seq_lens, None, self.block_table, self.block_size, self.q_buf, self.k_cache[li],
+                                self.v_cache[li], cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim,
+                                cfg.rope_theta, v_transposed=self.attn_tc, pos_delta=self.rope_delta)
             self._decode_attention(li, scale)
             if fuse:
                 attn_out = torch.nn.functional.linear(self.attn_buf.view(self.max_seqs, -1), l.o_proj)
@@ -401,6 +442,13 @@ class RolloutEngine:
         if self.seen is not None and sp.repetition_penalty != 1.0:
             seen = self.seen if rows is None else self.seen[rows]
             z = apply_repetition_penalty(z.float(), seen, sp.repetition_penalty)
+        greedy = sp.greedy or sp.temperature == 0
+        if sp.needs_filter_pass and not greedy and not sp.eos_prob_floor:
+            # filters and draw in one kernel, with the random numbers of the sampler below
+            K.sample_filtered(z, temperature=max(sp.temperature, 1e-6), top_k=sp.top_k or 0,
+                              top_p=1.0 if sp.top_p is None else sp.top_p, min_p=sp.min_p or 0.0, seed=_KERNEL_SEED,
+                              step_ptr=self.step_counter, out_tok=tok, out_logp=logp)
+            return
         if sp.needs_filter_pass:
             z = filter_top_k_top_p(z.float() / max(sp.temperature, 1e-6), sp.top_k, sp.top_p).contiguous()
             inv_t = 1.0
@@ -409,7 +457,7 @@ class RolloutEngine:
         # the seed argument is a constant (it is baked into the captured graph); the call's seed enters through the
         # start value of the device-side step counter, so a new seed needs no new capture
         K.sample_tokens(z, inv_t, sp.min_p, sp.eos_token_id, sp.eos_prob_floor, _KERNEL_SEED, self.step_counter,
-                        sp.greedy or sp.temperature == 0, tok, logp)
+                        greedy, tok, logp)
 
     # ---- prefill -------------------------------------------------------------------------------------
     @torch.no_grad()

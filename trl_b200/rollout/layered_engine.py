@@ -376,6 +376,8 @@ class LayeredRolloutEngine(RolloutEngine):
     def _check_model(self, max_model_len, block_size):
         if self.tp != 1:
             raise NotImplementedError("tensor-parallel decode of layered decoders")
+        if self.kv8:
+            raise NotImplementedError("an 8-bit cache for layered decoders")
         self.dtype = self.model.dtype
         if self.dtype not in (torch.bfloat16, torch.float32):
             raise NotImplementedError(f"layered decoders are served in bfloat16 or float32, not {self.dtype}")

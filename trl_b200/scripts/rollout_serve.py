@@ -44,6 +44,7 @@ class ServeArguments:
     data_parallel_size: int = 1
     gpu_memory_utilization: float = 0.9
     enable_prefix_caching: Optional[bool] = None
+    kv_cache_dtype: str = field(default="auto", metadata={"help": "'auto' (the model's type) or 'fp8': 8-bit pages, on a GPU."})
     log_level: str = "info"
 
 
@@ -96,10 +97,13 @@ class EngineHolder:
         if cuda and tp_group is not None:
             from ..rollout.tp_engine import TPRolloutEngine
 
-            self.engine = TPRolloutEngine(self.model, tp_group, max_num_seqs=a.max_num_seqs, max_model_len=a.max_model_len or 2048)
+            self.engine = TPRolloutEngine(self.model, tp_group, max_num_seqs=a.max_num_seqs, max_model_len=a.max_model_len or 2048,
+                                          kv_cache_dtype=a.kv_cache_dtype)
         elif cuda:
-            self.engine = make_engine(self.model, a.max_num_seqs, a.max_model_len or 2048)
+            self.engine = make_engine(self.model, a.max_num_seqs, a.max_model_len or 2048, kv_cache_dtype=a.kv_cache_dtype)
         else:
+            if a.kv_cache_dtype != "auto":
+                raise ValueError(f"kv_cache_dtype={a.kv_cache_dtype!r} needs a GPU: without one nothing is cached")
             self.engine = EagerGenerator(self.model)
         self.world_size = a.tensor_parallel_size * a.data_parallel_size
         self.max_model_len = a.max_model_len or 2048

@@ -81,6 +81,7 @@ class _OnlineConfig(_BaseConfig):
     # synthetic-benchmark knob: floor on the end-of-sequence probability during sampling
     eos_prob_floor: float = 0.0
     rollout_block_size: int = 0  # 0 = chosen by the engine (64-token pages for the tensor-core decode attention)
+    rollout_kv_cache_dtype: str = "auto"  # "fp8": the rollout engine in this process keeps keys and values in 8-bit pages
     rollout_poll_every: int = 16
 
     def _derive_generation_batch(self):

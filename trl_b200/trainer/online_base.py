@@ -254,21 +254,26 @@ class OnlineTrainer(Trainer):
                     groups = [list(range(i, i + tp)) for i in range(0, D.world_size(), tp)]
                     self._tp_group = D.new_subgroups_by_enumeration(groups)
                     self._rollout = TPRolloutEngine(gen_model, self._tp_group, max_num_seqs=nseq, max_model_len=max_len,
-                                                    block_size=bs, poll_every=a.rollout_poll_every)
+                                                    block_size=bs, poll_every=a.rollout_poll_every,
+                                                    kv_cache_dtype=a.rollout_kv_cache_dtype)
                 else:
                     try:
                         self._rollout = make_engine(gen_model, max_num_seqs=nseq, max_model_len=max_len, block_size=bs,
-                                                      poll_every=a.rollout_poll_every)
+                                                      poll_every=a.rollout_poll_every, kv_cache_dtype=a.rollout_kv_cache_dtype)
                     except NotImplementedError as e:  # e.g. GeGLU models: correct but slow eager generation
                         import warnings
 
                         from ..rollout.engine import EagerGenerator
 
+                        if a.rollout_kv_cache_dtype != "auto":
+                            raise
                         warnings.warn(f"{e}; falling back to the eager generator")
                         self._rollout = EagerGenerator(gen_model)
             else:
                 from ..rollout.engine import EagerGenerator
 
+                if getattr(self.args, "rollout_kv_cache_dtype", "auto") != "auto":
+                    raise ValueError("rollout_kv_cache_dtype needs a GPU: the eager generator caches nothing")
                 self._rollout = EagerGenerator(gen_model)
         return self._rollout
 
