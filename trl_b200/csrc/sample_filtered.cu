@@ -13,9 +13,9 @@
 // the latency of the few exchanges between the blocks; so logits are compared undivided, and the border is found in as few
 // passes as the row allows:
 //   1. the maximum and the mass, each thread with a running maximum of its own;
-//   2. candidates for the kept tokens: with top-k what is not below the k-th largest of the threads' maxima (k logits are at
-//      least that large), with top-p alone what is not lighter than (1 - top_p) mass / V (lighter ones together are less than
-//      what top-p leaves out).  Where one block's list holds them, it finds the border there and draws: done.
+//   2. candidates for the kept tokens: with top-k of C blocks what is not below the k/C-th largest of the threads' maxima of any
+//      (k logits are at least that large), with top-p alone what is not lighter than (1 - top_p) mass / V (lighter ones together
+//      are less than what top-p leaves out).  Where one block's list holds them, it finds the border there and draws: done.
 //   3. otherwise a histogram of the distances to the maximum.  From counts alone the bins bound the mass above each of them from
 //      both sides, which brackets the border; the tokens of the bracket are listed, and the exact mass above it says which of
 //      them is the last.  A bracket with too many tokens for the list is cut again by histograms over the logits' bits.
@@ -36,9 +36,10 @@ namespace trlb {
 constexpr int SF_THREADS = 512, SF_WARPS = SF_THREADS / 32;  // two blocks an SM
 constexpr int SF_EACH = 4;         // bins of a thread: SF_BINS / SF_THREADS
 constexpr int SF_BINS = 2048;      // histogram bins; the last one holds all that lies further below
-constexpr int SF_LIST = 4096;      // tokens that the list holds
+constexpr int SF_LIST = 2048;      // tokens that the list holds
 constexpr int SF_CUT = 1024;       // and the cut around the border; more are sorted in the list itself
-constexpr int SF_HELD = 4096;      // 16-byte vectors of a row in a block's shared memory, at most: with it two blocks an SM
+constexpr int SF_FEW = 64;          // of so few tokens each is compared with all others
+constexpr int SF_HELD = 5120;      // 16-byte vectors of a row in a block's shared memory, at most: with it two blocks an SM
 constexpr float SF_FINE = 1024.f;  // parts of a bin in which the histogram adds up where in the bin its tokens lie
 constexpr int SF_BATCH = 16;       // logits that a thread loads at once
 constexpr float SF_MAX = 3.4028234663852886e38f;
@@ -159,11 +160,13 @@ struct SfShared {
     unsigned long long cut[SF_CUT];   // the part of the list around the border
   };
   unsigned long long list[SF_LIST];   // ~key << 32 | column: ascending is "larger logit, then lower column"
-  double red[3][SF_WARPS];
+  double red[2][SF_WARPS];
+  float warp_best[SF_WARPS], warp_z[SF_WARPS];
+  int warp_col[SF_WARPS];
   unsigned long long sum[SF_WARPS];
   double mass, first_mass, sums[2];   // this block's shares of sums
   double kept;                        // mass down to the border, 0: unknown
-  float fmax;
+  float fmax, from;
   unsigned kmin, kmax, list_n, cut_n;
   int bin_lo, bin_hi;                 // the bracket, its tokens and those above it: the same in every block
   unsigned above, upto;
@@ -236,8 +239,9 @@ __device__ __forceinline__ double sf_block_sum(double v, SfShared& s) {
   __syncthreads();
   if ((threadIdx.x & 31) == 0) s.red[0][threadIdx.x >> 5] = v;
   __syncthreads();
-  double all = 0.;
-  for (int w = 0; w < SF_WARPS; ++w) all += s.red[0][w];
+  double all = s.red[0][threadIdx.x & (SF_WARPS - 1)];  // one order in every warp
+#pragma unroll
+  for (int o = SF_WARPS / 2; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
   return all;
 }
 __device__ __forceinline__ unsigned long long sf_block_count(unsigned long long v, SfShared& s) {
@@ -246,8 +250,9 @@ __device__ __forceinline__ unsigned long long sf_block_count(unsigned long long 
   __syncthreads();
   if ((threadIdx.x & 31) == 0) s.sum[threadIdx.x >> 5] = v;
   __syncthreads();
-  unsigned long long all = 0;
-  for (int w = 0; w < SF_WARPS; ++w) all += s.sum[w];
+  unsigned long long all = s.sum[threadIdx.x & (SF_WARPS - 1)];
+#pragma unroll
+  for (int o = SF_WARPS / 2; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
   return all;
 }
 // Inclusive prefixes over the threads of a block.
@@ -271,6 +276,52 @@ __device__ __forceinline__ void sf_block_prefix(double (&v)[N], SfShared& s) {
     for (int n = 0; n < N; ++n) v[n] += s.red[n][w];
 }
 
+// One step of a bitonic sort between the lanes of a warp: `up` says whether the run that the lane is in ascends.
+template <int J>
+__device__ __forceinline__ void sf_sort_step(unsigned long long& x, bool up) {
+  const unsigned long long y = __shfl_xor_sync(0xffffffffu, x, J);
+  if ((x > y) == (((threadIdx.x & J) == 0) == up)) x = y;
+}
+// Sorts n <= SF_THREADS entries ascending, one in a register of each thread of as many warps as it takes; `at` has room for the
+// next power of two.
+__device__ __noinline__ void sf_sort_few(unsigned long long* at, int n) {
+  int size = 32;
+  while (size < n) size <<= 1;
+  const int i = threadIdx.x;
+  __syncthreads();
+  if (i < size) {
+    unsigned long long x = i < n ? at[i] : ~0ull;
+    sf_sort_step<1>(x, (i & 2) == 0);
+    sf_sort_step<2>(x, (i & 4) == 0);
+    sf_sort_step<1>(x, (i & 4) == 0);
+    sf_sort_step<4>(x, (i & 8) == 0);
+    sf_sort_step<2>(x, (i & 8) == 0);
+    sf_sort_step<1>(x, (i & 8) == 0);
+    sf_sort_step<8>(x, (i & 16) == 0);
+    sf_sort_step<4>(x, (i & 16) == 0);
+    sf_sort_step<2>(x, (i & 16) == 0);
+    sf_sort_step<1>(x, (i & 16) == 0);
+#pragma unroll 1
+    for (int k = 32; k <= size; k <<= 1) {
+      const bool up = (i & k) == 0;
+#pragma unroll 1
+      for (int j = k >> 1; j >= 32; j >>= 1) {
+        at[i] = x;
+        asm volatile("bar.sync 1, %0;" ::"r"(size) : "memory");
+        const unsigned long long y = at[i ^ j];
+        if ((x > y) == (((i & j) == 0) == up)) x = y;
+        asm volatile("bar.sync 1, %0;" ::"r"(size) : "memory");
+      }
+      sf_sort_step<16>(x, up);
+      sf_sort_step<8>(x, up);
+      sf_sort_step<4>(x, up);
+      sf_sort_step<2>(x, up);
+      sf_sort_step<1>(x, up);
+    }
+    at[i] = x;
+  }
+  __syncthreads();
+}
 // Sorts n entries ascending; `at` has room for the next power of two.  As many warps as it takes pairs for work on it: the
 // others wait once, at the end.
 __device__ __noinline__ void sf_sort(unsigned long long* at, int n) {
@@ -312,12 +363,20 @@ __device__ __forceinline__ void sf_block_best(float& best, int& col, float& z, S
   }
   __syncthreads();
   if ((threadIdx.x & 31) == 0) {
-    s.red[0][threadIdx.x >> 5] = best;
-    s.red[1][threadIdx.x >> 5] = col;
-    s.red[2][threadIdx.x >> 5] = z;
+    s.warp_best[threadIdx.x >> 5] = best;
+    s.warp_col[threadIdx.x >> 5] = col;
+    s.warp_z[threadIdx.x >> 5] = z;
   }
   __syncthreads();
-  for (int w = 0; w < SF_WARPS; ++w) sf_better(best, col, z, (float)s.red[0][w], (int)s.red[1][w], (float)s.red[2][w]);
+  best = s.warp_best[threadIdx.x & (SF_WARPS - 1)];
+  col = s.warp_col[threadIdx.x & (SF_WARPS - 1)];
+  z = s.warp_z[threadIdx.x & (SF_WARPS - 1)];
+#pragma unroll
+  for (int o = SF_WARPS / 2; o > 0; o >>= 1) {
+    const float ob = __shfl_xor_sync(0xffffffffu, best, o), oz = __shfl_xor_sync(0xffffffffu, z, o);
+    const int oc = __shfl_xor_sync(0xffffffffu, col, o);
+    sf_better(best, col, z, ob, oc, oz);
+  }
 }
 
 template <typename T>
@@ -454,24 +513,21 @@ struct SfSampler {
       if (lane >= o) { v[0] += x; v[1] += y; cnt += z; }
     }
     __syncthreads();
-    if (lane == 31) { s.red[0][wid] = v[0]; s.red[1][wid] = v[1]; s.red[2][wid] = cnt; }
+    if (lane == 31) { s.warp_best[wid] = v[0]; s.warp_z[wid] = v[1]; s.warp_col[wid] = (int)cnt; }
     __syncthreads();
-    float up = (float)mass, low = (float)mass;
-    unsigned before = 0;
-#pragma unroll
-    for (int w = 0; w < SF_WARPS; ++w)
-      if (w < wid) { up += (float)s.red[0][w]; low += (float)s.red[1][w]; before += (unsigned)s.red[2][w]; }
-    up += v[0] - own[0];  // bounds before this thread's bins
-    low += v[1] - own[1];
+    const float up = (float)mass + warp_sum(lane < wid ? s.warp_best[lane] : 0.f) + v[0] - own[0];  // bounds before this thread's bins
+    const float low = (float)mass + warp_sum(lane < wid ? s.warp_z[lane] : 0.f) + v[1] - own[1];
+    const unsigned before = __reduce_add_sync(0xffffffffu, lane < wid ? (unsigned)s.warp_col[lane] : 0u);
     cnt += before - own_n;
     const float limit = (float)goal;
+    float upper = up, lower = low;
     int first_up = SF_BINS - 1, first_low = SF_BINS - 1;
 #pragma unroll
     for (int i = 0; i < SF_EACH; ++i) {
-      up += hi[i];
-      low += lo[i];
-      if (up * 1.00001f > limit) first_up = min(first_up, SF_EACH * tid + i);
-      if (low * 0.99999f > limit) first_low = min(first_low, SF_EACH * tid + i);
+      upper += hi[i];
+      lower += lo[i];
+      if (upper * 1.00001f > limit) first_up = min(first_up, SF_EACH * tid + i);
+      if (lower * 0.99999f > limit) first_low = min(first_low, SF_EACH * tid + i);
     }
     first_up = __reduce_min_sync(0xffffffffu, first_up);
     first_low = __reduce_min_sync(0xffffffffu, first_low);
@@ -568,31 +624,82 @@ struct SfSampler {
 
   // ---- the first block alone: borders in its list of n tokens -----------------------------------------------------------
   __device__ __forceinline__ unsigned long long whole(double w) const { return (unsigned long long)(w * SF_UNIT + 0.5); }
-  // The border among n <= SF_THREADS sorted entries, a thread an entry; `above` tokens and `mass` above them.
-  __device__ __noinline__ void small_border(const unsigned long long* at, int n, bool by_mass, double goal, unsigned above, double mass) {
-    const unsigned long long mine = tid < n ? at[tid] : 0;
-    bool border = !by_mass && tid < n && above + tid + 1 == (unsigned)goal;
+  // Where one of n <= SF_THREADS entries stands among them: entries before it and their mass; is_k: its logit is at least that of
+  // the k-th.  Up to SF_FEW each is compared with all others, by each_of(n) threads, more are sorted: measured alike at 100.
+  struct Place {
+    unsigned long long entry, own, before;
+    unsigned rank;
+    bool valid, is_k;  // valid: this thread answers for the entry
+  };
+  __device__ __forceinline__ unsigned long long mass_of(unsigned long long e) const { return whole((double)expf(quotient(sf_entry_x(e)) - zmax)); }
+  __device__ __noinline__ Place place_of(unsigned long long* at, int n, int k) {
+    Place p;
+    if (n <= SF_FEW) {
+      int each = SF_THREADS / SF_FEW;
+      while (each < 32 && 2 * each * n <= SF_THREADS) each *= 2;
+      ulonglong2* pairs = reinterpret_cast<ulonglong2*>(s.hist);
+      __syncthreads();
+      if (tid < n) pairs[tid] = make_ulonglong2(at[tid], mass_of(at[tid]));
+      __syncthreads();
+      const ulonglong2 mine = pairs[min(tid / each, n - 1)];
+      p.entry = mine.x;
+      p.own = mine.y;
+      p.before = 0;
+      p.rank = 0;
+      unsigned larger = 0;
+      for (int j = tid & (each - 1); j < n; j += each) {
+        const ulonglong2 o = pairs[j];
+        if (o.x < mine.x) {
+          p.before += o.y;
+          ++p.rank;
+        }
+        larger += (unsigned)(o.x >> 32) < (unsigned)(mine.x >> 32);
+      }
+      for (int o = each / 2; o > 0; o >>= 1) {
+        p.before += __shfl_xor_sync(0xffffffffu, p.before, o);
+        p.rank += __shfl_xor_sync(0xffffffffu, p.rank, o);
+        larger += __shfl_xor_sync(0xffffffffu, larger, o);
+      }
+      p.valid = tid < n * each && (tid & (each - 1)) == 0;
+      p.is_k = (int)larger < k;
+      return p;
+    }
+    sf_sort_few(at, n);
+    const int lane = tid & 31, wid = tid >> 5;
+    p.valid = tid < n;
+    p.entry = at[min(tid, n - 1)];
+    p.own = p.valid ? mass_of(p.entry) : 0;
+    p.rank = (unsigned)tid;
+    p.is_k = k > 0 && (unsigned)(p.entry >> 32) <= (unsigned)(at[min(k, n) - 1] >> 32);
+    unsigned long long upto = p.own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    if (lane == 31) s.sum[wid] = upto;
+    __syncthreads();
+    unsigned long long others = lane < wid ? s.sum[lane & (SF_WARPS - 1)] : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) others += __shfl_xor_sync(0xffffffffu, others, o);
+    p.before = upto - p.own + others;
+    return p;
+  }
+  // The border among n <= SF_THREADS entries; `above` tokens and `mass` above them.
+  __device__ __noinline__ void few_border(unsigned long long* at, int n, bool by_mass, double goal, unsigned above, double mass) {
+    const Place p = place_of(at, n, 0);
+    bool border = p.valid;
     double kept = 0.;
     if (by_mass) {
-      const int lane = tid & 31, wid = tid >> 5;
-      const unsigned long long own = tid < n ? whole((double)weight(sf_entry_x(mine))) : 0;
-      unsigned long long upto = own;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long x = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += x;
-      }
-      if (lane == 31) s.sum[wid] = upto;
-      __syncthreads();
-      for (int w = 0; w < wid; ++w) upto += s.sum[w];
       // the last entry before which at most `goal` stands: its successor is behind more
-      const double behind = mass + (double)upto / SF_UNIT;
-      border = tid < n && (tid == 0 || mass + (double)(upto - own) / SF_UNIT <= goal) && (tid == n - 1 || behind > goal);
-      kept = behind;
+      kept = mass + (double)(p.before + p.own) / SF_UNIT;
+      border = border && (p.rank == 0 || mass + (double)p.before / SF_UNIT <= goal) && (p.rank == n - 1 || kept > goal);
+    } else {
+      border = border && above + p.rank + 1 == (unsigned)goal;
     }
     if (border) {
-      s.border = sf_entry_x(mine);
-      s.border_col = by_mass ? (int)(unsigned)mine : 0x7fffffff;
+      s.border = sf_entry_x(p.entry);
+      s.border_col = by_mass ? (int)(unsigned)p.entry : 0x7fffffff;
       s.kept = kept;
     }
     __syncthreads();
@@ -637,8 +744,7 @@ struct SfSampler {
   // stands (by_mass), or the goal-th token and its equals.  Leaves s.border, s.border_col and s.kept (0: unknown).
   __device__ __noinline__ void list_border(int n, bool by_mass, double goal, unsigned above, double mass) {
     if (n <= SF_THREADS) {
-      sf_sort(s.list, n);
-      small_border(s.list, n, by_mass, goal, above, mass);
+      few_border(s.list, n, by_mass, goal, above, mass);
       return;
     }
     unsigned lo = 0xffffffffu, hi = 0u;
@@ -685,9 +791,12 @@ struct SfSampler {
     __syncthreads();
     const int m = (int)s.cut_n;
     above += a0;
-    sf_sort(s.cut, m);
-    if (m <= SF_THREADS) small_border(s.cut, m, by_mass, goal, above, mass);
-    else sorted_border(s.cut, m, by_mass, goal, above, mass);
+    if (m <= SF_THREADS) {
+      few_border(s.cut, m, by_mass, goal, above, mass);
+    } else {
+      sf_sort(s.cut, m);
+      sorted_border(s.cut, m, by_mass, goal, above, mass);
+    }
   }
   static __device__ __forceinline__ bool within(float x, int col, float border, int border_col) {
     return x > border || (x == border && col <= border_col);
@@ -924,7 +1033,7 @@ struct SfSampler {
     }
     if (tid < C) sf_better(best, col, best_z, s.bests[tid], s.best_cols[tid], s.best_zs[tid]);
     sf_block_best(best, col, best_z, s);
-    if (!greedy && (double)best < (double)zmax + log(mass) - 3.) {  // once in 10^8 rows: without the shortcut of the draws
+    if (!greedy && (double)best < (double)zmax + (double)logf((float)mass) - 2.999) {  // once in 10^8 rows: without the shortcut of the draws
       SfRow<T> q = r;
       q.v0 = 0;
       q.v1 = a.V;
@@ -958,7 +1067,7 @@ struct SfSampler {
     const float top_p = a.top_p ? a.top_p[row] : a.top_p_all, min_p = a.min_p ? a.min_p[row] : a.min_p_all;
     const int top_k = a.top_k ? a.top_k[row] : a.top_k_all;
     const bool by_k = top_k > 0 && top_k < a.V, by_p = top_p < 1.f;
-    if (by_k && (top_k > SF_THREADS / 2 || top_k * C > SF_LIST / 2)) return false;  // too many for the lists
+    if (by_k && top_k > min(SF_LIST / 4, C * SF_THREADS / 2)) return false;  // too many for the lists
     const int first = r.v0;
     float mine = -INFINITY;
     {
@@ -1008,23 +1117,27 @@ struct SfSampler {
     bmax = warp_max(bmax);
     bmin = -warp_max(-bmin);
     if (by_k) {
-      // What this block can have among the k largest is not below the k-th largest of its threads' maxima.
-      float from = -SF_MAX;  // all, where fewer than k threads have any
+      // A k-th part of the blocks' number: as many threads of each block have a maximum of at least `from`, so that k logits of
+      // the row are at least the smallest of the blocks' numbers.
+      const unsigned share = (unsigned)((top_k + C - 1) / C);
+      float from = -SF_MAX;  // all, where fewer threads have any
       const float scale = (float)(SF_BINS - 2) / (bmax - bmin);
       if (scale < 1e30f) {  // false also where the block has none or all maxima are equal
         if (mine > -INFINITY) atomicAdd(&sh.hist[(int)fminf((bmax - mine) * scale, (float)(SF_BINS - 1))], 1u);
         unsigned h[SF_EACH];
         own_bins(h);
-        bracket_count(h, (unsigned)top_k);
+        bracket_count(h, share);
         if (sh.bin_lo < SF_BINS - 1) from = fmaxf(from, bmax - (float)(sh.bin_lo + 1) / scale * 1.000001f);  // a little below the bin's end
       }
+      if (tid == 0) { sh.fmax = bmax; sh.from = from; }
+      cluster.sync();
+      xmax = max_of([](const SfShared& o) { return o.fmax; });
+      from = -max_of([](const SfShared& o) { return -o.from; });
       each([&](float x, int col) {
         if (x >= from) append(sh, x, col);
       });
-      if (tid == 0) sh.fmax = bmax;
       const int n = collect();
       if (n == 0) return false;  // none at all, or too many
-      xmax = max_of([](const SfShared& o) { return o.fmax; });
       zmax = quotient(xmax);
       if (n < top_k) return false;
       release(false);
@@ -1047,53 +1160,72 @@ struct SfSampler {
     }
     const Pass q = pass();
     const float floor = min_p > 0.f ? least_logit(min_p) : -INFINITY;
-    if (!by_p) {
-      double mass = total;
-      if (floor > -INFINITY) {
-        float part = 0.f;
-        each([&](float x, int) { part += x >= floor ? q.weight(x) : 0.f; });
-        const double sum = sf_block_sum((double)part, sh);
-        if (tid == 0) sh.sums[1] = sum;
-        cluster.sync();
-        mass = sum_of([](const SfShared& o) { return o.sums[1]; });
-      }
-      draw(each, q, mass, floor);
-      cluster.sync();
-      release(true);
-      if (rank == 0) finish_blocks(0, fmaxf(floor, -SF_MAX), 0x7fffffff, mass);
-      return true;
-    }
+    const double goal = by_p ? fmax(0., (double)top_p * total) : 0.;
+    float from = -SF_MAX;
     // ---- top-p ----
-    // lighter tokens than this together have less than what top-p leaves out; a little is added for the sums' rounding
-    const double goal = fmax(0., (double)top_p * total), least = (1. - (double)top_p - 2e-5) * total / a.V;
-    if (!(least > 0.)) return false;
-    const float from = fmaxf(-SF_MAX, xmax + (logf((float)least) - 1e-3f) * temperature);
-    // weights are at most 1: at least `goal` tokens are kept, and with many of them come more than the list holds
-    if (goal < SF_LIST / 16) {
-      each([&](float x, int col) {
-        if (x >= from) append(sh, x, col);
-      });
+    if (by_p) {
+      // lighter tokens than this together have less than what top-p leaves out; a little is added for the sums' rounding
+      const double least = (1. - (double)top_p - 2e-5) * total / a.V;
+      if (!(least > 0.)) return false;
+      from = fmaxf(-SF_MAX, xmax + (logf((float)least) - 1e-3f) * temperature);
+    }
+    if (by_p && goal < SF_LIST / 16) {
+      // twice a block's part of the list says that there are too many, without a look at the rest
+      const unsigned most = (unsigned)min(SF_LIST, 2 * SF_LIST / C);
+#pragma unroll 1
+      for (int v = tid; v < vecs && *reinterpret_cast<volatile unsigned*>(&sh.list_n) <= most; v += SF_THREADS) {
+        float y[N];
+        sf_unpack<T>(data[v], y);
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+          if (y[k] >= from) append(sh, y[k], first + v * N + k);
+      }
+      __syncthreads();
+      if (tid == 0 && sh.list_n > most) sh.list_n = SF_LIST + 1;
       const int n = collect();
       if (n > 0) {
         release(false);
         if (rank == 0) {
-          list_border(n, true, goal, 0, 0.);
-          finish_list(n, sh.border, sh.border_col, floor);
+          const int m = n > SF_FEW ? thin_out(n, goal, total) : n;
+          if (m <= SF_THREADS) {
+            finish_few(m, 0, 0., goal, floor);
+          } else {
+            list_border(m, true, goal, 0, 0.);
+            finish_list(m, sh.border, sh.border_col, floor);
+          }
         }
         return true;
       }
       cluster.sync();  // the numbers of the lists have been read
       if (tid == 0) sh.list_n = 0;
     }
-    if (floor > -INFINITY) return false;
+    // ---- min-p: either all that it keeps is within top-p, or top-p keeps less and min-p changes nothing ----
+    bool all = !by_p;
+    double floor_mass = total;
+    if (floor > -INFINITY) {
+      float part = 0.f;
+      each([&](float x, int) { part += x >= floor ? q.weight(x) : 0.f; });
+      const double sum = sf_block_sum((double)part, sh);
+      if (tid == 0) sh.sums[1] = sum;
+      cluster.sync();
+      floor_mass = sum_of([](const SfShared& o) { return o.sums[1]; });
+      all = all || floor_mass <= goal;
+    }
+    if (all) {
+      draw(each, q, floor_mass, floor);
+      cluster.sync();
+      release(true);
+      if (rank == 0) finish_blocks(0, fmaxf(floor, -SF_MAX), 0x7fffffff, floor_mass);
+      return true;
+    }
     set_step(from);
     const Pass h = pass();
     each([&](float x, int) {
       if (x >= from) {
-        const float y = (h.xmax - x) * h.step;
-        const int bin = (int)fminf(y, (float)(SF_BINS - 1));
-        atomicAdd(&sh.hist[bin], 1u);
-        atomicAdd(&sh.where[bin], (unsigned)fminf((y - (float)bin) * SF_FINE, SF_FINE));
+        // bin and place in it: the whole number and the fraction of linear_bin's quotient; the last bin has all that is further
+        const unsigned y = (unsigned)fminf((h.xmax - x) * h.step * SF_FINE, SF_BINS * SF_FINE - 1.f);
+        atomicAdd(&sh.hist[y / (unsigned)SF_FINE], 1u);
+        atomicAdd(&sh.where[y / (unsigned)SF_FINE], y % (unsigned)SF_FINE);
       }
     });
     cluster.sync();
@@ -1111,19 +1243,20 @@ struct SfSampler {
     if (lead->upto - above > SF_LIST) return false;
     // above the bracket: the mass, and the draw (at least `goal` is kept); the bracket: listed
     {
-      const float reach = (float)(4294967296. * 20.0855369 * 1.001 / goal), t = temperature;
+      const float reach = (float)(20.0855369 * 1.001 / goal), t = temperature;
       const uint32_t w = word;
       const bool most = greedy, as = as_sampler;
       float part = 0.f, top = -INFINITY, top_z = 0.f;
       int at = -1;
+      // linear_bin() < b0 and <= b1 without its conversion
+      const float end0 = (float)b0, end1 = b1 == SF_BINS - 1 ? INFINITY : (float)(b1 + 1);
       each([&](float x, int col) {
-        if (x < from) return;
-        const int b = h.linear_bin(x);
-        if (b < b0) {
+        const float y = (h.xmax - x) * h.step;
+        if (y < end0 && x >= from) {
           const float wt = h.weight(x);
           part += wt;
           consider(x, col, wt, reach, t, w, most, as, top, at, top_z);
-        } else if (b <= b1) {
+        } else if (y < end1 && x >= from) {
           append(sh, x, col);
         }
       });
@@ -1158,8 +1291,9 @@ struct SfSampler {
     float z = x, k = x;
     if (!most) {
       const uint32_t h = sf_bits(word, (uint32_t)col);
-      // 2^13: what 24 bits and fast logarithms may make of 1 - u, 2^-20 at most
-      if ((float)(~h) > reach * weight + (as_sampler ? 8192.f : 0.f)) return;
+      // 1 - u in [0, 1), its bits set behind a one; the margin is for the bits cut off and, as_sampler, for what 24 bits and fast
+      // logarithms may make of it
+      if (__uint_as_float(0x3f800000u | ~h >> 9) > fmaf(reach, weight, as_sampler ? 1.f + 2e-6f : 1.f + 3e-7f)) return;
       z = sf_quotient(x, t);
       k = z + (as_sampler ? sf_gumbel_as_sampler(h) : sf_gumbel(h));
     }
@@ -1168,7 +1302,7 @@ struct SfSampler {
   // This block's draw among its tokens of at least `floor`.
   template <typename E>
   __device__ __forceinline__ void draw(E each, const Pass& q, double mass, float floor) {
-    const float reach = (float)(4294967296. * 20.0855369 * 1.001 / mass), t = temperature, from = fmaxf(floor, -SF_MAX);
+    const float reach = (float)(20.0855369 * 1.001 / mass), t = temperature, from = fmaxf(floor, -SF_MAX);
     const uint32_t w = word;
     const bool most = greedy, as = as_sampler;
     float top = -INFINITY, top_z = 0.f;
@@ -1189,8 +1323,56 @@ struct SfSampler {
     for (int i = 0; i < 8 && (double)quotient(floor) < least && floor < xmax; ++i) floor = nextafterf(floor, INFINITY);
     return fminf(floor, xmax);
   }
+  // The first block: top-k (0: none), then top-p of `goal`, or of the share top_p of what top-k kept, then the floor and the draw, in
+  // a list of n <= SF_THREADS tokens that holds all that is kept.
+  __device__ __noinline__ void finish_few(int n, int top_k, double top_p, double goal, float floor) {
+    const Place p = place_of(s.list, n, top_k);
+    const float x = sf_entry_x(p.entry);
+    bool kept = p.valid;
+    if (top_k > 0) {
+      kept = kept && p.is_k;
+      goal = top_p < 1. ? fmax(0., top_p * ((double)sf_block_count(kept ? p.own : 0, s) / SF_UNIT)) : INFINITY;
+    }
+    kept = kept && (p.rank == 0 || (double)p.before / SF_UNIT <= goal) && x >= floor;
+    float best = -INFINITY, best_z = 0.f;
+    int col = -1;
+    if (kept) {
+      const float z = quotient(x);
+      sf_better(best, col, best_z, greedy ? z : z + noise(sf_bits(word, (unsigned)p.entry)), (int)(unsigned)p.entry, z);
+    }
+    const unsigned long long sum = sf_block_count(kept ? p.own : 0, s);
+    sf_block_best(best, col, best_z, s);
+    write(best_z, col, (double)sum / SF_UNIT);
+  }
+  // The first block, for top-p: its list of n tokens without those that are lighter than room / n, the mass that may be left out
+  // parted among them.  `total`: the row's mass; returns how many are left.
+  __device__ __noinline__ int thin_out(int n, double goal, double total) {
+    constexpr int E = SF_LIST / SF_THREADS;
+    unsigned long long e[E], sum = 0;
+    float w[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const bool in = tid + i * SF_THREADS < n;
+      e[i] = in ? s.list[tid + i * SF_THREADS] : ~0ull;
+      w[i] = in ? weight(sf_entry_x(e[i])) : 0.f;
+      sum += whole((double)w[i]);
+    }
+    if (tid == 0) s.list_n = 0;
+    // what is not in the list is left out; a little more for the sums' rounding
+    const double in_list = (double)sf_block_count(sum, s) / SF_UNIT, room = fmin(in_list, total) - goal - 2e-5 * total;
+    const float least = (float)(fmax(room, 0.) / n * 0.999);
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if (tid + i * SF_THREADS < n && w[i] >= least) s.list[atomicAdd(&s.list_n, 1u)] = e[i];
+    __syncthreads();
+    return (int)s.list_n;
+  }
   // The first block: top-k, then top-p, then the draw, in a list that holds the k largest.
   __device__ __noinline__ void top_k_of_list(int n, int top_k, bool by_p, float top_p, float floor) {
+    if (n <= SF_THREADS) {
+      finish_few(n, top_k, by_p ? (double)top_p : 1., 0., floor);
+      return;
+    }
     list_border(n, false, (double)top_k, 0, 0.);
     const float border = s.border;
     if (by_p) {
@@ -1322,7 +1504,7 @@ struct SfSampler {
     int col = -1;
     for (int turn = 0; turn < 2 && (col < 0 || (!greedy && (double)best < reached)); ++turn) {
       const Pass q = pass();
-      const float reach = turn == 1 ? INFINITY : (float)(4294967296. * 20.0855369 * 1.001 / mass), last = fmaxf(border, -SF_MAX), t = temperature;
+      const float reach = turn == 1 ? INFINITY : (float)(20.0855369 * 1.001 / mass), last = fmaxf(border, -SF_MAX), t = temperature;
       const int last_col = border == -INFINITY ? 0x7fffffff : border_col;
       const uint32_t w = word;
       const bool most = greedy, as = as_sampler;
@@ -1387,7 +1569,7 @@ int sample_filtered_launch(const SampleArgs& a, int B, cudaStream_t st) {
   // while there are fewer than two an SM.
   constexpr long long N = 16 / sizeof(T);
   int C = 1;
-  while (C < 8 && (C * N * SF_HELD < a.V || (long long)C * B <= trlb_host::sm_count())) C *= 2;
+  while (C < 8 && (C * N * SF_HELD < a.V || (long long)C * B <= trlb_host::sm_count())) ++C;
   const long long need = ((a.V + C - 1) / C + N - 1) / N;
   const int vecs = need <= SF_HELD ? (int)need : 0;
   cudaError_t e = cudaFuncSetAttribute(sample_filtered_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
