@@ -360,3 +360,67 @@ def test_fused_rope_append_equals_its_parts():
                     held = codes[blk, :, row].cpu().double() * scale[blk].cpu().double()[:, None]
                     t = 2.0**-4 * want.abs() * (1 + 2.0**-7) + 2.0**-8 * want.abs() + 2.0**-18 * size + 2.0**-10 * scale[blk].cpu().double()[:, None]
                     assert ((held - want).abs() <= t).all()
+
+
+@pytest.mark.parametrize("vocab, dtype", [(200003, torch.float32), (400000, torch.bfloat16)])
+@pytest.mark.parametrize("kw", [{}, {"top_k": 70}, {"top_p": 0.9}, {"top_k": 900, "top_p": 0.5, "min_p": 0.001}, {"min_p": 0.1}])
+def test_sampling_of_rows_beyond_shared_memory(vocab, dtype, kw):
+    logits, rng = _logits(2, vocab, dtype, seed=7)
+    check_sample(logits, rng, *F.sample_filtered(logits, rng, **kw), **kw)
+
+
+@pytest.mark.parametrize("count", [1, 31, 63, 64, 65, 128, 129, 511, 512, 513, 1024, 1025, 2047, 2048, 2049, 5000])
+def test_sampling_of_lists_of_all_lengths(count):
+    """``count`` tokens, evenly spaced from likely to unlikely, among others that are out of reach."""
+    g = torch.Generator().manual_seed(count)
+    rows, vocab = 5, 20011
+    z = torch.full((rows, vocab), -60.0)
+    for i in range(rows):
+        at = torch.randperm(vocab, generator=g)[:count]
+        z[i, at] = -torch.arange(count) * (0.5, 0.05, 0.003, 12.0 / count, 0.0)[i]
+    rng = torch.randint(-2**31, 2**31 - 1, (rows,), generator=g).to(torch.int32).cuda()
+    for kw in ({"top_p": 0.9}, {"top_p": 0.999}, {"top_k": max(1, count // 2)}, {"top_k": min(count + 1, 512), "top_p": 0.7},
+               {"top_p": 0.97, "min_p": 0.02}, {"top_p": 0.4, "min_p": 1e-4}):
+        check_sample(z, rng, *F.sample_filtered(z.cuda(), rng, **kw), **kw)
+
+
+def test_sampling_on_two_streams_and_replayed():
+    logits, rng = _logits(9, 33000, torch.bfloat16)
+    other, rng2 = _logits(9, 33000, torch.bfloat16, seed=1)
+    kw = {"top_p": 0.9, "top_k": 400}
+    want, want2 = F.sample_filtered(logits, rng, **kw), F.sample_filtered(other, rng2, **kw)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        a = F.sample_filtered(logits, rng, **kw)
+        with torch.cuda.stream(side):
+            b = F.sample_filtered(other, rng2, **kw)
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip((*a, *b), (*want, *want2)))
+    z, words = logits.clone(), rng.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c = F.sample_filtered(z, words, **kw)
+    for x, r, w in ((logits, rng, want), (other, rng2, want2), (logits, rng, want)):
+        z.copy_(x)
+        words.copy_(r)
+        graph.replay()
+        assert all(torch.equal(p, q) for p, q in zip(c, w))
+
+
+@pytest.mark.parametrize("D, Hq, Hk", [(64, 8, 2), (128, 4, 4), (256, 8, 1)])
+def test_attention_repeats_itself(D, Hq, Hk):
+    """The same call gives the same bits, whatever runs beside it."""
+    lens = [1, 700, 4097, 63, 0, 129]
+    cache, table = filled_cache(lens, Hk, 32, D, "cuda", seed=D)
+    q = torch.randn(len(lens), Hq, D, device="cuda").to(torch.bfloat16)
+    at = _i32([n - 1 for n in lens])
+    first = F.kv8_decode_attn(q, *cache, table, at, D**-0.5)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(10):
+        with torch.cuda.stream(side):
+            beside = F.kv8_decode_attn(q, *cache, table, at, D**-0.5)
+        assert torch.equal(first, F.kv8_decode_attn(q, *cache, table, at, D**-0.5))
+    torch.cuda.synchronize()
+    assert torch.equal(first, beside)
