@@ -189,8 +189,8 @@ struct SfRow {
   bool vec;
   float cap;  // logits from here on are equals: their quotients by the temperature are not finite
   __device__ __forceinline__ float clean(float y) const { return sf_clean1(y, cap); }
-  // f(logit, column) over the block's columns, until stop() says so
-  template <typename F, typename G>
+  // f(logit, column) over the block's columns, until stop() says so; RAW: logits as they are
+  template <bool RAW = false, typename F, typename G>
   __device__ __forceinline__ void each(F f, G stop) const {
     constexpr int N = 16 / sizeof(T);
     int i = v0 + threadIdx.x;
@@ -210,7 +210,7 @@ struct SfRow {
           float y[N];
           sf_unpack<T>(u[j], y);
 #pragma unroll
-          for (int k = 0; k < N; ++k) f(clean(y[k]), (at + j * SF_THREADS) * N + k);
+          for (int k = 0; k < N; ++k) f(RAW ? y[k] : clean(y[k]), (at + j * SF_THREADS) * N + k);
         }
       }
       i = n1 * N + threadIdx.x;
@@ -218,7 +218,7 @@ struct SfRow {
 #pragma unroll 1
     for (; i < v1; i += SF_THREADS) {
       if (stop()) return;
-      f(clean(sf_load(x, i)), i);
+      f(RAW ? sf_load(x, i) : clean(sf_load(x, i)), i);
     }
   }
   template <typename F>
@@ -398,7 +398,8 @@ struct SfSampler {
   struct Pass {
     SfRow<T> r;
     float xmax, c, step;
-    __device__ __forceinline__ float weight(float x) const { return exp2f((x - xmax) * c); }
+    // 2^y by one instruction: off by 2^-22 at most; what is below 2^-126 counts as nothing
+    __device__ __forceinline__ float weight(float x) const { return fast_exp2((x - xmax) * c); }
     __device__ __forceinline__ int linear_bin(float x) const { return (int)fminf((xmax - x) * step, (float)(SF_BINS - 1)); }
   };
   __device__ __forceinline__ Pass pass() const { return {r, xmax, c, step}; }
@@ -1060,8 +1061,9 @@ struct SfSampler {
     cluster.sync();
   }
 
-  // The block's columns in shared memory, `vecs` vectors, of which a thread reads what it has written.  False where the row needs
-  // run().
+  // The block's columns, HELD: in shared memory, `vecs` vectors, of which a thread reads what it has written; else read again for
+  // each pass.  False where the row needs run().
+  template <bool HELD>
   __device__ __forceinline__ bool fast(uint4* data, int vecs) {
     constexpr int N = 16 / sizeof(T);
     const float top_p = a.top_p ? a.top_p[row] : a.top_p_all, min_p = a.min_p ? a.min_p[row] : a.min_p_all;
@@ -1070,7 +1072,13 @@ struct SfSampler {
     if (by_k && top_k > min(SF_LIST / 4, C * SF_THREADS / 2)) return false;  // too many for the lists
     const int first = r.v0;
     float mine = -INFINITY;
-    {
+    if constexpr (!HELD) {
+      // what is NaN or has no finite quotient spoils the maximum, and the row: run() cleans each logit
+      const SfRow<T> q = r;
+      bool fine = true;
+      q.template each<true>([&](float x, int) { mine = fmaxf(mine, x); fine = fine && x <= q.cap; }, [] { return false; });
+      if (!fine) mine = INFINITY;
+    } else {
       const SfRow<T> q = r;
 #pragma unroll 4
       for (int v = tid; v < vecs; v += SF_THREADS) {
@@ -1096,15 +1104,22 @@ struct SfSampler {
         data[v] = u;
       }
     }
-    auto each = [&](auto f) {
+    auto each_until = [&](auto f, auto stop) {
+      if constexpr (HELD) {
 #pragma unroll 1
-      for (int v = tid; v < vecs; v += SF_THREADS) {
-        float y[N];
-        sf_unpack<T>(data[v], y);
+        for (int v = tid; v < vecs; v += SF_THREADS) {
+          if (stop()) return;
+          float y[N];
+          sf_unpack<T>(data[v], y);
 #pragma unroll
-        for (int k = 0; k < N; ++k) f(y[k], first + v * N + k);
+          for (int k = 0; k < N; ++k) f(y[k], first + v * N + k);
+        }
+      } else {
+        const SfRow<T> q = r;
+        q.template each<true>(f, stop);
       }
     };
+    auto each = [&](auto f) { each_until(f, [] { return false; }); };
     SfShared& sh = s;
     // ---- the maximum of the block, the smallest of its threads' ----
     const int lane = tid & 31, wid = tid >> 5;
@@ -1132,6 +1147,7 @@ struct SfSampler {
       if (tid == 0) { sh.fmax = bmax; sh.from = from; }
       cluster.sync();
       xmax = max_of([](const SfShared& o) { return o.fmax; });
+      if (!HELD && xmax == INFINITY) return false;
       from = -max_of([](const SfShared& o) { return -o.from; });
       each([&](float x, int col) {
         if (x >= from) append(sh, x, col);
@@ -1149,12 +1165,12 @@ struct SfSampler {
     {
       const float k = c;
       float part = 0.f;
-      if (bmax > -INFINITY) each([&](float x, int) { part += exp2f((x - bmax) * k); });
+      if (bmax > -INFINITY) each([&](float x, int) { part += fast_exp2((x - bmax) * k); });
       const double sum = sf_block_sum((double)part, sh);
       if (tid == 0) { sh.fmax = bmax; sh.sums[0] = sum; }
       cluster.sync();
       xmax = max_of([](const SfShared& o) { return o.fmax; });
-      if (xmax == -INFINITY) return false;
+      if (xmax == -INFINITY || (!HELD && xmax == INFINITY)) return false;
       zmax = quotient(xmax);
       total = sum_of([&](const SfShared& o) { return o.fmax > -INFINITY ? o.sums[0] * (double)exp2f((o.fmax - xmax) * c) : 0.; });
     }
@@ -1172,14 +1188,11 @@ struct SfSampler {
     if (by_p && goal < SF_LIST / 16) {
       // twice a block's part of the list says that there are too many, without a look at the rest
       const unsigned most = (unsigned)min(SF_LIST, 2 * SF_LIST / C);
-#pragma unroll 1
-      for (int v = tid; v < vecs && *reinterpret_cast<volatile unsigned*>(&sh.list_n) <= most; v += SF_THREADS) {
-        float y[N];
-        sf_unpack<T>(data[v], y);
-#pragma unroll
-        for (int k = 0; k < N; ++k)
-          if (y[k] >= from) append(sh, y[k], first + v * N + k);
-      }
+      each_until(
+          [&](float x, int col) {
+            if (x >= from) append(sh, x, col);
+          },
+          [&] { return *reinterpret_cast<volatile unsigned*>(&sh.list_n) > most; });
       __syncthreads();
       if (tid == 0 && sh.list_n > most) sh.list_n = SF_LIST + 1;
       const int n = collect();
@@ -1281,7 +1294,7 @@ struct SfSampler {
   }
   static __device__ __forceinline__ void append(SfShared& sh, float x, int col) {
     const unsigned i = atomicAdd(&sh.list_n, 1u);
-    if (i < SF_LIST) sh.list[i] = (unsigned long long)(~sf_key(x)) << 32 | (unsigned)col;
+    if (i < SF_LIST) sh.list[i] = (unsigned long long)(~sf_key(x + 0.f)) << 32 | (unsigned)col;
   }
   // One token's chance in a draw.  The largest z - log(-log u) of the kept tokens is lse + a Gumbel variate, which is below
   // lse - 3 once in 10^8 rows.  A token reaches K = lse - 3 only if -log u <= exp(z - K), and -log u >= 1 - u: most are out
@@ -1528,8 +1541,8 @@ struct SfSampler {
 };
 
 constexpr size_t SF_HEAD = (sizeof(SfShared) + 15) / 16 * 16;
-// vecs: vectors of a row in each block's shared memory, 0: the row is too large for that.
-template <typename T>
+// vecs, HELD: vectors of a row in each block's shared memory.
+template <typename T, bool HELD>
 __global__ void __launch_bounds__(SF_THREADS, 2)
 sample_filtered_kernel(const __grid_constant__ SampleArgs a, int vecs) {
   extern __shared__ __align__(16) unsigned char raw[];
@@ -1556,24 +1569,16 @@ sample_filtered_kernel(const __grid_constant__ SampleArgs a, int vecs) {
   f.row = row;
   f.tid = threadIdx.x;
   f.lead = cluster.map_shared_rank(&f.s, 0);
-  bool done = false;
-  if (vecs > 0) done = f.fast(reinterpret_cast<uint4*>(raw + SF_HEAD), vecs);
+  const bool done = f.template fast<HELD>(reinterpret_cast<uint4*>(raw + SF_HEAD), vecs);
   if (done) return;  // the others may have left already
   f.run();           // all blocks of a cluster take the same way
   cluster.sync();    // no block leaves while another may read its shared memory
 }
 
-template <typename T>
-int sample_filtered_launch(const SampleArgs& a, int B, cudaStream_t st) {
-  // Blocks a row: enough for the row to fit into their shared memory, two blocks an SM, up to the 8 of a portable cluster; more
-  // while there are fewer than two an SM.
-  constexpr long long N = 16 / sizeof(T);
-  int C = 1;
-  while (C < 8 && (C * N * SF_HELD < a.V || (long long)C * B <= trlb_host::sm_count())) ++C;
-  const long long need = ((a.V + C - 1) / C + N - 1) / N;
-  const int vecs = need <= SF_HELD ? (int)need : 0;
-  cudaError_t e = cudaFuncSetAttribute(sample_filtered_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)(SF_HEAD + SF_HELD * 16));
+template <typename T, bool HELD>
+int sample_filtered_launch(const SampleArgs& a, int B, int C, int vecs, cudaStream_t st) {
+  cudaError_t e = cudaFuncSetAttribute(sample_filtered_kernel<T, HELD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)(SF_HEAD + (HELD ? SF_HELD * 16 : 0)));
   if (e != cudaSuccess) return (int)e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(B * C));
@@ -1588,7 +1593,23 @@ int sample_filtered_launch(const SampleArgs& a, int B, cudaStream_t st) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = trlb_host::pdl_enabled() ? 2 : 1;
-  return (int)cudaLaunchKernelEx(&cfg, sample_filtered_kernel<T>, a, vecs);
+  return (int)cudaLaunchKernelEx(&cfg, sample_filtered_kernel<T, HELD>, a, vecs);
+}
+template <typename T>
+int sample_filtered_pick(const SampleArgs& a, int B, cudaStream_t st) {
+  // Blocks a row, up to the 8 of a portable cluster: as few as hold it in their shared memory, two blocks an SM, and more while
+  // there are fewer than one an SM.  More rows than that makes one wave of are not held: they get as many blocks each as make one
+  // wave, and at least two, so that a long row (top-p of a flat one takes five times as long as top-k) has two SMs.  Measured
+  // with 256 rows of 128256 fp32 logits, all of one kind: held 311 us, two blocks 194, one block 194; of all kinds: 170, 116, 160.
+  // 64 rows of 152064 bf16 logits held 67 us, not held 72.
+  constexpr long long N = 16 / sizeof(T);
+  const long long sms = trlb_host::sm_count();
+  int C = 1;
+  while (C < 8 && (C * N * SF_HELD < a.V || (long long)C * B <= sms)) ++C;
+  const long long need = ((a.V + C - 1) / C + N - 1) / N;
+  if (need <= SF_HELD && (long long)C * B <= 2 * sms) return sample_filtered_launch<T, true>(a, B, C, (int)need, st);
+  C = (int)min(8ll, max(2ll, 2 * sms / B));
+  return sample_filtered_launch<T, false>(a, B, C, 0, st);
 }
 
 }  // namespace trlb
@@ -1618,8 +1639,8 @@ TRLB_API int trlb_sample_filtered(const SampleCall* call) {
   if (c.V < 1 || c.B < 0 || c.B > (1 << 27)) return -1;
   SampleArgs a{c.logits, c.row_stride, c.V, c.temperature, c.top_p, c.min_p, c.top_k, c.temperature_all, c.top_p_all, c.min_p_all,
                c.top_k_all, c.words, c.seed, c.step_ptr, c.tok, c.logp};
-  if (c.dtype == 0) return sample_filtered_launch<__nv_bfloat16>(a, c.B, c.stream);
-  if (c.dtype == 1) return sample_filtered_launch<__half>(a, c.B, c.stream);
-  if (c.dtype == 2) return sample_filtered_launch<float>(a, c.B, c.stream);
+  if (c.dtype == 0) return sample_filtered_pick<__nv_bfloat16>(a, c.B, c.stream);
+  if (c.dtype == 1) return sample_filtered_pick<__half>(a, c.B, c.stream);
+  if (c.dtype == 2) return sample_filtered_pick<float>(a, c.B, c.stream);
   return -2;
 }
