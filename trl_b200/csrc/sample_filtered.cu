@@ -225,6 +225,36 @@ struct SfRow {
   __device__ __forceinline__ void each(F f) const {
     each(f, [] { return false; });
   }
+  // f(logits, first column) over the block's vectors of N logits (or 1), as they are
+  template <typename F>
+  __device__ __forceinline__ void each_vector(F f) const {
+    constexpr int N = 16 / sizeof(T);
+    int i = v0 + threadIdx.x;
+    if (vec) {
+      constexpr int U = SF_BATCH / N;
+      const int n1 = v1 / N;
+#pragma unroll 1
+      for (int at = v0 / N + threadIdx.x; at < n1; at += U * SF_THREADS) {
+        uint4 u[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+          if (at + j * SF_THREADS < n1) u[j] = reinterpret_cast<const uint4*>(x)[at + j * SF_THREADS];
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+          if (at + j * SF_THREADS >= n1) break;
+          float y[N];
+          sf_unpack<T>(u[j], y);
+          f(y, (at + j * SF_THREADS) * N);
+        }
+      }
+      i = n1 * N + threadIdx.x;
+    }
+#pragma unroll 1
+    for (; i < v1; i += SF_THREADS) {
+      float y[1] = {sf_load(x, i)};
+      f(y, i);
+    }
+  }
   // The same, small instead of fast: for what rows hardly ever need.
   template <typename F>
   __device__ __forceinline__ void each_slowly(F f) const {
@@ -1120,6 +1150,19 @@ struct SfSampler {
       }
     };
     auto each = [&](auto f) { each_until(f, [] { return false; }); };
+    auto each_vector = [&](auto f) {
+      if constexpr (HELD) {
+#pragma unroll 1
+        for (int v = tid; v < vecs; v += SF_THREADS) {
+          float y[N];
+          sf_unpack<T>(data[v], y);
+          f(y, first + v * N);
+        }
+      } else {
+        const SfRow<T> q = r;
+        q.each_vector(f);
+      }
+    };
     SfShared& sh = s;
     // ---- the maximum of the block, the smallest of its threads' ----
     const int lane = tid & 31, wid = tid >> 5;
@@ -1225,7 +1268,7 @@ struct SfSampler {
       all = all || floor_mass <= goal;
     }
     if (all) {
-      draw(each, q, floor_mass, floor);
+      draw(each_vector, q, floor_mass, floor);
       cluster.sync();
       release(true);
       if (rank == 0) finish_blocks(0, fmaxf(floor, -SF_MAX), 0x7fffffff, floor_mass);
@@ -1256,31 +1299,36 @@ struct SfSampler {
     if (lead->upto - above > SF_LIST) return false;
     // above the bracket: the mass, and the draw (at least `goal` is kept); the bracket: listed
     {
-      const float reach = (float)(20.0855369 * 1.001 / goal), t = temperature;
-      const uint32_t w = word;
-      const bool most = greedy, as = as_sampler;
-      float part = 0.f, top = -INFINITY, top_z = 0.f;
-      int at = -1;
+      Draw d = {(float)(20.0855369 * 1.001 / goal), temperature, word, greedy, as_sampler, 0.f, -INFINITY, 0.f, -1};
       // linear_bin() < b0 and <= b1 without its conversion
       const float end0 = (float)b0, end1 = b1 == SF_BINS - 1 ? INFINITY : (float)(b1 + 1);
-      each([&](float x, int col) {
-        const float y = (h.xmax - x) * h.step;
-        if (y < end0 && x >= from) {
-          const float wt = h.weight(x);
-          part += wt;
-          consider(x, col, wt, reach, t, w, most, as, top, at, top_z);
-        } else if (y < end1 && x >= from) {
-          append(sh, x, col);
+      each_vector([&](auto& x, int col) {
+        constexpr int M = sizeof(x) / sizeof(float);
+        unsigned keep = 0, list = 0;
+#pragma unroll
+        for (int k = 0; k < M; ++k) {
+          const float y = (h.xmax - x[k]) * h.step;
+          if (x[k] >= from) {
+            keep |= (y < end0 ? 1u : 0u) << k;
+            list |= (y < end1 ? 1u : 0u) << k;
+          }
         }
+        list &= ~keep;
+        if (list) {
+#pragma unroll
+          for (int k = 0; k < M; ++k)
+            if (list >> k & 1) append(sh, x[k], col + k);
+        }
+        if (keep) consider_vector(h, d, x, col, keep);
       });
-      if (most && at >= 0) top_z = quotient(top_z);
-      const double sum = sf_block_sum((double)part, sh);
-      sf_block_best(top, at, top_z, sh);
+      if (greedy && d.at >= 0) d.top_z = quotient(d.top_z);
+      const double sum = sf_block_sum((double)d.part, sh);
+      sf_block_best(d.top, d.at, d.top_z, sh);
       if (tid == 0) {
         sh.sums[1] = sum;
-        sh.best = top;
-        sh.best_col = at;
-        sh.best_z = top_z;
+        sh.best = d.top;
+        sh.best_col = d.at;
+        sh.best_z = d.top_z;
       }
     }
     const int n = collect();
@@ -1312,20 +1360,57 @@ struct SfSampler {
     }
     if (at < 0 || k > top || (k == top && col < at)) { top = k; at = col; top_z = z; }
   }
+  // The same for those of a vector's logits x[] that `keep` names, from column col on, and their mass.  All their random bits are
+  // made before the first branch, so that the eight chains run beside each other.
+  struct Draw {
+    float reach, t;
+    uint32_t word;
+    bool most, as;
+    float part, top, top_z;
+    int at;
+  };
+  template <int M>
+  static __device__ __forceinline__ void consider_vector(const Pass& q, Draw& d, const float (&x)[M], int col, unsigned keep) {
+    if (d.most) {  // a thread's columns ascend: the first of equals stays
+#pragma unroll
+      for (int k = 0; k < M; ++k) {
+        const bool in = keep >> k & 1;
+        d.part += in ? q.weight(x[k]) : 0.f;
+        if (in && (d.at < 0 || x[k] > d.top)) { d.top = d.top_z = x[k]; d.at = col + k; }
+      }
+      return;
+    }
+    const float margin = d.as ? 1.f + 2e-6f : 1.f + 3e-7f;
+    unsigned maybe = 0;
+#pragma unroll
+    for (int k = 0; k < M; ++k) {
+      const bool in = keep >> k & 1;
+      const float w = in ? q.weight(x[k]) : 0.f;
+      const uint32_t h = sf_bits(d.word, (uint32_t)(col + k));
+      d.part += w;
+      if (in && !(__uint_as_float(0x3f800000u | ~h >> 9) > fmaf(d.reach, w, margin))) maybe |= 1u << k;
+    }
+    if (maybe) {
+#pragma unroll
+      for (int k = 0; k < M; ++k)
+        if (maybe >> k & 1) consider(x[k], col + k, INFINITY, INFINITY, d.t, d.word, false, d.as, d.top, d.at, d.top_z);
+    }
+  }
   // This block's draw among its tokens of at least `floor`.
   template <typename E>
-  __device__ __forceinline__ void draw(E each, const Pass& q, double mass, float floor) {
-    const float reach = (float)(20.0855369 * 1.001 / mass), t = temperature, from = fmaxf(floor, -SF_MAX);
-    const uint32_t w = word;
-    const bool most = greedy, as = as_sampler;
-    float top = -INFINITY, top_z = 0.f;
-    int at = -1;
-    each([&](float x, int col) {
-      if (x >= from) consider(x, col, q.weight(x), reach, t, w, most, as, top, at, top_z);
+  __device__ __forceinline__ void draw(E each_vector, const Pass& q, double mass, float floor) {
+    const float from = fmaxf(floor, -SF_MAX);
+    Draw d = {(float)(20.0855369 * 1.001 / mass), temperature, word, greedy, as_sampler, 0.f, -INFINITY, 0.f, -1};
+    each_vector([&](auto& x, int col) {
+      constexpr int M = sizeof(x) / sizeof(float);
+      unsigned keep = 0;
+#pragma unroll
+      for (int k = 0; k < M; ++k) keep |= (x[k] >= from ? 1u : 0u) << k;
+      if (keep) consider_vector(q, d, x, col, keep);
     });
-    if (most && at >= 0) top_z = quotient(top_z);
-    sf_block_best(top, at, top_z, s);
-    if (tid == 0) { s.best = top; s.best_col = at; s.best_z = top_z; }
+    if (greedy && d.at >= 0) d.top_z = quotient(d.top_z);
+    sf_block_best(d.top, d.at, d.top_z, s);
+    if (tid == 0) { s.best = d.top; s.best_col = d.at; s.best_z = d.top_z; }
   }
   // The smallest logit that min-p keeps.
   __device__ __noinline__ float least_logit(float min_p) const {
