@@ -424,3 +424,24 @@ def test_attention_repeats_itself(D, Hq, Hk):
         assert torch.equal(first, F.kv8_decode_attn(q, *cache, table, at, D**-0.5))
     torch.cuda.synchronize()
     assert torch.equal(first, beside)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_sampling_of_more_rows_than_are_held(dtype):
+    """Rows that start at odd places, of all kinds of parameters, some with infinities and NaN."""
+    rows, vocab = 330, 4099
+    logits, rng = _logits(rows, vocab, torch.float32, seed=3, sharp=1.5)
+    g = torch.Generator().manual_seed(9)
+    logits[::11, :2000] = -math.inf
+    logits[5::37, 17] = math.nan
+    logits[6::41, 400] = math.inf
+    logits[7::53] = -math.inf
+    logits[8::59] = 0.25
+    logits = logits.to(dtype)
+    kw = {"temperature": torch.where(torch.rand(rows, generator=g) < 0.1, 0.0, 0.2 + torch.rand(rows, generator=g) * 2),
+          "top_k": torch.where(torch.rand(rows, generator=g) < 0.5, 0, torch.randint(0, 1500, (rows,), generator=g)).to(torch.int32),
+          "top_p": 0.2 + torch.rand(rows, generator=g), "min_p": torch.rand(rows, generator=g) * 0.1 * (torch.rand(rows, generator=g) < 0.5)}
+    tok, logp = F.sample_filtered(logits, rng, **{k: v.cuda() for k, v in kw.items()})
+    check_sample(logits, rng, tok, logp, **kw)
+    few = F.sample_filtered(logits[40:60], rng[40:60], **{k: v[40:60].cuda() for k, v in kw.items()})
+    assert torch.equal(tok[40:60], few[0])  # a row's draw does not depend on how many there are

@@ -1499,6 +1499,7 @@ struct SfSampler {
     const float top_p = a.top_p ? a.top_p[row] : a.top_p_all, min_p = a.min_p ? a.min_p[row] : a.min_p_all;
     const int top_k = a.top_k ? a.top_k[row] : a.top_k_all;
     const bool by_k = top_k > 0 && top_k < a.V, by_p = top_p < 1.f;
+    cluster.sync();  // what fast() has left may still be read
     // ---- the maximum, and the mass relative to each thread's own ----
     float mine = -INFINITY, part = 0.f;
     {
