@@ -1096,6 +1096,8 @@ def allreduce_add_rmsnorm(arena, byte_offset, buf_elems, res, w, eps, sync, out=
 # 8-bit paged cache (csrc/kv8.cu, csrc/kv8_attn.cu) and filtered sampling (csrc/sample_filtered.cu)
 # -------------------------------------------------------------------------------------------
 _KV8_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_KV8_PAGES, _KV8_DIMS = frozenset((16, 32, 64, 128)), frozenset((64, 96, 128, 256))
+_E4M3, _F32, _I32 = torch.float8_e4m3fn, torch.float32, torch.int32
 _TYPES = {"p": c_void_p, "i": c_int, "l": c_longlong, "f": c_float, "u": ctypes.c_uint, "s": ctypes.c_char_p}
 _bound: dict = {}
 
@@ -1141,19 +1143,19 @@ def _same_device(index, **tensors):
 
 
 def _want_i32(t, name):
-    if t.dtype != torch.int32 or not t.is_contiguous():
+    if t.dtype != _I32 or not t.is_contiguous():
         raise ValueError(f"{name} has to be a contiguous int32 tensor")
 
 
 def _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table):
     """(pages, heads, page size, head dim, device) of a cache as :func:`functional.kv8_alloc` makes it."""
     shape = k_cache.shape
-    if len(shape) != 4 or v_cache.shape != shape or k_cache.dtype != torch.float8_e4m3fn or v_cache.dtype != torch.float8_e4m3fn:
+    if len(shape) != 4 or v_cache.shape != shape or not k_cache.dtype == v_cache.dtype == _E4M3:
         raise ValueError("the codes of keys and values are float8_e4m3fn tensors [pages, heads, page size, head dim] of one shape")
     pages, heads, page, dim = shape
-    if page < 16 or page > 128 or page & (page - 1) or dim not in (64, 96, 128, 256):
+    if page not in _KV8_PAGES or dim not in _KV8_DIMS:
         raise ValueError(f"page sizes are 16, 32, 64 or 128 and head dims 64, 96, 128 or 256, not {page} and {dim}")
-    if k_scale.shape != shape[:2] or v_scale.shape != shape[:2] or k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+    if not k_scale.shape == v_scale.shape == (pages, heads) or not k_scale.dtype == v_scale.dtype == _F32:
         raise ValueError(f"k_scale and v_scale have to be fp32 [pages, heads] = [{pages}, {heads}]")
     if (k_cache.data_ptr() | v_cache.data_ptr()) & 15 or not (k_cache.is_contiguous() and v_cache.is_contiguous()
                                                               and k_scale.is_contiguous() and v_scale.is_contiguous()):
@@ -1167,29 +1169,31 @@ def _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table):
     return pages, heads, page, dim, index
 
 
-def _kv8_rows(t, name, heads, dim):
-    """[tokens, heads, dim] with dense rows on 16 bytes."""
-    shape = t.shape
-    if len(shape) != 3 or shape[1] != heads or shape[2] != dim:
-        raise ValueError(f"{name} has to be [tokens, {heads}, {dim}], not {tuple(shape)}")
+def _kv8_rows(t, mask):
+    """(tensor, stride of its tokens, of its heads) of [tokens, heads, dim] with dense rows on 16 bytes: of ``mask`` + 1 values."""
     a, b, c = t.stride()
-    mask = 16 // t.element_size() - 1
     if c != 1 or (a | b) & mask or t.data_ptr() & 15:
         t = t.contiguous()
-    return t
+        a, b, _ = t.stride()
+    return t, a, b
 
 
+_kv8_scratch: dict = {}  # fp32 words that attention needs, by heads, head dim and device
 _KV8_APPEND = struct.Struct("12P4q10i")
 
 
 def kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, starts, *, cu_seqlens=None, slots=None, max_new=None):
     """See :func:`functional.kv8_append`."""
     pages, heads, page, dim, index = _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table)
-    dtype = _KV8_DTYPES.get(k.dtype)
-    if dtype is None or k.dtype != v.dtype or k.shape != v.shape:
+    kind, shape = k.dtype, k.shape
+    dtype = _KV8_DTYPES.get(kind)
+    if dtype is None or v.dtype != kind or v.shape != shape:
         raise ValueError("k and v have to be bf16, fp16 or fp32 tensors of one type and shape")
-    k, v = _kv8_rows(k, "k", heads, dim), _kv8_rows(v, "v", heads, dim)
-    tokens, n = k.shape[0], starts.shape[0]
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim:
+        raise ValueError(f"k has to be [tokens, {heads}, {dim}], not {tuple(shape)}")
+    mask = 3 if dtype == 2 else 7
+    (k, k_tok, k_head), (v, v_tok, v_head) = _kv8_rows(k, mask), _kv8_rows(v, mask)
+    tokens, n = shape[0], len(starts)
     rows, blocks = block_table.shape
     _want_i32(starts, "starts")
     if not index == k.get_device() == v.get_device() == starts.get_device():
@@ -1215,8 +1219,6 @@ def kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, starts, *,
         return
     if max_new < 1:
         raise ValueError("max_new is the largest number of new tokens of a sequence: at least 1")
-    k_tok, k_head, _ = k.stride()
-    v_tok, v_head, _ = v.stride()
     call = _KV8_APPEND.pack(k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
                             v_scale.data_ptr(), block_table.data_ptr(), starts.data_ptr(), _ptr(cu_seqlens), _ptr(slots),
                             _status_ptr(index), _raw_stream(index), k_tok, k_head, v_tok, v_head, dtype, pages, heads, page,
@@ -1272,17 +1274,20 @@ def kv8_decode_attn(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens
     if window is not None and window < 1:
         raise ValueError("a window sees at least the newest token")
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(shape)
     elif out.shape != shape or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() & 15 or out.get_device() != index:
         raise ValueError("out has to be contiguous, on 16 bytes, of the shape, type and device of q")
     if B == 0:
         return out
     # scratch of this call alone: calls on other streams, and graphs, have their own
-    part = torch.empty(_fn("trlb_kv8_attn_scratch", "iiii", c_longlong)(index, Hq, heads, dim), dtype=torch.float32, device=q.device)
+    words = _kv8_scratch.get((Hq, heads, dim, index))
+    if words is None:
+        words = _kv8_scratch[Hq, heads, dim, index] = _fn("trlb_kv8_attn_scratch", "iiii", c_longlong)(index, Hq, heads, dim)
+    part = k_scale.new_empty(words)
     call = _KV8_ATTN.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                           block_table.data_ptr(), seq_lens.data_ptr(), _ptr(slots), part.data_ptr(), out.data_ptr(),
                           _status_ptr(index), _raw_stream(index), a, b, _KV8_DTYPES[q.dtype], pages, page, rows, blocks, B, Hq,
-                          heads, dim, min(window or 0, 2**31 - 1), part.numel(), scale)
+                          heads, dim, min(window or 0, 2**31 - 1), words, scale)
     _launch(index, _fn("trlb_kv8_decode_attn", "s"), "kv8_decode_attn", call)
     return out
 
@@ -1322,12 +1327,14 @@ def sample_filtered(logits, rng=None, *, temperature=1.0, top_k=0, top_p=1.0, mi
             rng = rng.to(torch.int32).contiguous()
     (t, t0), (k, k0) = _per_row(temperature, "temperature", B, torch.float32, index), _per_row(top_k, "top_k", B, torch.int32, index)
     (p, p0), (m, m0) = _per_row(top_p, "top_p", B, torch.float32, index), _per_row(min_p, "min_p", B, torch.float32, index)
-    tok = torch.empty(B, dtype=torch.int32, device=logits.device) if out_tok is None else out_tok
-    logp = torch.empty(B, dtype=torch.float32, device=logits.device) if out_logp is None else out_logp
-    for name, x, dt in (("out_tok", out_tok, torch.int32), ("out_logp", out_logp, torch.float32)):
-        if x is not None and (x.shape != (B,) or x.dtype != dt or not x.is_contiguous()):
-            raise ValueError(f"{name} has to be a contiguous {dt} tensor [{B}]")
-    _same_device(index, rng=rng, step_ptr=step_ptr, out_tok=out_tok, out_logp=out_logp)
+    tok = logits.new_empty(B, dtype=_I32) if out_tok is None else out_tok
+    logp = logits.new_empty(B, dtype=_F32) if out_logp is None else out_logp
+    if out_tok is not None or out_logp is not None:
+        for name, x, dt in (("out_tok", out_tok, _I32), ("out_logp", out_logp, _F32)):
+            if x is not None and (x.shape != (B,) or x.dtype != dt or not x.is_contiguous()):
+                raise ValueError(f"{name} has to be a contiguous {dt} tensor [{B}]")
+        _same_device(index, out_tok=out_tok, out_logp=out_logp)
+    _same_device(index, rng=rng, step_ptr=step_ptr)
     if B == 0:
         return tok, logp
     call = _SAMPLE_FILTERED.pack(logits.data_ptr(), _ptr(t), _ptr(k), _ptr(p), _ptr(m), _ptr(rng), _ptr(step_ptr),
