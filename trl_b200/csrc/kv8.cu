@@ -137,7 +137,8 @@ struct Kv8Source {
 
 // The new rows of pages, read once into registers: their largest magnitude decides the scale, then they are written.  A group
 // of threads (a warp for pages of up to 2048 values, else the block) takes one page and ITEMS of its 2 x heads tiles (head, keys
-// or values), whose loads are all under way together.  Bound by the bytes: 2 or 4 read and 1 written a value.
+// or values), whose loads are all under way together.  Bound by the bytes, 2 or 4 read and 1 written a value: 65536 tokens of
+// 8 heads and 128 dimensions in bf16 take 70 us, 5.7 TB/s; 16 prompts of up to 1024 tokens 7.8 us, a page's chain of reads.
 template <typename T, int VECS, int ITEMS, bool WARP>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 || VECS == 16 ? 2 : 4)
 kv8_append_pages_kernel(Kv8Source<T> src, Kv8Cache c, const int* __restrict__ table, int table_rows, int max_blocks,

@@ -22,6 +22,9 @@
 //   4. a last pass over the row draws among what is kept.
 // A row that fits into the shared memory of a cluster is read once and stays there for all of it (SfSampler::fast); the few rows
 // that need what fast() leaves out, and larger ones, are read again for each pass (SfSampler::run).
+// Measured: one row of 152064 bf16 logits with top-k 20 and top-p 0.8 13.2 us; 64 rows with top-p 0.95 72 us, of which the
+// flattest row's 60 us are: load 3, mass 4, list given up 3, histogram 7, its border's bins 6, draw 18, list of the bracket 4, border 6,
+// last draw 4; 256 rows of 128256 fp32 logits with parameters of all kinds 116 us.
 // Counts and the sums over lists are integers, other sums are taken in a fixed order: results do not depend on timing.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
@@ -656,7 +659,8 @@ struct SfSampler {
   // ---- the first block alone: borders in its list of n tokens -----------------------------------------------------------
   __device__ __forceinline__ unsigned long long whole(double w) const { return (unsigned long long)(w * SF_UNIT + 0.5); }
   // Where one of n <= SF_THREADS entries stands among them: entries before it and their mass; is_k: its logit is at least that of
-  // the k-th.  Up to SF_FEW each is compared with all others, by each_of(n) threads, more are sorted: measured alike at 100.
+  // the k-th.  Up to SF_FEW each is compared with all others, by as many threads as there are for it, more are sorted: of 44 that takes 4.9 us
+  // instead of 5.8, of 59 6.9 instead of 8.4, of 117 as long as sorting.
   struct Place {
     unsigned long long entry, own, before;
     unsigned rank;
