@@ -1105,12 +1105,35 @@ struct SfSampler {
     const bool by_k = top_k > 0 && top_k < a.V, by_p = top_p < 1.f;
     if (by_k && top_k > min(SF_LIST / 4, C * SF_THREADS / 2)) return false;  // too many for the lists
     const int first = r.v0;
-    float mine = -INFINITY;
+    // A thread's maximum and, where it counts, the mass relative to it.
+    float mine = -INFINITY, part = 0.f;
+    const float per_unit = c;
+    auto take = [&](auto& y) {
+      constexpr int M = sizeof(y) / sizeof(float);
+      float top = y[0];
+#pragma unroll
+      for (int k = 1; k < M; ++k) top = fmaxf(top, y[k]);
+      if (by_k) {
+        mine = fmaxf(mine, top);
+        return;
+      }
+      if (top > mine) {  // rare after the first few
+        part *= fast_exp2((mine - top) * per_unit);
+        mine = top;
+      }
+      if (mine > -INFINITY)
+#pragma unroll
+        for (int k = 0; k < M; ++k) part += fast_exp2((y[k] - mine) * per_unit);
+    };
     if constexpr (!HELD) {
       // what is NaN or has no finite quotient spoils the maximum, and the row: run() cleans each logit
       const SfRow<T> q = r;
       bool fine = true;
-      q.template each<true>([&](float x, int) { mine = fmaxf(mine, x); fine = fine && x <= q.cap; }, [] { return false; });
+      q.each_vector([&](auto& y, int) {
+#pragma unroll
+        for (int k = 0; k < (int)(sizeof(y) / sizeof(float)); ++k) fine = fine && y[k] <= q.cap;
+        take(y);
+      });
       if (!fine) mine = INFINITY;
     } else {
       const SfRow<T> q = r;
@@ -1133,8 +1156,7 @@ struct SfSampler {
         sf_clean<T>(u, q.cap);
         float y[N];
         sf_unpack<T>(u, y);
-#pragma unroll
-        for (int k = 0; k < N; ++k) mine = fmaxf(mine, y[k]);
+        take(y);
         data[v] = u;
       }
     }
@@ -1207,13 +1229,10 @@ struct SfSampler {
       if (rank == 0) top_k_of_list(n, top_k, by_p, top_p, min_p > 0.f ? least_logit(min_p) : -INFINITY);
       return true;
     }
-    // ---- the mass relative to the block's maximum; then both for the row ----
+    // ---- the mass relative to the block's maximum, then that of the row ----
     double total;
     {
-      const float k = c;
-      float part = 0.f;
-      if (bmax > -INFINITY) each([&](float x, int) { part += fast_exp2((x - bmax) * k); });
-      const double sum = sf_block_sum((double)part, sh);
+      const double sum = sf_block_sum(mine > -INFINITY ? (double)(part * fast_exp2((mine - bmax) * per_unit)) : 0., sh);
       if (tid == 0) { sh.fmax = bmax; sh.sums[0] = sum; }
       cluster.sync();
       xmax = max_of([](const SfShared& o) { return o.fmax; });
