@@ -156,7 +156,7 @@ def test_alloc_refuses():
 @pytest.mark.parametrize("kw, message", [
     (dict(logits=torch.zeros(3, dtype=torch.float32)), "vocabulary"), (dict(logits=torch.zeros(3, 5, dtype=torch.float64)), "bf16, fp16 or fp32"),
     (dict(rng=torch.zeros(2, dtype=torch.int32)), "rng"), (dict(rng=torch.zeros(3)), "rng"), (dict(top_p=torch.ones(2)), "top_p"),
-    (dict(out_tok=torch.zeros(3, dtype=torch.int64)), "out_tok"), (dict(logits=torch.zeros(3, 0)), "vocabulary")])
+    (dict(out_tok=torch.zeros(3, dtype=torch.int64)), "out_tok"), (dict(step_ptr=torch.zeros(1, dtype=torch.int64)), "step_ptr"), (dict(logits=torch.zeros(3, 0)), "vocabulary")])
 def test_sampling_refuses(kw, message):
     from trl_b200.ops import cuda as K
 

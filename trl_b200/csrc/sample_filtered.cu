@@ -22,9 +22,9 @@
 //   4. a last pass over the row draws among what is kept.
 // A row that fits into the shared memory of a cluster is read once and stays there for all of it (SfSampler::fast); the few rows
 // that need what fast() leaves out, and larger ones, are read again for each pass (SfSampler::run).
-// Measured: one row of 152064 bf16 logits with top-k 20 and top-p 0.8 13.2 us; 64 rows with top-p 0.95 72 us, of which the
-// flattest row's 60 us are: load 3, mass 4, list given up 3, histogram 7, its border's bins 6, draw 18, list of the bracket 4, border 6,
-// last draw 4; 256 rows of 128256 fp32 logits with parameters of all kinds 116 us.
+// Measured: one row of 152064 bf16 logits with top-k 20 and top-p 0.8 13.3 us; 64 rows with top-p 0.95 71 us, of which the
+// flattest row's 61 us are: load and mass 8, list given up 4, histogram 8, its border's bins 8, draw 20, list of the bracket 5,
+// border 5, last draw 3; 256 rows of 128256 fp32 logits with parameters of all kinds 114 us.
 // Counts and the sums over lists are integers, other sums are taken in a fixed order: results do not depend on timing.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>

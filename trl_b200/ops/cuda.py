@@ -1334,6 +1334,8 @@ def sample_filtered(logits, rng=None, *, temperature=1.0, top_k=0, top_p=1.0, mi
             if x is not None and (x.shape != (B,) or x.dtype != dt or not x.is_contiguous()):
                 raise ValueError(f"{name} has to be a contiguous {dt} tensor [{B}]")
         _same_device(index, out_tok=out_tok, out_logp=out_logp)
+    if step_ptr is not None:
+        _want_i32(step_ptr, "step_ptr")
     _same_device(index, rng=rng, step_ptr=step_ptr)
     if B == 0:
         return tok, logp
