@@ -22,7 +22,7 @@
 //   4. a last pass over the row draws among what is kept.
 // A row that fits into the shared memory of a cluster is read once and stays there for all of it (SfSampler::fast); the few rows
 // that need what fast() leaves out, and larger ones, are read again for each pass (SfSampler::run).
-// Measured: one row of 152064 bf16 logits with top-k 20 and top-p 0.8 13.3 us; 64 rows with top-p 0.95 71 us, of which the
+// Measured: one row of 152064 bf16 logits with top-k 20 and top-p 0.8 13.3 us; 64 rows with top-p 0.95 71 us (32 rows 48 us), of which the
 // flattest row's 61 us are: load and mass 8, list given up 4, histogram 8, its border's bins 8, draw 20, list of the bracket 5,
 // border 5, last draw 3; 256 rows of 128256 fp32 logits with parameters of all kinds 114 us.
 // Counts and the sums over lists are integers, other sums are taken in a fixed order: results do not depend on timing.
@@ -1685,16 +1685,11 @@ sample_filtered_kernel(const __grid_constant__ SampleArgs a, int vecs) {
 }
 
 template <typename T, bool HELD>
-int sample_filtered_launch(const SampleArgs& a, int B, int C, int vecs, cudaStream_t st) {
-  cudaError_t e = cudaFuncSetAttribute(sample_filtered_kernel<T, HELD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)(SF_HEAD + (HELD ? SF_HELD * 16 : 0)));
-  if (e != cudaSuccess) return (int)e;
-  cudaLaunchConfig_t cfg = {};
+void sample_filtered_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute (&attr)[2], int B, int C, int vecs, cudaStream_t st) {
   cfg.gridDim = dim3((unsigned)(B * C));
   cfg.blockDim = dim3(SF_THREADS);
   cfg.dynamicSmemBytes = SF_HEAD + (size_t)vecs * 16;
   cfg.stream = st;
-  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = C;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
@@ -1702,22 +1697,56 @@ int sample_filtered_launch(const SampleArgs& a, int B, int C, int vecs, cudaStre
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = trlb_host::pdl_enabled() ? 2 : 1;
+}
+template <typename T, bool HELD>
+cudaError_t sample_filtered_ready() {
+  return cudaFuncSetAttribute(sample_filtered_kernel<T, HELD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              (int)(SF_HEAD + (HELD ? SF_HELD * 16 : 0)));
+}
+// Clusters of C blocks that find a place at once, asked for once: on 148 SMs 148 of 2, 71 of 4, 56 of 5, 33 of 8.
+template <typename T, bool HELD>
+int sample_filtered_places(int device, int C) {
+  static int known[64][9] = {};  // a second thread that asks at once writes the same
+  if (device < 64 && known[device][C] > 0) return known[device][C];
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  sample_filtered_config<T, HELD>(cfg, attr, 1, C, HELD ? SF_HELD : 0, nullptr);
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (sample_filtered_ready<T, HELD>() != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, sample_filtered_kernel<T, HELD>, &cfg) != cudaSuccess || n < 1) {
+    (void)cudaGetLastError();
+    n = 1;
+  }
+  if (device < 64) known[device][C] = n;
+  return n;
+}
+template <typename T, bool HELD>
+int sample_filtered_launch(const SampleArgs& a, int B, int C, int vecs, cudaStream_t st) {
+  const cudaError_t e = sample_filtered_ready<T, HELD>();
+  if (e != cudaSuccess) return (int)e;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  sample_filtered_config<T, HELD>(cfg, attr, B, C, vecs, st);
   return (int)cudaLaunchKernelEx(&cfg, sample_filtered_kernel<T, HELD>, a, vecs);
 }
 template <typename T>
 int sample_filtered_pick(const SampleArgs& a, int B, cudaStream_t st) {
-  // Blocks a row, up to the 8 of a portable cluster: as few as hold it in their shared memory, two blocks an SM, and more while
-  // there are fewer than one an SM.  More rows than that makes one wave of are not held: they get as many blocks each as make one
-  // wave, and at least two, so that a long row (top-p of a flat one takes five times as long as top-k) has two SMs.  Measured
-  // with 256 rows of 128256 fp32 logits, all of one kind: held 311 us, two blocks 194, one block 194; of all kinds: 170, 116, 160.
-  // 64 rows of 152064 bf16 logits held 67 us, not held 72.
+  // Blocks a row, up to the 8 of a portable cluster: enough to hold it in their shared memory, and as many more as all rows find a
+  // place for at once.  More rows than that are not held: they get as many blocks as find a place, and at least two, so that a long
+  // row (top-p of a flat one takes five times as long as top-k) has two SMs.  Measured with 256 rows of 128256 fp32 logits, all of
+  // one kind: held 311 us, two blocks 194, one block 194; of all kinds: 170, 116, 160.  64 rows of 152064 bf16 logits: held 67 us,
+  // not held 72; 32 of them with 8 blocks each 48, with 5 56; 72 of them, held in two waves, 93.
   constexpr long long N = 16 / sizeof(T);
-  const long long sms = trlb_host::sm_count();
-  int C = 1;
-  while (C < 8 && (C * N * SF_HELD < a.V || (long long)C * B <= sms)) ++C;
-  const long long need = ((a.V + C - 1) / C + N - 1) / N;
-  if (need <= SF_HELD && (long long)C * B <= 2 * sms) return sample_filtered_launch<T, true>(a, B, C, (int)need, st);
-  C = (int)min(8ll, max(2ll, 2 * sms / B));
+  int device = 0, C = 1;
+  const cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return (int)e;
+  while (C < 8 && C * N * SF_HELD < a.V) ++C;
+  if (C * N * SF_HELD >= a.V && sample_filtered_places<T, true>(device, C) >= B) {
+    while (C < 8 && sample_filtered_places<T, true>(device, C + 1) >= B) ++C;
+    return sample_filtered_launch<T, true>(a, B, C, (int)(((a.V + C - 1) / C + N - 1) / N), st);
+  }
+  C = 8;
+  while (C > 2 && sample_filtered_places<T, false>(device, C) < B) --C;
   return sample_filtered_launch<T, false>(a, B, C, 0, st);
 }
 
