@@ -199,3 +199,15 @@ def test_a_trainer_on_the_cpu_refuses_an_8_bit_cache(tmp_path):
     args = GRPOConfig(output_dir=str(tmp_path), rollout_kv_cache_dtype="fp8", use_cpu=True)
     with pytest.raises(ValueError, match="rollout_kv_cache_dtype needs a GPU"):
         OnlineTrainer._get_rollout(SimpleNamespace(args=args, model=None, _rollout=None))
+
+
+@pytest.mark.parametrize("change, message", [
+    (dict(qkv=torch.zeros(3, 8 * 64 + 1, dtype=torch.bfloat16)), "dense rows"), (dict(bias=torch.zeros(512, dtype=torch.bfloat16)), "bias"),
+    (dict(lens=torch.zeros(3, dtype=torch.int64)), "seq_lens"), (dict(lens=torch.zeros(2, dtype=torch.int32)), "3 rows"),
+    (dict(q_out=torch.zeros(3, 3, 64, dtype=torch.bfloat16)), "q_out"), (dict(slots=torch.zeros(2, dtype=torch.int32)), "slots")])
+def test_rope_append_refuses(change, message):
+    from trl_b200.ops import cuda as K
+
+    a = {**_cuda_args(), "qkv": torch.zeros(3, 8 * 64, dtype=torch.bfloat16), "q_out": torch.zeros(3, 4, 64, dtype=torch.bfloat16), **change}
+    with pytest.raises(ValueError, match=message):
+        K.kv8_rope_append(a["qkv"], a.get("bias"), None, None, 1e-6, a["lens"], a.get("slots"), a["table"], a["q_out"], *a["cache"], 4, 1e4)

@@ -1236,6 +1236,15 @@ def kv8_rope_append(qkv, bias, q_norm, k_norm, norm_eps, seq_lens, slot_ids, blo
         raise ValueError("qkv has to be dense rows of bf16 or fp32 for heads of at most 128 values")
     if not f32 and bias is not None:
         raise ValueError("a bias belongs to fp32 sums: a bf16 row has it already")
+    _want_i32(seq_lens, "seq_lens")
+    if q_out.shape != (B, Hq, dim) or q_out.dtype != torch.bfloat16 or not q_out.is_contiguous():
+        raise ValueError(f"q_out has to be a contiguous bf16 tensor [{B}, {Hq}, {dim}]")
+    for name, x in (("slot_ids", slot_ids), ("pos_delta", pos_delta)):
+        if x is not None:
+            _want_i32(x, name)
+    if min(seq_lens.shape[0], block_table.shape[0]) < (B if slot_ids is None else 1) or (slot_ids is not None and slot_ids.shape != (B,)):
+        raise ValueError(f"{B} rows need as many lengths, rows of the block table and slots")
+    _same_device(index, qkv=qkv, bias=bias, q_norm=q_norm, k_norm=k_norm, seq_lens=seq_lens, slot_ids=slot_ids, q_out=q_out, pos_delta=pos_delta)
     _launch(index, _fn("trlb_kv8_rope_append", "pilpppfpppiipppppiiiiiifppp"), "kv8_rope_append", qkv.data_ptr(), int(f32),
             qkv.stride(0), _ptr(bias), _ptr(q_norm), _ptr(k_norm), norm_eps, seq_lens.data_ptr(), _ptr(slot_ids),
             block_table.data_ptr(), *block_table.shape, q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
