@@ -445,3 +445,22 @@ def test_sampling_of_more_rows_than_are_held(dtype):
     check_sample(logits, rng, tok, logp, **kw)
     few = F.sample_filtered(logits[40:60], rng[40:60], **{k: v[40:60].cuda() for k, v in kw.items()})
     assert torch.equal(tok[40:60], few[0])  # a row's draw does not depend on how many there are
+
+
+@pytest.mark.parametrize("D, Hq, Hk, page, dtype", [(64, 14, 2, 16, torch.bfloat16), (128, 34, 2, 64, torch.float16), (96, 5, 5, 32, torch.bfloat16), (256, 8, 1, 16, torch.bfloat16)])
+@pytest.mark.parametrize("room", [64, 600, 1600])
+def test_attention_of_few_rows_whatever_the_table_has_room_for(D, Hq, Hk, page, dtype, room):
+    """The room in the block table decides how the work is dealt, not what comes out."""
+    lens = [0, 1, 17, 63]
+    cache, narrow = filled_cache(lens, Hk, page, D, "cuda", seed=room)
+    table = torch.zeros(len(lens), room // page, dtype=torch.int32, device="cuda")
+    table[:, :narrow.shape[1]] = narrow
+    q = torch.randn(len(lens), Hq, D, device="cuda").to(dtype)
+    slots = _i32([3, 1, 0, 2])
+    at = _i32([n - 1 for n in lens])
+    for window in (None, 5):
+        out = F.kv8_decode_attn(q, *cache, table, at, D**-0.5, slots=slots, window=window)
+        order = [lens[i] for i in slots.tolist()]
+        want, tol = attention64(q.cpu(), [x.cpu() for x in cache], table[slots.long()].cpu(), order, D**-0.5, window)
+        assert ((out.cpu().double() - want).abs() <= tol).all()
+        assert (out[2] == 0).all()

@@ -27,6 +27,10 @@
 // a row writes its output.  Else it leaves (m, l, o); where all of a block's runs lie in one row, the block joins its warps'
 // first and leaves one.  The warp that has a row's first step says which row it is, for kv8_attn_join_kernel, which adds a
 // row's parts in the order of the warps.  No atomics: results do not depend on timing.
+//
+// Where there are no more rows than SMs and the block table has room for few steps a warp only (kv8_attn_alone), each row gets a
+// block of its own instead (by_row): no list of all rows, no parts, no second kernel.  One sequence of 211 tokens with 14 and 2
+// heads of 64 takes 6.3 us so, 10.2 us from the list.
 #include <cuda_fp16.h>
 
 #include "kv8.cuh"
@@ -44,6 +48,9 @@ constexpr float KA_NONE = -1e30f;    // maximum of no token: finite, so that exp
 // One block an SM, with as many warps as registers allow, and the steps in a warp's queue: about 190 KB of codes under way.
 __host__ __device__ constexpr int kv8_attn_warps(int D, int HT) { return D == 256 ? 8 : (D == 64 && HT == 8 ? 16 : 12); }
 __host__ __device__ constexpr int kv8_attn_stages(int D) { return D == 256 ? 3 : (D == 128 ? 4 : (D == 96 ? 5 : 6)); }
+// Steps of a warp up to which a block takes a row alone: 4 sequences with 28 and 4 heads of 128 take 10.0 us alone and 11.7 from
+// the list at 700 tokens, 11.8 and 12.9 at 1000, 13.9 and 13.2 at 1500; with 8 heads of 256 11.9 and 13.8 at 400, 15.1 and 13.4 at 700.
+__host__ __device__ constexpr int kv8_attn_alone(int D) { return D == 256 ? 3 : 5; }
 // Swizzle of a row's bytes in shared memory; 96 bytes stand as they are.
 __host__ __device__ constexpr int kv8_attn_swizzle(int D) { return D % 128 == 0 ? 128 : (D == 64 ? 64 : 0); }
 
@@ -106,7 +113,7 @@ struct Kv8AttnArgs {
   float2* part_ml;  // [2 * warps][HT]: their maxima and denominators
   SharedRow* rows;  // [warps]: the row whose first step is in a warp's run and whose last is not
   int* status;
-  int pages, Hk, G, tiles, page_shift, table_rows, max_blocks, B, window, min_run;
+  int pages, Hk, G, tiles, page_shift, table_rows, max_blocks, B, window, by_row;
   float scale;
 };
 
@@ -194,29 +201,59 @@ kv8_attn_kernel(const __grid_constant__ Kv8AttnArgs a) {
   }
   pdl_launch_dependents();
   pdl_wait();
-  kv8_prefix<KA_WARPS>(a, prefix, warp_sums);  // its barriers show the mbarriers, too
-  // sequences without a token to see have no steps: their zeros are written here
-  for (int b = blockIdx.x; b < a.B; b += gridDim.x)
-    if (prefix[b + 1] == prefix[b])
-      for (int i = tid; i < a.Hk * a.G * D; i += KA_THREADS)
-        store1(reinterpret_cast<T*>(a.out) + (size_t)b * a.Hk * a.G * D + i, 0.f);
   const int rows_per_seq = a.Hk * a.tiles, warp = blockIdx.x * KA_WARPS + wid;
-  const long long total = (long long)prefix[a.B] * rows_per_seq, warps = (long long)gridDim.x * KA_WARPS;
-  const long long run = max((long long)a.min_run, (total + warps - 1) / warps);
-  const long long u0 = (long long)warp * run, u1 = min(total, u0 + run);
-  const long long block0 = (long long)blockIdx.x * KA_WARPS * run, block1 = min(total, block0 + KA_WARPS * run);
-  SharedRow shared = {-1, 0, 0, 0, 0, 0, {0, 0}};
+  long long total, run, u0, u1, block0, block1;
   int b = 0;
   bool joined = false;  // all of the block's runs lie in one row
-  if (block0 < block1) {  // the sequence that the block begins in
-    int hi = a.B - 1;
-    while (b < hi) {
-      const int mid = (b + hi + 1) >> 1;
-      if ((long long)prefix[mid] * rows_per_seq <= block0) b = mid; else hi = mid - 1;
+  SharedRow shared = {-1, 0, 0, 0, 0, 0, {0, 0}};
+  if (a.by_row) {
+    b = blockIdx.x / rows_per_seq;
+    const int row = blockIdx.x % rows_per_seq;
+    if (tid == 0) {  // the row's sequence is all of the list
+      int lo, hi;
+      const int n = kv8_steps(a, b, lo, hi);
+      prefix[b] = 0;
+      prefix[b + 1] = n > 0 ? n + KA_ROW : 0;
     }
-    const int cost = prefix[b + 1] - prefix[b];
-    const long long seq0 = (long long)prefix[b] * rows_per_seq;
-    joined = seq0 + (long long)(kv8_div(block0 - seq0, cost) + 1) * cost >= block1;
+    __syncthreads();  // shows the mbarriers, too
+    const int cost = prefix[b + 1];
+    if (cost == 0) {
+      const int h0 = (row % a.tiles) * HT, heads = min(HT, a.G - h0);
+      for (int i = tid; i < heads * D; i += KA_THREADS)
+        store1(reinterpret_cast<T*>(a.out) + ((size_t)b * a.Hk * a.G + row / a.tiles * a.G + h0) * D + i, 0.f);
+      return;
+    }
+    total = (long long)cost * rows_per_seq;
+    run = (cost - KA_ROW + KA_WARPS - 1) / KA_WARPS;
+    block0 = (long long)row * cost + KA_ROW;
+    block1 = (long long)(row + 1) * cost;
+    u0 = min(block1, block0 + wid * run);
+    u1 = min(block1, u0 + run);
+    joined = true;
+  } else {
+    kv8_prefix<KA_WARPS>(a, prefix, warp_sums);  // its barriers show the mbarriers, too
+    // sequences without a token to see have no steps: their zeros are written here
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x)
+      if (prefix[b + 1] == prefix[b])
+        for (int i = tid; i < a.Hk * a.G * D; i += KA_THREADS)
+          store1(reinterpret_cast<T*>(a.out) + (size_t)b * a.Hk * a.G * D + i, 0.f);
+    const long long warps = (long long)gridDim.x * KA_WARPS;
+    total = (long long)prefix[a.B] * rows_per_seq;
+    run = max(1ll, (total + warps - 1) / warps);
+    u0 = (long long)warp * run;
+    u1 = min(total, u0 + run);
+    block0 = (long long)blockIdx.x * KA_WARPS * run;
+    block1 = min(total, block0 + KA_WARPS * run);
+    if (block0 < block1) {  // the sequence that the block begins in
+      int hi = a.B - 1;
+      while (b < hi) {
+        const int mid = (b + hi + 1) >> 1;
+        if ((long long)prefix[mid] * rows_per_seq <= block0) b = mid; else hi = mid - 1;
+      }
+      const int cost = prefix[b + 1] - prefix[b];
+      const long long seq0 = (long long)prefix[b] * rows_per_seq;
+      joined = seq0 + (long long)(kv8_div(block0 - seq0, cost) + 1) * cost >= block1;
+    }
   }
   if (lane < HT) sh_ml[wid][lane] = make_float2(KA_NONE, 0.f);
   uint8_t* queue = smem + wid * S * STAGE;
@@ -483,7 +520,7 @@ kv8_attn_kernel(const __grid_constant__ Kv8AttnArgs a) {
       }
     }
   }
-  if (lane == 0) a.rows[warp] = shared;
+  if (lane == 0 && !a.by_row) a.rows[warp] = shared;
   if (!joined) return;
   __syncthreads();  // each warp's sums stand in its queue, which is empty
   // (a warp behind the end of the list has seen no row)
@@ -626,6 +663,11 @@ kv8_attn_join_kernel(const __grid_constant__ Kv8AttnArgs a) {
   for (int e = 0; e < E; ++e) store1(out + lane + 32 * e, o[e] * inv);
 }
 
+// Whether each row gets a block: a rule on what the host knows, the room in the block table and the window.
+inline bool kv8_by_row(int D, int ht, long long rows, long long tokens, int window) {
+  const long long steps = (window > 0 && window + KA_STEP < tokens ? window + KA_STEP : tokens) / KA_STEP + 1;
+  return rows <= trlb_host::sm_count() && steps <= (long long)kv8_attn_alone(D) * kv8_attn_warps(D, ht);
+}
 inline int kv8_head_tile(int D, int G) { return G <= 8 || D > 128 ? 8 : 16; }
 
 template <int D, int HT, typename T>
@@ -646,11 +688,11 @@ int kv8_attn_launch(Kv8AttnArgs& a, const void* k, const void* v, cudaStream_t s
   if (trlb_host::make_tmap_3d_u8(&a.k, k, D, page, tiles, box, KA_STEP, kv8_attn_swizzle(D)) ||
       trlb_host::make_tmap_3d_u8(&a.v, v, D, page, tiles, box, KA_STEP, kv8_attn_swizzle(D)))
     return -6;
-  const int blocks = trlb_host::sm_count();
+  const int blocks = a.by_row ? a.B * a.Hk * a.tiles : trlb_host::sm_count();
   a.part_ml = reinterpret_cast<float2*>(a.part + (size_t)2 * blocks * WARPS * HT * D);  // each on 16 bytes
   a.rows = reinterpret_cast<SharedRow*>(a.part_ml + (size_t)2 * blocks * WARPS * HT);
   e = trlb_host::launch_kernel(kv8_attn_kernel<D, HT, T>, dim3(blocks), dim3(WARPS * 32), smem, st, trlb_host::pdl_enabled(), a);
-  if (e != cudaSuccess) return (int)e;
+  if (e != cudaSuccess || a.by_row) return (int)e;
   // it waits for the attention kernel by itself, so it may always be set up under that kernel's end
   return (int)trlb_host::launch_kernel(kv8_attn_join_kernel<D, HT, T>, dim3(blocks), dim3(KA_JOIN), 0, st, true, a);
 }
@@ -671,10 +713,11 @@ int kv8_attn_pick(Kv8AttnArgs& a, const void* k, const void* v, int D, cudaStrea
 
 using namespace trlb;
 
-// fp32 words of scratch that a call needs: parts of rows that several blocks share
-TRLB_API long long trlb_kv8_attn_scratch(int device, int Hq, int Hk, int D) {
-  (void)device;
+// fp32 words of scratch that a call needs: parts of rows that several blocks share.  `tokens`: what a row of the block table has
+// room for.
+TRLB_API long long trlb_kv8_attn_scratch(int B, int Hq, int Hk, int D, long long tokens, int window) {
   const int ht = kv8_head_tile(D, Hq / Hk);
+  if (kv8_by_row(D, ht, (long long)B * Hk * ((Hq / Hk + ht - 1) / ht), tokens, window)) return 0;
   return (2ll * ht * (D + 2) + sizeof(SharedRow) / 4) * kv8_attn_warps(D, ht) * trlb_host::sm_count();
 }
 
@@ -698,11 +741,13 @@ TRLB_API int trlb_kv8_decode_attn(const Kv8AttnCall* call) {
   if (c.Hk <= 0 || c.Hq <= 0 || c.Hq % c.Hk || c.B > KA_MAX_SEQS || c.window < 0) return -2;
   if (c.page_size < KA_STEP || (c.page_size & (c.page_size - 1))) return -3;
   if ((long long)c.pages * c.Hk > 2147483647ll) return -5;
-  if (c.part_words < trlb_kv8_attn_scratch(0, c.Hq, c.Hk, c.D)) return -7;
   int shift = 0;
   while ((1 << shift) < c.page_size) ++shift;
   Kv8AttnArgs a{{}, {}, c.q, c.q_row, c.q_head, c.k_scale, c.v_scale, c.table, c.seq_lens, c.slots, c.out, c.part, nullptr,
-                nullptr, c.status, c.pages, c.Hk, c.Hq / c.Hk, 1, shift, c.table_rows, c.max_blocks, c.B, c.window, 1, c.scale};
+                nullptr, c.status, c.pages, c.Hk, c.Hq / c.Hk, 1, shift, c.table_rows, c.max_blocks, c.B, c.window, 0, c.scale};
+  const long long words = trlb_kv8_attn_scratch(c.B, c.Hq, c.Hk, c.D, (long long)c.max_blocks << shift, c.window);
+  if (c.part_words < words) return -7;
+  a.by_row = words == 0;
   if (c.dtype == 0) return kv8_attn_pick<__nv_bfloat16>(a, c.k_codes, c.v_codes, c.D, c.stream);
   if (c.dtype == 1) return kv8_attn_pick<__half>(a, c.k_codes, c.v_codes, c.D, c.stream);
   return -4;

@@ -1178,7 +1178,7 @@ def _kv8_rows(t, mask):
     return t, a, b
 
 
-_kv8_scratch: dict = {}  # fp32 words that attention needs, by heads, head dim and device
+_kv8_scratch: dict = {}  # fp32 words that attention needs, by its sizes and device
 _KV8_APPEND = struct.Struct("12P4q10i")
 
 
@@ -1289,14 +1289,19 @@ def kv8_decode_attn(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens
     if B == 0:
         return out
     # scratch of this call alone: calls on other streams, and graphs, have their own
-    words = _kv8_scratch.get((Hq, heads, dim, index))
+    window = min(window or 0, 2**31 - 1)
+    sizes = (B, Hq, heads, dim, blocks * page, window, index)
+    words = _kv8_scratch.get(sizes)
     if words is None:
-        words = _kv8_scratch[Hq, heads, dim, index] = _fn("trlb_kv8_attn_scratch", "iiii", c_longlong)(index, Hq, heads, dim)
-    part = k_scale.new_empty(words)
+        if len(_kv8_scratch) > 10000:
+            _kv8_scratch.clear()
+        with torch.cuda.device(index):
+            words = _kv8_scratch[sizes] = _fn("trlb_kv8_attn_scratch", "iiiili", c_longlong)(*sizes[:-1])
+    part = k_scale.new_empty(words) if words else None
     call = _KV8_ATTN.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-                          block_table.data_ptr(), seq_lens.data_ptr(), _ptr(slots), part.data_ptr(), out.data_ptr(),
+                          block_table.data_ptr(), seq_lens.data_ptr(), _ptr(slots), _ptr(part), out.data_ptr(),
                           _status_ptr(index), _raw_stream(index), a, b, _KV8_DTYPES[q.dtype], pages, page, rows, blocks, B, Hq,
-                          heads, dim, min(window or 0, 2**31 - 1), words, scale)
+                          heads, dim, window, words, scale)
     _launch(index, _fn("trlb_kv8_decode_attn", "s"), "kv8_decode_attn", call)
     return out
 
