@@ -458,7 +458,7 @@ def test_attention_of_few_rows_whatever_the_table_has_room_for(D, Hq, Hk, page, 
     q = torch.randn(len(lens), Hq, D, device="cuda").to(dtype)
     slots = _i32([3, 1, 0, 2])
     at = _i32([n - 1 for n in lens])
-    for window in (None, 5):
+    for window in (None, 5, 2**31 - 1):
         out = F.kv8_decode_attn(q, *cache, table, at, D**-0.5, slots=slots, window=window)
         order = [lens[i] for i in slots.tolist()]
         want, tol = attention64(q.cpu(), [x.cpu() for x in cache], table[slots.long()].cpu(), order, D**-0.5, window)

@@ -664,7 +664,7 @@ kv8_attn_join_kernel(const __grid_constant__ Kv8AttnArgs a) {
 }
 
 // Whether each row gets a block: a rule on what the host knows, the room in the block table and the window.
-inline bool kv8_by_row(int D, int ht, long long rows, long long tokens, int window) {
+inline bool kv8_by_row(int D, int ht, long long rows, long long tokens, long long window) {
   const long long steps = (window > 0 && window + KA_STEP < tokens ? window + KA_STEP : tokens) / KA_STEP + 1;
   return rows <= trlb_host::sm_count() && steps <= (long long)kv8_attn_alone(D) * kv8_attn_warps(D, ht);
 }
