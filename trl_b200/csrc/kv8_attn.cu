@@ -3,8 +3,8 @@
 //   o = sum_j softmax_j(scale q . k_j) v_j,   k_j = code * k_scale[page, head],  v_j = code * v_scale[page, head]
 //
 // Bound by the cache's bytes: 2 D bytes a token and key head for 4 G D operations (G query heads share a key head).  Measured, with
-// 32 query and 8 key heads of 128: 131067 tokens of one sequence 53.6 us (268 MB: 5.3 TB/s in the main kernel), 128 sequences of up to
-// 8192 tokens 49.9 us; 64 sequences of 1024 tokens with 28 and 4 heads 22.7 us, of which 4 us pass before the first codes are
+// 32 query and 8 key heads of 128: 131067 tokens of one sequence 54.5 us (268 MB: 5.3 TB/s in the main kernel), 128 sequences of up to
+// 8192 tokens 49.9 us; 64 sequences of 1024 tokens with 28 and 4 heads 22.5 us, of which 4 us pass before the first codes are
 // there and 4 us in the join.
 //
 // A warp takes 16 tokens a step.  Each warp has a queue of steps in shared memory that its first lane keeps filled by TMA, a few
@@ -393,7 +393,8 @@ kv8_attn_kernel(const __grid_constant__ Kv8AttnArgs a) {
 
     int page_now = -1;
     float kscale = 0.f, lv = 0.f, inv_v = 0.f;
-    for (int s = s0; s < s1; ++s) {
+    int s = s0;
+    for (; s < s1; ++s) {
       copy();
       if (!mbar_wait(&full[wid][slot_out], parity, &abort_flag, a.status, SITE_KV8_ATTN)) break;
       const uint32_t kq = smem_u32(queue) + slot_out * STAGE, vq = kq + 16 * D;
@@ -490,6 +491,16 @@ kv8_attn_kernel(const __grid_constant__ Kv8AttnArgs a) {
           for (int n = 0; n < NT; ++n) mma_f16(o[2 * i + half][n], a0, a1, a2, a3, p[n][0], p[n][1]);
         }
       }
+    }
+    if (s < s1) {  // a wait has run out (reported): no more copies, and those under way are waited for, with a limit
+      for (; s < next; ++s) {
+        for (int i = 0; i < 1 << 16 && !mbar_try_wait(&full[wid][slot_out], parity); ++i) {}
+        if (++slot_out == S) {
+          slot_out = 0;
+          parity ^= 1;
+        }
+      }
+      u = u1;
     }
 
     // o[2 i + half][n]: dimensions 4 i' + 2 half of the lane's units, for the heads 2t ([0], [2]) and 2t + 1 ([1], [3])
