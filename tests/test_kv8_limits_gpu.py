@@ -1,0 +1,60 @@
+"""The 8-bit paged cache, its decode attention and filtered sampling at the limits of their numbers (B200)."""
+import pytest
+import torch
+
+from kv8_util import attention64, filled_cache
+from trl_b200.ops import functional as F
+
+pytestmark = pytest.mark.gpu
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _cpu(cache):
+    return [t.cpu() for t in cache]
+
+
+# rows that a block takes alone; that a warp takes whole; that a block's warps share; that several blocks share
+SHAPES = [("a block a row", [60, 17, 200, 33], 4, 2, 64, 16), ("a warp a row", [20 + i % 30 for i in range(700)], 8, 4, 64, 16),
+          ("a block's warps", [9000, 8500, 9100, 9050] * 3, 8, 4, 128, 64), ("blocks", [120000, 90001, 50], 8, 1, 128, 64)]
+
+
+# ---- attention -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("name, lens, Hq, Hk, D, page", SHAPES, ids=[s[0] for s in SHAPES])
+@pytest.mark.parametrize("what", ["nan query", "inf query", "-inf query", "nan key", "nan value"])
+def test_attention_keeps_nan_that_is_in_sight(name, lens, Hq, Hk, D, page, what):
+    """NaN comes out wherever the formula gives it, however a row is dealt to warps, and nowhere else."""
+    cache, table = filled_cache(lens, Hk, page, D, "cuda", seed=3, extra=0)
+    B, G = len(lens), Hq // Hk
+    q = torch.randn(B, Hq, D, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    bad = torch.zeros(B, Hq, D, dtype=torch.bool)
+    row, head = 1, Hq - 1
+    if what.endswith("query"):
+        if what != "nan query":  # scores of one sign: all +inf (NaN by inf - inf) or all -inf (0 / 0)
+            pages = table[row, : -(-lens[row] // page)].long()
+            u = cache[0].view(torch.uint8)
+            u[pages, head // G, :, 5] = torch.tensor([1.0]).to(torch.float8_e4m3fn).view(torch.uint8).item()
+        q[row, head, 5] = float(what.split()[0])
+        bad[row, head] = True
+    else:
+        at = lens[row] - 3
+        u = cache[0 if what == "nan key" else 1].view(torch.uint8)
+        u[int(table[row, at // page]), head // G, at % page, 7] = 0x7F
+        heads = slice(head // G * G, head // G * G + G)
+        bad[row, heads] = True
+        if what == "nan value":
+            bad[row, heads] = False
+            bad[row, heads, 7] = True
+    some = [0, 1, 2, B - 1] if B > 3 else list(range(B))
+    out = F.kv8_decode_attn(q, *cache, table, _i32([n - 1 for n in lens]), 0.01).cpu()
+    assert torch.equal(torch.isnan(out), bad)
+    clean, c8 = q.clone(), [t.clone() for t in cache]
+    clean[~torch.isfinite(clean)] = 0
+    for c in c8[:2]:
+        u = c.view(torch.uint8)
+        u[(u & 0x7F) == 0x7F] = 0
+    want, tol = attention64(clean[some].cpu(), _cpu(c8), table[some].cpu(), [lens[i] for i in some], 0.01)
+    err = (out[some].double() - want).abs()
+    assert (err <= tol)[~bad[some]].all()

@@ -357,7 +357,7 @@ kv8_attn_kernel(const __grid_constant__ Kv8AttnArgs a) {
     for (int n = 0; n < NT; ++n) {
       const int h = g + 8 * n;
       const T* qp = reinterpret_cast<const T*>(a.q) + (long long)b * a.q_row + (long long)(kvh * a.G + h0 + h) * a.q_head;
-      float most = 0.f;
+      uint32_t most = 0;  // the largest magnitude's bits: those of infinities and NaN are above all others
 #pragma unroll
       for (int w = 0; w < KW; ++w) {
         const int d = KU * (t + 4 * (w / (KU / 4))) + 4 * (w % (KU / 4));
@@ -365,13 +365,15 @@ kv8_attn_kernel(const __grid_constant__ Kv8AttnArgs a) {
         qa[w][2 * n] = raw.x;
         qa[w][2 * n + 1] = raw.y;
         const float2 x = unpack2<T>(raw.x), y = unpack2<T>(raw.y);
-        most = fmaxf(fmaxf(most, fmaxf(kv8_magnitude(x.x), kv8_magnitude(x.y))), fmaxf(kv8_magnitude(y.x), kv8_magnitude(y.y)));
+        auto bits = [](float f) { return __float_as_uint(f) & 0x7fffffffu; };
+        most = max(max(most, max(bits(x.x), bits(x.y))), max(bits(y.x), bits(y.y)));
       }
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-      const int e = min(120, max(-100, (int)(__float_as_uint(most) >> 23) - 127));
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      const int e = min(120, max(-100, (int)(most >> 23) - 127));
       const float inv = kv8_pow2(-e);
-      cq[n] = a.scale * 1.4426950408889634f * kv8_pow2(e);
+      // a query that is not finite has NaN as its output: its scores are infinite or NaN, all of them
+      cq[n] = most < 0x7f800000u ? a.scale * 1.4426950408889634f * kv8_pow2(e) : NAN;
 #pragma unroll
       for (int w = 0; w < KW; ++w)
 #pragma unroll
@@ -549,7 +551,7 @@ kv8_attn_kernel(const __grid_constant__ Kv8AttnArgs a) {
 #pragma unroll
     for (int w = 0; w < KA_WARPS; ++w) {
       const float2 ml = sh_ml[w][h];
-      if (ml.x == KA_NONE) continue;  // a warp without steps has written no sums
+      if (ml.x == KA_NONE && ml.y == 0.f) continue;  // a warp without steps has written no sums (one that saw NaN alone has)
       const float f = fast_exp2(ml.x - mx);
       const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + w * S * STAGE) + h * D + d);
       den = fmaf(ml.y, f, den);
