@@ -58,3 +58,22 @@ def test_attention_keeps_nan_that_is_in_sight(name, lens, Hq, Hk, D, page, what)
     want, tol = attention64(clean[some].cpu(), _cpu(c8), table[some].cpu(), [lens[i] for i in some], 0.01)
     err = (out[some].double() - want).abs()
     assert (err <= tol)[~bad[some]].all()
+
+
+@pytest.mark.parametrize("name, lens, Hq, Hk, D, page", SHAPES, ids=[s[0] for s in SHAPES])
+def test_attention_of_scores_far_below_zero(name, lens, Hq, Hk, D, page):
+    """All scores of a row equal and about -2^120: the softmax is uniform, the output the values' mean.
+
+    Its error: the output's half step, weights and sums 2^-11 of the magnitudes' mean.  One scale for all values: in 32 bits
+    scores of this size have steps of 2^97, beside which the logarithm of a page's scale is nothing."""
+    cache, table = filled_cache(lens, Hk, page, D, "cuda", seed=4, extra=0)
+    cache[0].view(torch.uint8).fill_(torch.tensor([1.0]).to(torch.float8_e4m3fn).view(torch.uint8).item())
+    cache[2].fill_(2.0**114)
+    cache[3].fill_(0.5)
+    q = torch.full((len(lens), Hq, D), -1.0, device="cuda", dtype=torch.bfloat16)
+    out = F.kv8_decode_attn(q, *cache, table, _i32([n - 1 for n in lens]), 1.0).cpu()
+    for b in {0, 1, len(lens) - 1}:
+        pages = table[b, : -(-lens[b] // page)].long()
+        v = (cache[1][pages].double() * cache[3][pages].double()[:, :, None, None]).transpose(0, 1).reshape(Hk, -1, D)[:, : lens[b]].cpu()
+        want, mags = (x.repeat_interleave(Hq // Hk, 0) for x in (v.mean(1), v.abs().mean(1)))
+        assert ((out[b].double() - want).abs() <= torch.finfo(torch.bfloat16).eps / 2 * want.abs() + 2.0**-10 * mags).all()

@@ -43,7 +43,7 @@ constexpr int KA_STEP = 16;          // tokens of a warp's step
 constexpr int KA_ROW = 4;            // steps that a row's beginning is worth
 constexpr int KA_JOIN = 512;         // threads of a joining block: 22.7 us for 64 x 1024 tokens, with 256 threads 24.2
 constexpr int KA_MAX_SEQS = 4096;    // the prefix sums of their steps stand in shared memory
-constexpr float KA_NONE = -1e30f;    // maximum of no token: finite, so that exp2(-inf - m) is 0
+constexpr float KA_NONE = -3.4028234663852886e38f;  // maximum of no token: no score is below it, and exp2(-inf - m) is 0
 
 // One block an SM, with as many warps as registers allow, and the steps in a warp's queue: about 190 KB of codes under way.
 __host__ __device__ constexpr int kv8_attn_warps(int D, int HT) { return D == 256 ? 8 : (D == 64 && HT == 8 ? 16 : 12); }
