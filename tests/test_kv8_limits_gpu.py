@@ -1,4 +1,6 @@
 """The 8-bit paged cache, its decode attention and filtered sampling at the limits of their numbers (B200)."""
+import math
+
 import pytest
 import torch
 
@@ -77,3 +79,32 @@ def test_attention_of_scores_far_below_zero(name, lens, Hq, Hk, D, page):
         v = (cache[1][pages].double() * cache[3][pages].double()[:, :, None, None]).transpose(0, 1).reshape(Hk, -1, D)[:, : lens[b]].cpu()
         want, mags = (x.repeat_interleave(Hq // Hk, 0) for x in (v.mean(1), v.abs().mean(1)))
         assert ((out[b].double() - want).abs() <= torch.finfo(torch.bfloat16).eps / 2 * want.abs() + 2.0**-10 * mags).all()
+
+
+@pytest.mark.parametrize("B, n, drop", [(1000, 8000, 20), (1000, 8000, 26), (900, 3000, 28), (3, 600, 24), (2, 600, 27)])
+def test_attention_keeps_many_small_weights_beside_a_large_one(B, n, drop):
+    """One token of value 0 has nearly all the weight, the others 2^-drop of it each: their sum is the output.  With many
+    sequences (of the same pages) a warp takes a whole row.
+
+    A weight is rounded to fp16 once, 2^-11 of it, and where it is below fp16's normal numbers by up to 2^-32 of the largest (the
+    largest stands at 2^7 or above, the smallest step of fp16 is 2^-24, its half 2^-25)."""
+    Hk, G, D, page = 2, 4, 128, 64
+    cache, table = filled_cache([n], Hk, page, D, "cuda", seed=5, extra=0)
+    cache[2].fill_(1.0)
+    cache[3].fill_(2.0**-3)
+    first, row = int(table[0, 0]), 7
+    u = cache[0].view(torch.uint8)
+    u.fill_(0)
+    u[first, :, row, 0] = torch.tensor([1.0]).to(torch.float8_e4m3fn).view(torch.uint8).item()
+    cache[1].view(torch.uint8).bitwise_and_(0x7F)  # values of one sign: no cancellation
+    cache[1].view(torch.uint8)[first, :, row] = 0  # the value of the heavy token
+    q = torch.zeros(B, Hk * G, D, device="cuda", dtype=torch.bfloat16)
+    q[..., 0] = 1.0
+    out = F.kv8_decode_attn(q, *cache, table.expand(B, -1).contiguous(), _i32([n - 1] * B), drop * math.log(2)).cpu().double()
+    v = (cache[1].double() * 2.0**-3)[table[0].long()].transpose(0, 1).reshape(Hk, -1, D)[:, :n].cpu()
+    den = 1 + (n - 1) * 2.0**-drop
+    want = (v.sum(1) * 2.0**-drop / den).repeat_interleave(G, 0)[None]
+    mags = (v.sum(1) / den).repeat_interleave(G, 0)[None]
+    tol = torch.finfo(q.dtype).eps / 2 * want + (2.0**-11 * 2.0**-drop + 2.0**-32 + 2.0**-18 * 2.0**-drop) * mags
+    assert ((out - want).abs() <= tol).all(), float(((out - want).abs() / tol).max())
+    assert (want > 8 * tol).all()  # what is lost would be seen

@@ -19,8 +19,9 @@
 // largest).
 //
 // Page scales.  k_scale multiplies the scores.  v_scale goes into the exponent: w_j = exp2(s_j + log2 v_scale - m) with m the
-// running maximum of that sum, so that weights stay within fp16 whatever the pages' scales, and the softmax's denominator is
-// sum w_j / v_scale.  m moves only when a weight would pass 2^8.
+// running maximum of that sum, less KA_BELOW, so that weights stay within fp16 whatever the pages' scales, and the softmax's
+// denominator is sum w_j / v_scale.  m moves only when a weight would pass 2^15; then the largest is 2^KA_BELOW.  A weight is rounded
+// once, to fp16: by 2^-11 of it, or below fp16's normal numbers by 2^-32 of the largest.
 //
 // Work: the steps of all rows (sequence, key head, head tile) are one list that is dealt to the warps in equal runs, so any mix
 // of lengths fills the GPU; a row counts KA_ROW steps more than it has, the cost of beginning one.  A warp that has all steps of
@@ -44,6 +45,7 @@ constexpr int KA_ROW = 4;            // steps that a row's beginning is worth
 constexpr int KA_JOIN = 512;         // threads of a joining block: 22.7 us for 64 x 1024 tokens, with 256 threads 24.2
 constexpr int KA_MAX_SEQS = 4096;    // the prefix sums of their steps stand in shared memory
 constexpr float KA_NONE = -3.4028234663852886e38f;  // maximum of no token: no score is below it, and exp2(-inf - m) is 0
+constexpr float KA_BELOW = 7.f;      // a weight is at most 2^15 before m moves, and the largest 2^7 when it has
 
 // One block an SM, with as many warps as registers allow, and the steps in a warp's queue: about 190 KB of codes under way.
 __host__ __device__ constexpr int kv8_attn_warps(int D, int HT) { return D == 256 ? 8 : (D == 64 && HT == 8 ? 16 : 12); }
@@ -460,9 +462,9 @@ kv8_attn_kernel(const __grid_constant__ Kv8AttnArgs a) {
             if (hidden(r)) x[r] = -INFINITY;
         }
         const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-        if (__any_sync(0xffffffffu, top > m[n] + 8.f)) {
+        if (__any_sync(0xffffffffu, top > m[n] + 15.f)) {
           float mx = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          mx = fmaxf(m[n], fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)));
+          mx = fmaxf(m[n], fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) - KA_BELOW);
           const float down = fast_exp2(m[n] - mx);
           m[n] = mx;
           l[n] *= down;
