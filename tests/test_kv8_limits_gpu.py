@@ -108,3 +108,27 @@ def test_attention_keeps_many_small_weights_beside_a_large_one(B, n, drop):
     tol = torch.finfo(q.dtype).eps / 2 * want + (2.0**-11 * 2.0**-drop + 2.0**-32 + 2.0**-18 * 2.0**-drop) * mags
     assert ((out - want).abs() <= tol).all(), float(((out - want).abs() / tol).max())
     assert (want > 8 * tol).all()  # what is lost would be seen
+
+
+# ---- RoPE and append -----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("f32", [False, True])
+def test_rope_append_reports_slots_that_the_table_does_not_have(f32):
+    """They are treated as idle: their sums are cleared, nothing is written for them, the other rows are as ever."""
+    from trl_b200.ops import cuda as K
+
+    K.check_status()
+    D, Hq, Hk, page = 64, 2, 1, 16
+    cache, table = filled_cache([40] * 3, Hk, page, D, "cuda", seed=6)
+    x = torch.randn(4, (Hq + 2 * Hk) * D, generator=torch.Generator().manual_seed(3)).bfloat16().cuda()
+    seq, delta = _i32([17, 5, 20]), _i32([0, 3, 0])
+    got, want = ([t.clone() for t in cache] for _ in range(2))
+    q, ref = (torch.full((4, Hq, D), 9.0, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    src = x.float() if f32 else x
+    K.kv8_rope_append(src, None, None, None, 1e-6, seq, _i32([3, 1, -1, 2**31 - 1]), table, q, *got, Hq, 1e4, pos_delta=delta)
+    with pytest.raises(RuntimeError, match="code=3"):
+        K.check_status()
+    K.kv8_rope_append(x[1:2], None, None, None, 1e-6, seq, _i32([1]), table, ref[1:2], *want, Hq, 1e4, pos_delta=delta)
+    K.check_status()
+    assert torch.equal(q, ref) and (not f32 or bool((src == 0).all()))
+    for a, b in zip(got, want):
+        assert torch.equal(*(t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t for t in (a, b)))

@@ -317,7 +317,9 @@ kv8_rope_append_kernel(void* __restrict__ qkv, long long row_stride, const __nv_
   if (item >= B * heads) return;
   const int b = item / heads, head = item % heads;
   const int slot = slot_ids ? slot_ids[b] : b;
-  const int pos = seq_lens[slot];
+  const bool known = slot >= 0 && slot < table_rows;  // a slot that the table does not have: reported, and treated as idle
+  if (!known && lane == 0) report_error(status, ERR_BOUNDS, SITE_KV8_ROPE, slot);
+  const int pos = known ? seq_lens[slot] : -1;
   const size_t base = (size_t)b * row_stride + (size_t)head * D;
   float lo[2], hi[2], ss = 0.f;
   auto bf = [](float x) { return __bfloat162float(__float2bfloat16(x)); };
@@ -475,6 +477,7 @@ TRLB_API int trlb_kv8_append(const Kv8AppendCall* call) {
 }
 
 // qkv: bf16 rows (f32 == 0) or fp32 sums that are cleared.  bias / norms / pos_delta / slot_ids may be null.  dim <= 128.
+// seq_lens and pos_delta have an entry for each slot that is used, with slot_ids for each row of the table.
 TRLB_API int trlb_kv8_rope_append(void* qkv, int f32, long long row_stride, const void* bias, const void* q_norm,
                                   const void* k_norm, float norm_eps, const int* seq_lens, const int* slot_ids,
                                   const int* table, int table_rows, int max_blocks, void* q_out, void* k_codes, void* v_codes,

@@ -1228,12 +1228,17 @@ def kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, starts, *,
 
 def kv8_rope_append(qkv, bias, q_norm, k_norm, norm_eps, seq_lens, slot_ids, block_table, q_out, k_cache, v_cache, k_scale,
                     v_scale, Hq, theta, pos_delta=None):
-    """:func:`rope_kv_write` (``qkv`` bf16) or :func:`rope_kv_write_f32` (``qkv`` fp32 sums, cleared) into an 8-bit cache."""
+    """:func:`rope_kv_write` (``qkv`` bf16) or :func:`rope_kv_write_f32` (``qkv`` fp32 sums, cleared) into an 8-bit cache.  ``bias``
+    and the norms' weights are bf16.  Slots that the block table does not have are reported by ``check_status`` and left out."""
     pages, heads, page, dim, index = _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table)
     B = qkv.shape[0]
     f32 = qkv.dtype == torch.float32
-    if dim > 128 or (not f32 and qkv.dtype != torch.bfloat16) or qkv.stride(1) != 1 or qkv.shape[1] != (Hq + 2 * heads) * dim:
+    if (dim > 128 or (not f32 and qkv.dtype != torch.bfloat16) or qkv.dim() != 2 or qkv.stride(1) != 1
+            or qkv.shape[1] != (Hq + 2 * heads) * dim):
         raise ValueError("qkv has to be dense rows of bf16 or fp32 for heads of at most 128 values")
+    for name, x, n in (("bias", bias, qkv.shape[1]), ("q_norm", q_norm, dim), ("k_norm", k_norm, dim)):
+        if x is not None and (x.dtype != torch.bfloat16 or x.shape != (n,) or not x.is_contiguous()):
+            raise ValueError(f"{name} has to be a contiguous bf16 tensor [{n}]")
     if not f32 and bias is not None:
         raise ValueError("a bias belongs to fp32 sums: a bf16 row has it already")
     _want_i32(seq_lens, "seq_lens")
@@ -1242,8 +1247,12 @@ def kv8_rope_append(qkv, bias, q_norm, k_norm, norm_eps, seq_lens, slot_ids, blo
     for name, x in (("slot_ids", slot_ids), ("pos_delta", pos_delta)):
         if x is not None:
             _want_i32(x, name)
-    if min(seq_lens.shape[0], block_table.shape[0]) < (B if slot_ids is None else 1) or (slot_ids is not None and slot_ids.shape != (B,)):
+    rows = block_table.shape[0]
+    if (slot_ids is None and B > rows) or (slot_ids is not None and slot_ids.shape != (B,)):
         raise ValueError(f"{B} rows need as many lengths, rows of the block table and slots")
+    for name, x in (("seq_lens", seq_lens), ("pos_delta", pos_delta)):
+        if x is not None and x.numel() < (B if slot_ids is None else rows):
+            raise ValueError(f"{name} needs an entry for each of " + (f"{B} rows" if slot_ids is None else f"the block table's {rows} rows"))
     _same_device(index, qkv=qkv, bias=bias, q_norm=q_norm, k_norm=k_norm, seq_lens=seq_lens, slot_ids=slot_ids, q_out=q_out, pos_delta=pos_delta)
     _launch(index, _fn("trlb_kv8_rope_append", "pilpppfpppiipppppiiiiiifppp"), "kv8_rope_append", qkv.data_ptr(), int(f32),
             qkv.stride(0), _ptr(bias), _ptr(q_norm), _ptr(k_norm), norm_eps, seq_lens.data_ptr(), _ptr(slot_ids),
