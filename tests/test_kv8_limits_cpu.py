@@ -21,3 +21,14 @@ def test_rope_append_refuses_what_it_would_read_wrongly(change, message):
     with pytest.raises(ValueError, match=message):
         K.kv8_rope_append(a["qkv"], a["bias"], a["q_norm"], a["k_norm"], 1e-6, a["lens"], a["slots"], a["table"],
                           torch.zeros(3, 4, 64, dtype=torch.bfloat16), *F.kv8_alloc(4, 2, 16, 64), 4, 1e4, pos_delta=a["delta"])
+
+
+def test_attention_refuses_more_steps_than_it_can_count():
+    """4096 sequences with room for 8.4 million tokens each have 2^31 steps of 16."""
+    from trl_b200.ops import cuda as K
+
+    B = 4096
+    table = torch.empty(B, 65536, dtype=torch.int32)
+    with pytest.raises(ValueError, match="2\\^31 steps"):
+        K.kv8_decode_attn(torch.zeros(B, 1, 64, dtype=torch.bfloat16), *F.kv8_alloc(2, 1, 128, 64), table,
+                          torch.full((B,), -1, dtype=torch.int32), 1.0)

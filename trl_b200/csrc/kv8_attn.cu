@@ -678,10 +678,13 @@ kv8_attn_join_kernel(const __grid_constant__ Kv8AttnArgs a) {
   for (int e = 0; e < E; ++e) store1(out + lane + 32 * e, o[e] * inv);
 }
 
-// Whether each row gets a block: a rule on what the host knows, the room in the block table and the window.
+// The most steps that a sequence can have, by the room in its row of the block table and the window.
+inline long long kv8_room_steps(long long tokens, long long window) {
+  return (window > 0 && window + KA_STEP < tokens ? window + KA_STEP : tokens) / KA_STEP + 1;
+}
+// Whether each row gets a block: a rule on what the host knows.
 inline bool kv8_by_row(int D, int ht, long long rows, long long tokens, long long window) {
-  const long long steps = (window > 0 && window + KA_STEP < tokens ? window + KA_STEP : tokens) / KA_STEP + 1;
-  return rows <= trlb_host::sm_count() && steps <= (long long)kv8_attn_alone(D) * kv8_attn_warps(D, ht);
+  return rows <= trlb_host::sm_count() && kv8_room_steps(tokens, window) <= (long long)kv8_attn_alone(D) * kv8_attn_warps(D, ht);
 }
 inline int kv8_head_tile(int D, int G) { return G <= 8 || D > 128 ? 8 : 16; }
 
@@ -729,9 +732,10 @@ int kv8_attn_pick(Kv8AttnArgs& a, const void* k, const void* v, int D, cudaStrea
 using namespace trlb;
 
 // fp32 words of scratch that a call needs: parts of rows that several blocks share.  `tokens`: what a row of the block table has
-// room for.
+// room for.  -1: so many steps that the list's 32-bit prefix sums might not hold them.
 TRLB_API long long trlb_kv8_attn_scratch(int B, int Hq, int Hk, int D, long long tokens, int window) {
   const int ht = kv8_head_tile(D, Hq / Hk);
+  if (kv8_room_steps(tokens, window) + KA_ROW > 2147483647ll / B) return -1;
   if (kv8_by_row(D, ht, (long long)B * Hk * ((Hq / Hk + ht - 1) / ht), tokens, window)) return 0;
   return (2ll * ht * (D + 2) + sizeof(SharedRow) / 4) * kv8_attn_warps(D, ht) * trlb_host::sm_count();
 }
@@ -761,6 +765,7 @@ TRLB_API int trlb_kv8_decode_attn(const Kv8AttnCall* call) {
   Kv8AttnArgs a{{}, {}, c.q, c.q_row, c.q_head, c.k_scale, c.v_scale, c.table, c.seq_lens, c.slots, c.out, c.part, nullptr,
                 nullptr, c.status, c.pages, c.Hk, c.Hq / c.Hk, 1, shift, c.table_rows, c.max_blocks, c.B, c.window, 0, c.scale};
   const long long words = trlb_kv8_attn_scratch(c.B, c.Hq, c.Hk, c.D, (long long)c.max_blocks << shift, c.window);
+  if (words < 0) return -8;
   if (c.part_words < words) return -7;
   a.by_row = words == 0;
   if (c.dtype == 0) return kv8_attn_pick<__nv_bfloat16>(a, c.k_codes, c.v_codes, c.D, c.stream);

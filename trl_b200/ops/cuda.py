@@ -1302,6 +1302,9 @@ def kv8_decode_attn(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens
     sizes = (B, Hq, heads, dim, blocks * page, window, index)
     words = _kv8_scratch.get(sizes)
     if words is None:
+        room = blocks * page
+        if B * ((min(room, window + 16) if window else room) // 16 + 5) >= 2**31:  # the kernel counts steps in 32 bits
+            raise ValueError(f"{B} sequences with room for {room} tokens each: a call has less than 2^31 steps of 16 tokens")
         if len(_kv8_scratch) > 10000:
             _kv8_scratch.clear()
         with torch.cuda.device(index):
