@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from kv8_util import attention64, filled_cache
+from kv8_util import attention64, check_sample, filled_cache
 from trl_b200.ops import functional as F
 
 pytestmark = pytest.mark.gpu
@@ -132,3 +132,22 @@ def test_rope_append_reports_slots_that_the_table_does_not_have(f32):
     assert torch.equal(q, ref) and (not f32 or bool((src == 0).all()))
     for a, b in zip(got, want):
         assert torch.equal(*(t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t for t in (a, b)))
+
+
+# ---- sampling ------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows", [6, 700])
+def test_sampling_of_infinite_logits(dtype, rows):
+    """+inf stands for fp32's largest number, beside the largest of a narrower type too, however many rows there are."""
+    vocab = 1500
+    g = torch.Generator().manual_seed(rows)
+    top = torch.finfo(dtype).max
+    z = (torch.randn(rows, vocab, generator=g) * 2).to(dtype)
+    z[0::6, 7], z[0::6, 3] = math.inf, top
+    z[1::6, 3], z[1::6, 4] = top, torch.nextafter(torch.tensor(top, dtype=dtype), torch.tensor(0.0, dtype=dtype))
+    z[2::6, 100], z[2::6, 90], z[2::6, 110] = math.inf, math.inf, top
+    z[3::6, 11], z[3::6, 12] = math.nan, top
+    rng = torch.randint(-2**31, 2**31 - 1, (rows,), generator=g).to(torch.int32)
+    for kw in ({}, {"top_k": 3}, {"top_p": 0.9}, {"top_k": 600, "top_p": 0.7}, {"temperature": 0.0}, {"min_p": 0.2, "temperature": 0.5}, {"temperature": 3.0}):
+        tok, logp = F.sample_filtered(z.cuda(), rng.cuda(), **kw)
+        check_sample(z, rng, tok, logp, **kw)

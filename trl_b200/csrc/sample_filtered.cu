@@ -127,32 +127,30 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 sf_lowest<__nv_bfloat16>() { return __ushort_as_bfloat16((unsigned short)0xff80); }
 template <>
 __device__ __forceinline__ __half sf_lowest<__half>() { return __ushort_as_half((unsigned short)0xfc00); }
-// NaN -> -inf (a maximum drops it), nothing above cap, one zero of both.
+// NaN -> -inf (a maximum drops it), nothing above cap, one zero of both.  (Held logits have no cap: see fast().)
 __device__ __forceinline__ float sf_clean1(float y, float cap) { return fminf(fmaxf(y, -INFINITY), cap) + 0.f; }
 template <typename T>
-__device__ __forceinline__ void sf_clean(uint4& u, float cap);
+__device__ __forceinline__ void sf_clean(uint4& u);
 template <>
-__device__ __forceinline__ void sf_clean<float>(uint4& u, float cap) {
-  u.x = __float_as_uint(sf_clean1(__uint_as_float(u.x), cap));
-  u.y = __float_as_uint(sf_clean1(__uint_as_float(u.y), cap));
-  u.z = __float_as_uint(sf_clean1(__uint_as_float(u.z), cap));
-  u.w = __float_as_uint(sf_clean1(__uint_as_float(u.w), cap));
+__device__ __forceinline__ void sf_clean<float>(uint4& u) {
+  u.x = __float_as_uint(sf_clean1(__uint_as_float(u.x), INFINITY));
+  u.y = __float_as_uint(sf_clean1(__uint_as_float(u.y), INFINITY));
+  u.z = __float_as_uint(sf_clean1(__uint_as_float(u.z), INFINITY));
+  u.w = __float_as_uint(sf_clean1(__uint_as_float(u.w), INFINITY));
 }
 template <>
-__device__ __forceinline__ void sf_clean<__nv_bfloat16>(uint4& u, float cap) {
-  const __nv_bfloat162 lo = __bfloat162bfloat162(sf_lowest<__nv_bfloat16>()), hi = __bfloat162bfloat162(__float2bfloat16_rz(cap)),
-                       zero = __bfloat162bfloat162(__float2bfloat16(0.f));
+__device__ __forceinline__ void sf_clean<__nv_bfloat16>(uint4& u) {
+  const __nv_bfloat162 lo = __bfloat162bfloat162(sf_lowest<__nv_bfloat16>()), zero = __bfloat162bfloat162(__float2bfloat16(0.f));
   __nv_bfloat162* p = reinterpret_cast<__nv_bfloat162*>(&u);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) p[i] = __hadd2(__hmin2(__hmax2(p[i], lo), hi), zero);
+  for (int i = 0; i < 4; ++i) p[i] = __hadd2(__hmax2(p[i], lo), zero);
 }
 template <>
-__device__ __forceinline__ void sf_clean<__half>(uint4& u, float cap) {
-  const __half2 lo = __half2half2(sf_lowest<__half>()), hi = __half2half2(__float2half_rz(fminf(cap, 65504.f))),
-                zero = __half2half2(__float2half(0.f));
+__device__ __forceinline__ void sf_clean<__half>(uint4& u) {
+  const __half2 lo = __half2half2(sf_lowest<__half>()), zero = __half2half2(__float2half(0.f));
   __half2* p = reinterpret_cast<__half2*>(&u);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) p[i] = __hadd2(__hmin2(__hmax2(p[i], lo), hi), zero);
+  for (int i = 0; i < 4; ++i) p[i] = __hadd2(__hmax2(p[i], lo), zero);
 }
 
 struct SfShared {
@@ -1153,12 +1151,14 @@ struct SfSampler {
           }
           u = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        sf_clean<T>(u, q.cap);
+        sf_clean<T>(u);
         float y[N];
         sf_unpack<T>(u, y);
         take(y);
         data[v] = u;
       }
+      // what has no finite quotient (of a narrow type: infinities, beside its largest numbers) spoils the row here, too
+      if (mine > q.cap) mine = INFINITY;
     }
     auto each_until = [&](auto f, auto stop) {
       if constexpr (HELD) {
@@ -1216,7 +1216,7 @@ struct SfSampler {
       if (tid == 0) { sh.fmax = bmax; sh.from = from; }
       cluster.sync();
       xmax = max_of([](const SfShared& o) { return o.fmax; });
-      if (!HELD && xmax == INFINITY) return false;
+      if (xmax == INFINITY) return false;
       from = -max_of([](const SfShared& o) { return -o.from; });
       each([&](float x, int col) {
         if (x >= from) append(sh, x, col);
@@ -1236,7 +1236,7 @@ struct SfSampler {
       if (tid == 0) { sh.fmax = bmax; sh.sums[0] = sum; }
       cluster.sync();
       xmax = max_of([](const SfShared& o) { return o.fmax; });
-      if (xmax == -INFINITY || (!HELD && xmax == INFINITY)) return false;
+      if (xmax == -INFINITY || xmax == INFINITY) return false;
       zmax = quotient(xmax);
       total = sum_of([&](const SfShared& o) { return o.fmax > -INFINITY ? o.sums[0] * (double)exp2f((o.fmax - xmax) * c) : 0.; });
     }
