@@ -135,7 +135,54 @@ def test_rope_append_reports_slots_that_the_table_does_not_have(f32):
 
 
 # ---- sampling ------------------------------------------------------------------------------------------------------
-@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def _neighbours(rows, vocab, seed, levels=8):
+    """fp32 logits on a few levels, each up to three steps of fp32 above its level: many quotients by a temperature are equal
+    where the logits are not."""
+    g = torch.Generator().manual_seed(seed)
+    base = (torch.randint(0, levels, (rows, vocab), generator=g) * 0.37 + 1.03 + torch.rand(rows, 1, generator=g))
+    z = (base.view(torch.int32) + torch.randint(0, 4, (rows, vocab), generator=g).to(torch.int32)).view(torch.float32)
+    rng = torch.randint(-2**31, 2**31 - 1, (rows,), generator=g).to(torch.int32)
+    return z, rng
+
+
+# rows in the shared memory of a cluster; more rows than are held; rows longer than shared memory
+@pytest.mark.parametrize("rows, vocab", [(40, 3001), (330, 4099), (6, 40000), (2, 200003)])
+@pytest.mark.parametrize("kw", [{"temperature": 0.0}, {"temperature": 0.0, "top_p": 0.9}, {"temperature": 0.0, "top_k": 7, "min_p": 0.3},
+                                {"temperature": 0.7, "top_k": 20}, {"temperature": 0.7, "top_k": 300, "top_p": 0.8}, {"temperature": 0.3, "top_k": 1000},
+                                {"temperature": 0.7, "top_p": 0.3}, {"temperature": 1.3, "top_p": 0.9}, {"temperature": 0.05, "top_p": 0.7},
+                                {"temperature": 0.7, "min_p": 1.0}, {"temperature": 0.9, "min_p": 0.4, "top_p": 0.6}])
+def test_sampling_compares_quotients(rows, vocab, kw):
+    """Logits whose quotients by the temperature are equal are equals, whichever of them is larger."""
+    z, rng = _neighbours(rows, vocab, rows + vocab)
+    tok, logp = F.sample_filtered(z.cuda(), rng.cuda(), **kw)
+    check_sample(z, rng, tok, logp, **kw)
+
+
+def test_sampling_compares_quotients_by_temperatures_of_rows():
+    rows, vocab = 300, 700
+    z, rng = _neighbours(rows, vocab, 1, levels=3)
+    g = torch.Generator().manual_seed(2)
+    kw = {"temperature": torch.where(torch.rand(rows, generator=g) < 0.3, 0.0, 0.1 + 2 * torch.rand(rows, generator=g)),
+          "top_k": torch.randint(0, 400, (rows,), generator=g).to(torch.int32), "top_p": 0.2 + torch.rand(rows, generator=g)}
+    tok, logp = F.sample_filtered(z.cuda(), rng.cuda(), **{k: v.cuda() for k, v in kw.items()})
+    check_sample(z, rng, tok, logp, **kw)
+
+
+@pytest.mark.parametrize("kw", [{}, {"top_k": 2}, {"top_p": 0.9}, {"min_p": 0.1}, {"temperature": 0.0}])
+def test_sampling_of_quotients_that_are_not_finite(kw):
+    """Finite logits whose quotients are infinite, and temperatures without bound."""
+    z = torch.full((6, 1000), -3.0e38)
+    z[1, 5], z[2, 9], z[2, 700] = -1.0e37, 3.0e38, 3.2e38
+    z[3] = torch.linspace(-1e-38, 1e-38, 1000)
+    z[4, 17], z[5, :] = 4.0, torch.linspace(-30, 30, 1000)
+    rng = torch.arange(6, dtype=torch.int32)
+    for t in (0.5, 0.25, 4e4, 1e20, math.inf):
+        par = {"temperature": t, **kw}
+        tok, logp = F.sample_filtered(z.cuda(), rng.cuda(), **par)
+        check_sample(z, rng, tok, logp, **par)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("rows", [6, 700])
 def test_sampling_of_infinite_logits(dtype, rows):
     """+inf stands for fp32's largest number, beside the largest of a narrower type too, however many rows there are."""

@@ -1,17 +1,18 @@
 // Sampling with temperature, top-k, top-p and min-p from one random word per row.
 //
-//   z = logit / max(temperature, 1e-6); NaN counts as -inf, +inf as the largest finite value
-//   top-k keeps what is at least the k-th largest logit (equals of the k-th too); 0 keeps all
+//   z = logit / max(temperature, 1e-6) in fp32; NaN counts as -inf, what is above fp32's largest number as that number
+//   top-k keeps what is at least the k-th largest z (equals of the k-th too); 0 keeps all
 //   top-p keeps, most likely first and the lower column first among equals, each token before which at most
 //         top_p of the mass of what top-k kept stands
 //   min-p keeps z >= max z + log(min_p)
 //   token = argmax over what is kept of z - log(-log u), u = (hash(word of the row, column) + 1/2) / 2^32; of z where
 //   temperature is 0; its log-probability is that in the distribution over what is kept
 //
-// All filters are one border: the last token kept, in the order "larger logit, then lower column".  A row is read by the blocks
+// All filters are one border: the last token kept, in the order "larger z, then lower column".  A row is read by the blocks
 // of a cluster.  What bounds it is the work per logit (the row's bytes stay in the second-level cache after the first pass) and
-// the latency of the few exchanges between the blocks; so logits are compared undivided, and the border is found in as few
-// passes as the row allows:
+// the latency of the few exchanges between the blocks; so logits are divided only where z decides, and the border is found in as
+// few passes as the row allows.  Logits of 16 bits have the order of their z.  Neighbouring fp32 logits can have one z, whichever
+// way round they stand: their lists hold z, and the numbers that they are compared with are the smallest logits of a z (least_of).
 //   1. the maximum and the mass, each thread with a running maximum of its own;
 //   2. candidates for the kept tokens: with top-k of C blocks what is not below the k/C-th largest of the threads' maxima of any
 //      (k logits are at least that large), with top-p alone what is not lighter than (1 - top_p) mass / V (lighter ones together
@@ -20,8 +21,9 @@
 //      both sides, which brackets the border; the tokens of the bracket are listed, and the exact mass above it says which of
 //      them is the last.  A bracket with too many tokens for the list is cut again by histograms over the logits' bits.
 //   4. a last pass over the row draws among what is kept.
-// A row that fits into the shared memory of a cluster is read once and stays there for all of it (SfSampler::fast); the few rows
-// that need what fast() leaves out, and larger ones, are read again for each pass (SfSampler::run).
+// A row that fits into the shared memory of a cluster is read once and stays there for all of it, larger ones are read again for
+// each pass (SfSampler::fast); the few rows that need what fast() leaves out are read again and, where their order is not that of
+// z, divided in each pass (SfSampler::run).
 // Measured: one row of 152064 bf16 logits with top-k 20 and top-p 0.8 13.3 us; 64 rows with top-p 0.95 71 us (32 rows 48 us), of which the
 // flattest row's 61 us are: load and mass 8, list given up 4, histogram 8, its border's bins 8, draw 20, list of the bracket 5,
 // border 5, last draw 3; 256 rows of 128256 fp32 logits with parameters of all kinds 114 us.
@@ -44,6 +46,9 @@ constexpr int SF_CUT = 1024;       // and the cut around the border; more are so
 constexpr int SF_FEW = 64;          // of so few tokens each is compared with all others
 constexpr int SF_HELD = 5120;      // 16-byte vectors of a row in a block's shared memory, at most: with it two blocks an SM
 constexpr float SF_FINE = 1024.f;  // parts of a bin in which the histogram adds up where in the bin its tokens lie
+// Temperatures from here on: below, few tokens have a weight, and rounding z shows in it.  Up to SF_HIGH z is no denormal number where
+// that would make one z of two 16-bit logits.
+constexpr float SF_LOW = 0.015625f, SF_HIGH = 32768.f;
 constexpr int SF_BATCH = 16;       // logits that a thread loads at once
 constexpr float SF_MAX = 3.4028234663852886e38f;
 constexpr float SF_LOG2E = 1.4426950408889634f;
@@ -127,7 +132,7 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 sf_lowest<__nv_bfloat16>() { return __ushort_as_bfloat16((unsigned short)0xff80); }
 template <>
 __device__ __forceinline__ __half sf_lowest<__half>() { return __ushort_as_half((unsigned short)0xfc00); }
-// NaN -> -inf (a maximum drops it), nothing above cap, one zero of both.  (Held logits have no cap: see fast().)
+// NaN -> -inf (a maximum drops it), nothing above cap, one zero of both.
 __device__ __forceinline__ float sf_clean1(float y, float cap) { return fminf(fmaxf(y, -INFINITY), cap) + 0.f; }
 template <typename T>
 __device__ __forceinline__ void sf_clean(uint4& u);
@@ -151,6 +156,12 @@ __device__ __forceinline__ void sf_clean<__half>(uint4& u) {
   __half2* p = reinterpret_cast<__half2*>(&u);
 #pragma unroll
   for (int i = 0; i < 4; ++i) p[i] = __hadd2(__hmax2(p[i], lo), zero);
+}
+
+// Four of them over t.
+__device__ __noinline__ float4 sf_over(float4 y, float t) {
+  return make_float4(sf_clean1(__fdiv_rn(y.x, t), SF_MAX), sf_clean1(__fdiv_rn(y.y, t), SF_MAX), sf_clean1(__fdiv_rn(y.z, t), SF_MAX),
+                     sf_clean1(__fdiv_rn(y.w, t), SF_MAX));
 }
 
 struct SfShared {
@@ -188,9 +199,11 @@ struct SfRow {
   const T* x;
   int v0, v1;
   bool vec;
-  float cap;  // logits from here on are equals: their quotients by the temperature are not finite
-  __device__ __forceinline__ float clean(float y) const { return sf_clean1(y, cap); }
-  // f(logit, column) over the block's columns, until stop() says so; RAW: logits as they are
+  float cap;  // the quotients of larger logits are not finite
+  float t;    // what logits are divided by: the temperature, or 1 where they stay as they are
+  float top;  // and what none is above then
+  __device__ __forceinline__ float clean(float y) const { return sf_clean1(t == 1.f ? y : __fdiv_rn(y, t), top); }
+  // f(logit over t, column) over the block's columns, until stop() says so; RAW: logits as they are
   template <bool RAW = false, typename F, typename G>
   __device__ __forceinline__ void each(F f, G stop) const {
     constexpr int N = 16 / sizeof(T);
@@ -210,8 +223,23 @@ struct SfRow {
           if (at + j * SF_THREADS >= n1) break;
           float y[N];
           sf_unpack<T>(u[j], y);
+          if (!RAW) {
 #pragma unroll
-          for (int k = 0; k < N; ++k) f(RAW ? y[k] : clean(y[k]), (at + j * SF_THREADS) * N + k);
+            for (int k = 0; k < N; k += 4) {
+              if (t == 1.f) {
+#pragma unroll
+                for (int e = k; e < k + 4; ++e) y[e] = sf_clean1(y[e], top);
+              } else {
+                const float4 z = sf_over(make_float4(y[k], y[k + 1], y[k + 2], y[k + 3]), t);
+                y[k] = z.x;
+                y[k + 1] = z.y;
+                y[k + 2] = z.z;
+                y[k + 3] = z.w;
+              }
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < N; ++k) f(y[k], (at + j * SF_THREADS) * N + k);
         }
       }
       i = n1 * N + threadIdx.x;
@@ -417,11 +445,14 @@ struct SfSampler {
   const SampleArgs& a;
   SfRow<T> r;
   int C, rank, row, tid;
-  float temperature, c;   // c: of a logit's distance to the maximum, the exponent of 2
+  // The temperature of what is compared (logits, or with `divided` z, in lists and in run()): 1 once that is z.
+  // c: of a distance to the maximum, the exponent of 2.
+  float temperature, c;
   float xmax, zmax;
   float step;             // bins of the linear histogram per unit of the logits
   uint32_t word;
   bool greedy, as_sampler;  // the latter: random numbers as trlb_sample makes them
+  bool divided;             // the order of the logits is not that of z
   SfShared* lead;
 
   __device__ __forceinline__ SfShared* of(int c) { return cluster.map_shared_rank(&s, c); }
@@ -437,6 +468,41 @@ struct SfSampler {
   __device__ __forceinline__ float weight(float x) const { return exp2f((x - xmax) * c); }
   __device__ __forceinline__ float noise(uint32_t h) const { return as_sampler ? sf_gumbel_as_sampler(h) : sf_gumbel(h); }
   __device__ __forceinline__ float quotient(float x) const { return sf_quotient(x, temperature); }
+  // Whether the row's logits are divided as they are read.
+  __device__ __forceinline__ void read_divided(bool yes) {
+    divided = yes;
+    r.t = yes ? temperature : 1.f;
+    r.top = yes ? SF_MAX : INFINITY;
+  }
+  // From here on what is compared is z.
+  __device__ __forceinline__ void to_z() {
+    temperature = 1.f;
+    c = SF_LOG2E;
+    xmax = zmax;
+  }
+  // The smallest logit whose quotient is at least z.
+  __device__ __noinline__ float least_of(float z) const {
+    if (temperature == 1.f) return z;
+    if (!(z >= -SF_MAX)) return -SF_MAX;
+    float x = fminf(fmaxf((float)((double)z * (double)temperature), -SF_MAX), SF_MAX);
+    for (int i = 0; i < 4 && quotient(x) < z; ++i) x = nextafterf(x, INFINITY);
+    for (int i = 0; i < 4 && quotient(nextafterf(x, -INFINITY)) >= z; ++i) x = nextafterf(x, -INFINITY);
+    if (quotient(x) >= z && quotient(nextafterf(x, -INFINITY)) < z) return x;
+    uint32_t lo = sf_key(-INFINITY), hi = sf_key(INFINITY);  // among the denormal numbers many logits have one quotient
+    while (hi - lo > 1) {
+      const uint32_t mid = lo + (hi - lo) / 2;
+      if (quotient(sf_unkey(mid)) >= z) hi = mid;
+      else lo = mid;
+    }
+    return sf_unkey(hi);
+  }
+  // x moved down, and up, to a logit at which a z begins.
+  __device__ __forceinline__ float class_from(float x) const { return sizeof(T) == 2 ? x : least_of(quotient(x)); }
+  __device__ __forceinline__ float class_above(float x) const {
+    if (sizeof(T) == 2) return x;
+    const float z = quotient(x), from = least_of(z);
+    return from >= x ? from : least_of(nextafterf(z, INFINITY));
+  }
   // Bins that reach down to `from`, where that is not too far.
   __device__ __forceinline__ void set_step(float from) {
     const float far = (xmax - from) / temperature;
@@ -1062,11 +1128,11 @@ struct SfSampler {
       const int at = (int)(unsigned)e;
       if (!within(x, at, border, border_col)) continue;
       const float z = quotient(x);
-      sf_better(best, col, best_z, greedy ? x : z + noise(sf_bits(word, (uint32_t)at)), at, z);
+      sf_better(best, col, best_z, z + noise(sf_bits(word, (uint32_t)at)), at, z);
     }
     if (tid < C) sf_better(best, col, best_z, s.bests[tid], s.best_cols[tid], s.best_zs[tid]);
     sf_block_best(best, col, best_z, s);
-    if (!greedy && (double)best < (double)zmax + (double)logf((float)mass) - 2.999) {  // once in 10^8 rows: without the shortcut of the draws
+    if ((double)best < (double)zmax + (double)logf((float)mass) - 2.999) {  // once in 10^8 rows: without the shortcut of the draws
       SfRow<T> q = r;
       q.v0 = 0;
       q.v1 = a.V;
@@ -1101,7 +1167,10 @@ struct SfSampler {
     const float top_p = a.top_p ? a.top_p[row] : a.top_p_all, min_p = a.min_p ? a.min_p[row] : a.min_p_all;
     const int top_k = a.top_k ? a.top_k[row] : a.top_k_all;
     const bool by_k = top_k > 0 && top_k < a.V, by_p = top_p < 1.f;
-    if (by_k && top_k > min(SF_LIST / 4, C * SF_THREADS / 2)) return false;  // too many for the lists
+    if (!(temperature <= SF_HIGH)) return false;
+    // Sums over many tokens are of the weights of undivided logits.  At low temperatures only those of the tokens that have any.
+    const bool low = temperature < SF_LOW;
+    if (by_k && !low && top_k > min(SF_LIST / 4, C * SF_THREADS / 2)) return false;  // too many for the lists
     const int first = r.v0;
     // A thread's maximum and, where it counts, the mass relative to it.
     float mine = -INFINITY, part = 0.f;
@@ -1111,7 +1180,7 @@ struct SfSampler {
       float top = y[0];
 #pragma unroll
       for (int k = 1; k < M; ++k) top = fmaxf(top, y[k]);
-      if (by_k) {
+      if (by_k || low) {
         mine = fmaxf(mine, top);
         return;
       }
@@ -1200,13 +1269,13 @@ struct SfSampler {
     float bmax = lane < SF_WARPS ? (float)sh.red[0][lane] : -INFINITY, bmin = lane < SF_WARPS ? (float)sh.red[1][lane] : INFINITY;
     bmax = warp_max(bmax);
     bmin = -warp_max(-bmin);
-    if (by_k) {
+    if (by_k || low) {
       // A k-th part of the blocks' number: as many threads of each block have a maximum of at least `from`, so that k logits of
       // the row are at least the smallest of the blocks' numbers.
       const unsigned share = (unsigned)((top_k + C - 1) / C);
       float from = -SF_MAX;  // all, where fewer threads have any
       const float scale = (float)(SF_BINS - 2) / (bmax - bmin);
-      if (scale < 1e30f) {  // false also where the block has none or all maxima are equal
+      if (scale < 1e30f && !low) {  // false also where the block has none or all maxima are equal
         if (mine > -INFINITY) atomicAdd(&sh.hist[(int)fminf((bmax - mine) * scale, (float)(SF_BINS - 1))], 1u);
         unsigned h[SF_EACH];
         own_bins(h);
@@ -1216,17 +1285,23 @@ struct SfSampler {
       if (tid == 0) { sh.fmax = bmax; sh.from = from; }
       cluster.sync();
       xmax = max_of([](const SfShared& o) { return o.fmax; });
-      if (xmax == INFINITY) return false;
+      zmax = quotient(xmax);
+      if (xmax == INFINITY || zmax == -INFINITY) return false;
       from = -max_of([](const SfShared& o) { return -o.from; });
+      // 104 below the largest z a weight is below 2^-149, and no noise (of -3.2 to 23) makes up for that
+      if (low) from = fmaxf(-SF_MAX, xmax - 105.f * temperature);
+      from = class_from(from);
       each([&](float x, int col) {
         if (x >= from) append(sh, x, col);
       });
       const int n = collect();
       if (n == 0) return false;  // none at all, or too many
-      zmax = quotient(xmax);
-      if (n < top_k) return false;
+      if (n < top_k && !low) return false;
       release(false);
-      if (rank == 0) top_k_of_list(n, top_k, by_p, top_p, min_p > 0.f ? least_logit(min_p) : -INFINITY);
+      if (rank == 0) {
+        if (sizeof(T) == 4 || low) divide_list(n);
+        top_k_of_list(n, by_k ? min(top_k, n) : n, by_p, top_p, min_p > 0.f ? least_of(least_kept(min_p)) : -INFINITY);
+      }
       return true;
     }
     // ---- the mass relative to the block's maximum, then that of the row ----
@@ -1238,10 +1313,12 @@ struct SfSampler {
       xmax = max_of([](const SfShared& o) { return o.fmax; });
       if (xmax == -INFINITY || xmax == INFINITY) return false;
       zmax = quotient(xmax);
+      if (zmax == -INFINITY) return false;
       total = sum_of([&](const SfShared& o) { return o.fmax > -INFINITY ? o.sums[0] * (double)exp2f((o.fmax - xmax) * c) : 0.; });
     }
     const Pass q = pass();
-    const float floor = min_p > 0.f ? least_logit(min_p) : -INFINITY;
+    const float floor_z = min_p > 0.f ? least_kept(min_p) : -INFINITY, floor = min_p > 0.f ? least_of(floor_z) : -INFINITY;
+    const float list_floor = sizeof(T) == 4 ? floor_z : floor;
     const double goal = by_p ? fmax(0., (double)top_p * total) : 0.;
     float from = -SF_MAX;
     // ---- top-p ----
@@ -1249,14 +1326,14 @@ struct SfSampler {
       // lighter tokens than this together have less than what top-p leaves out; a little is added for the sums' rounding
       const double least = (1. - (double)top_p - 2e-5) * total / a.V;
       if (!(least > 0.)) return false;
-      from = fmaxf(-SF_MAX, xmax + (logf((float)least) - 1e-3f) * temperature);
+      from = class_from(fmaxf(-SF_MAX, xmax + (logf((float)least) - 1e-3f) * temperature));
     }
     if (by_p && goal < SF_LIST / 16) {
       // twice a block's part of the list says that there are too many, without a look at the rest
       const unsigned most = (unsigned)min(SF_LIST, 2 * SF_LIST / C);
       each_until(
           [&](float x, int col) {
-            if (x >= from) append(sh, x, col);
+            if (x >= from) append(sh, listed(x), col);
           },
           [&] { return *reinterpret_cast<volatile unsigned*>(&sh.list_n) > most; });
       __syncthreads();
@@ -1265,12 +1342,13 @@ struct SfSampler {
       if (n > 0) {
         release(false);
         if (rank == 0) {
+          if (sizeof(T) == 4) to_z();
           const int m = n > SF_FEW ? thin_out(n, goal, total) : n;
           if (m <= SF_THREADS) {
-            finish_few(m, 0, 0., goal, floor);
+            finish_few(m, 0, 0., goal, list_floor);
           } else {
             list_border(m, true, goal, 0, 0.);
-            finish_list(m, sh.border, sh.border_col, floor);
+            finish_list(m, sh.border, sh.border_col, list_floor);
           }
         }
         return true;
@@ -1294,7 +1372,10 @@ struct SfSampler {
       draw(each_vector, q, floor_mass, floor);
       cluster.sync();
       release(true);
-      if (rank == 0) finish_blocks(0, fmaxf(floor, -SF_MAX), 0x7fffffff, floor_mass);
+      if (rank == 0) {
+        if (sizeof(T) == 4) to_z();
+        finish_blocks(0, fmaxf(list_floor, -SF_MAX), 0x7fffffff, floor_mass);
+      }
       return true;
     }
     set_step(from);
@@ -1322,29 +1403,29 @@ struct SfSampler {
     if (lead->upto - above > SF_LIST) return false;
     // above the bracket: the mass, and the draw (at least `goal` is kept); the bracket: listed
     {
-      Draw d = {(float)(20.0855369 * 1.001 / goal), temperature, word, greedy, as_sampler, 0.f, -INFINITY, 0.f, -1};
-      // linear_bin() < b0 and <= b1 without its conversion
-      const float end0 = (float)b0, end1 = b1 == SF_BINS - 1 ? INFINITY : (float)(b1 + 1);
+      Draw d = {(float)(20.0855369 * 1.001 / goal), temperature, word, as_sampler, 0.f, -INFINITY, 0.f, -1};
+      // From `sure` on a logit is in a bin above the bracket, below `last` in one behind it: the bins' ends, moved by more than the
+      // rounding of linear_bin() (2^-22 of the distance), then to where a z begins.  So the list holds the bracket and the few
+      // logits beside it; what is kept for sure has less mass than the goal, all of it with the list's more.
+      const double bin = 1. / (double)h.step;
+      const float sure = b0 > 0 ? class_above(__double2float_ru((double)h.xmax - b0 * bin * (1. - 1e-6))) : INFINITY;
+      const float last = b1 < SF_BINS - 1 ? fmaxf(from, class_from(__double2float_rd((double)h.xmax - (b1 + 1) * bin * (1. + 1e-6)))) : from;
       each_vector([&](auto& x, int col) {
         constexpr int M = sizeof(x) / sizeof(float);
         unsigned keep = 0, list = 0;
 #pragma unroll
         for (int k = 0; k < M; ++k) {
-          const float y = (h.xmax - x[k]) * h.step;
-          if (x[k] >= from) {
-            keep |= (y < end0 ? 1u : 0u) << k;
-            list |= (y < end1 ? 1u : 0u) << k;
-          }
+          keep |= (x[k] >= sure ? 1u : 0u) << k;
+          list |= (x[k] >= last ? 1u : 0u) << k;
         }
         list &= ~keep;
         if (list) {
 #pragma unroll
           for (int k = 0; k < M; ++k)
-            if (list >> k & 1) append(sh, x[k], col + k);
+            if (list >> k & 1) append(sh, listed(x[k]), col + k);
         }
         if (keep) consider_vector(h, d, x, col, keep);
       });
-      if (greedy && d.at >= 0) d.top_z = quotient(d.top_z);
       const double sum = sf_block_sum((double)d.part, sh);
       sf_block_best(d.top, d.at, d.top_z, sh);
       if (tid == 0) {
@@ -1355,9 +1436,11 @@ struct SfSampler {
       }
     }
     const int n = collect();
+    if (n == 0) return false;  // too many equals at the bracket's ends
     const double mass = sum_of([](const SfShared& o) { return o.sums[1]; });
     release(true);
     if (rank == 0) {
+      if (sizeof(T) == 4) to_z();
       list_border(n, true, goal, above, mass);
       finish_blocks(n, sh.border, sh.border_col, sh.kept);
     }
@@ -1388,21 +1471,12 @@ struct SfSampler {
   struct Draw {
     float reach, t;
     uint32_t word;
-    bool most, as;
+    bool as;
     float part, top, top_z;
     int at;
   };
   template <int M>
   static __device__ __forceinline__ void consider_vector(const Pass& q, Draw& d, const float (&x)[M], int col, unsigned keep) {
-    if (d.most) {  // a thread's columns ascend: the first of equals stays
-#pragma unroll
-      for (int k = 0; k < M; ++k) {
-        const bool in = keep >> k & 1;
-        d.part += in ? q.weight(x[k]) : 0.f;
-        if (in && (d.at < 0 || x[k] > d.top)) { d.top = d.top_z = x[k]; d.at = col + k; }
-      }
-      return;
-    }
     const float margin = d.as ? 1.f + 2e-6f : 1.f + 3e-7f;
     unsigned maybe = 0;
 #pragma unroll
@@ -1423,7 +1497,7 @@ struct SfSampler {
   template <typename E>
   __device__ __forceinline__ void draw(E each_vector, const Pass& q, double mass, float floor) {
     const float from = fmaxf(floor, -SF_MAX);
-    Draw d = {(float)(20.0855369 * 1.001 / mass), temperature, word, greedy, as_sampler, 0.f, -INFINITY, 0.f, -1};
+    Draw d = {(float)(20.0855369 * 1.001 / mass), temperature, word, as_sampler, 0.f, -INFINITY, 0.f, -1};
     each_vector([&](auto& x, int col) {
       constexpr int M = sizeof(x) / sizeof(float);
       unsigned keep = 0;
@@ -1431,18 +1505,26 @@ struct SfSampler {
       for (int k = 0; k < M; ++k) keep |= (x[k] >= from ? 1u : 0u) << k;
       if (keep) consider_vector(q, d, x, col, keep);
     });
-    if (greedy && d.at >= 0) d.top_z = quotient(d.top_z);
     sf_block_best(d.top, d.at, d.top_z, s);
     if (tid == 0) { s.best = d.top; s.best_col = d.at; s.best_z = d.top_z; }
   }
-  // The smallest logit that min-p keeps.
-  __device__ __noinline__ float least_logit(float min_p) const {
-    const double least = (double)zmax + log((double)min_p);
-    float floor = fminf(xmax, (float)(least * (double)temperature));
-    // the quotients, rounded, decide: at most a few logits around the product are on its wrong side
-    for (int i = 0; i < 8 && (double)quotient(nextafterf(floor, -INFINITY)) >= least; ++i) floor = nextafterf(floor, -INFINITY);
-    for (int i = 0; i < 8 && (double)quotient(floor) < least && floor < xmax; ++i) floor = nextafterf(floor, INFINITY);
-    return fminf(floor, xmax);
+  // The smallest z that min-p keeps: at most the largest of the row.
+  __device__ __noinline__ float least_kept(float min_p) const {
+    const double least = (double)zmax + log(fmin((double)min_p, 1.));
+    float z = (float)least;
+    if ((double)z < least) z = nextafterf(z, INFINITY);
+    return fmaxf(z, -SF_MAX);
+  }
+  // What stands in the list of top-p for a logit: z where the order is not that of the logits.
+  __device__ __forceinline__ float listed(float x) const { return sizeof(T) == 4 ? sf_quotient(x, temperature) : x; }
+  // The first block: divides the list's entries, from which on what is compared is z.
+  __device__ __noinline__ void divide_list(int n) {
+    for (int i = tid; i < n; i += SF_THREADS) {
+      const unsigned long long e = s.list[i];
+      s.list[i] = (unsigned long long)(~sf_key(quotient(sf_entry_x(e)) + 0.f)) << 32 | (unsigned)e;
+    }
+    __syncthreads();
+    to_z();
   }
   // The first block: top-k (0: none), then top-p of `goal`, or of the share top_p of what top-k kept, then the floor and the draw, in
   // a list of n <= SF_THREADS tokens that holds all that is kept.
@@ -1523,9 +1605,12 @@ struct SfSampler {
     const int top_k = a.top_k ? a.top_k[row] : a.top_k_all;
     const bool by_k = top_k > 0 && top_k < a.V, by_p = top_p < 1.f;
     cluster.sync();  // what fast() has left may still be read
+    if (divided) to_z();
     // ---- the maximum, and the mass relative to each thread's own ----
-    float mine = -INFINITY, part = 0.f;
-    {
+    float mine, part;
+    for (;;) {
+      mine = -INFINITY;
+      part = 0.f;
       const SfRow<T> q = r;
       const float k = c;
       q.each([&](float x, int) {
@@ -1535,26 +1620,30 @@ struct SfSampler {
         }
         if (x >= -SF_MAX) part += exp2f((x - mine) * k);
       });
+      float mx = warp_max(mine);
+      if ((tid & 31) == 0) s.red[0][tid >> 5] = mx;
+      __syncthreads();
+      mx = (float)s.red[0][0];
+      for (int w = 1; w < SF_WARPS; ++w) mx = fmaxf(mx, (float)s.red[0][w]);
+      const double sum = sf_block_sum(mine == -INFINITY ? 0. : (double)(part * exp2f((mine - mx) * c)), s);
+      if (tid == 0) {
+        s.fmax = mx;
+        s.first_mass = sum;
+      }
+      cluster.sync();
+      xmax = max_of([](const SfShared& o) { return o.fmax; });
+      if (divided || !(xmax > r.cap)) break;
+      read_divided(true);  // 16-bit logits of which some have no finite quotient: once more, as z
+      to_z();
+      cluster.sync();
     }
-    float mx = warp_max(mine);
-    if ((tid & 31) == 0) s.red[0][tid >> 5] = mx;
-    __syncthreads();
-    mx = (float)s.red[0][0];
-    for (int w = 1; w < SF_WARPS; ++w) mx = fmaxf(mx, (float)s.red[0][w]);
-    const double sum = sf_block_sum(mine == -INFINITY ? 0. : (double)(part * exp2f((mine - mx) * c)), s);
-    if (tid == 0) {
-      s.fmax = mx;
-      s.first_mass = sum;
-    }
-    cluster.sync();
-    xmax = max_of([](const SfShared& o) { return o.fmax; });
-    if (xmax == -INFINITY) {  // nothing to draw from
+    zmax = quotient(xmax);
+    if (zmax == -INFINITY) {  // nothing to draw from
       if (rank == 0 && tid == 0) { a.tok[row] = 0; a.logp[row] = -INFINITY; }
       return;
     }
-    zmax = quotient(xmax);
     const double total = sum_of([&](const SfShared& o) { return o.fmax > -INFINITY ? o.first_mass * (double)exp2f((o.fmax - xmax) * c) : 0.; });
-    const float floor = min_p > 0.f ? least_logit(min_p) : -INFINITY;
+    const float floor = min_p > 0.f ? least_of(least_kept(min_p)) : -INFINITY;
     float border = -INFINITY;
     int border_col = 0x7fffffff;
     double kept = 0.;
@@ -1667,9 +1756,10 @@ sample_filtered_kernel(const __grid_constant__ SampleArgs a, int vecs) {
   f.r.v1 = rank == C - 1 ? a.V : min(a.V / N * N, (rank + 1) * per);
   f.r.vec = (reinterpret_cast<uintptr_t>(f.r.x) & 15) == 0;
   const float temp = a.temperature ? a.temperature[row] : a.temperature_all;
-  f.temperature = fminf(fmaxf(temp, 1e-6f), 1e37f);
+  f.temperature = temp < 1e-6f ? 1e-6f : temp;
   f.c = SF_LOG2E / f.temperature;
   f.r.cap = SF_MAX * fminf(f.temperature, 1.f);
+  f.read_divided(sizeof(T) == 4 || !(f.temperature >= SF_LOW && f.temperature <= SF_HIGH));
   f.greedy = !(temp > 0.f);
   f.as_sampler = a.words == nullptr;
   f.word = a.words ? a.words[row] : a.seed ^ sf_hash((a.step_ptr ? (uint32_t)*a.step_ptr : 0u) * 0x9E3779B9U + (uint32_t)row);
