@@ -198,3 +198,10 @@ def test_sampling_of_infinite_logits(dtype, rows):
     for kw in ({}, {"top_k": 3}, {"top_p": 0.9}, {"top_k": 600, "top_p": 0.7}, {"temperature": 0.0}, {"min_p": 0.2, "temperature": 0.5}, {"temperature": 3.0}):
         tok, logp = F.sample_filtered(z.cuda(), rng.cuda(), **kw)
         check_sample(z, rng, tok, logp, **kw)
+
+
+def test_sampling_takes_numbers_of_tokens_beyond_32_bits():
+    z, rng = torch.randn(4, 100, generator=torch.Generator().manual_seed(0)), torch.arange(4, dtype=torch.int32)
+    k = torch.tensor([2**32 + 1, 2**31 + 1, -2**32 + 1, 3], dtype=torch.int64)
+    tok, logp = F.sample_filtered(z.cuda(), rng.cuda(), top_k=k.cuda())
+    check_sample(z, rng, tok, logp, top_k=k)
