@@ -205,3 +205,7 @@ def test_sampling_takes_numbers_of_tokens_beyond_32_bits():
     k = torch.tensor([2**32 + 1, 2**31 + 1, -2**32 + 1, 3], dtype=torch.int64)
     tok, logp = F.sample_filtered(z.cuda(), rng.cuda(), top_k=k.cuda())
     check_sample(z, rng, tok, logp, top_k=k)
+    for dtype in (torch.uint8, torch.int16, torch.int32, torch.int64):
+        few = torch.tensor([1, 0, 50, 3], dtype=dtype)
+        tok, logp = F.sample_filtered(z.cuda(), rng.cuda(), top_k=few.cuda())
+        check_sample(z, rng, tok, logp, top_k=few)

@@ -1351,7 +1351,7 @@ def sample_filtered(logits, rng=None, *, temperature=1.0, top_k=0, top_p=1.0, mi
             raise ValueError(f"rng has to be an int32 or int64 tensor [{B}]: the low 32 bits of each are used")
         if rng.dtype != torch.int32 or not rng.is_contiguous():
             rng = rng.to(torch.int32).contiguous()
-    if isinstance(top_k, torch.Tensor) and top_k.dtype != torch.int32:
+    if isinstance(top_k, torch.Tensor) and top_k.dtype == torch.int64:
         top_k = top_k.clamp(-1, 2**31 - 1)  # as int32, a number beyond it would be another one
     (t, t0), (k, k0) = _per_row(temperature, "temperature", B, torch.float32, index), _per_row(top_k, "top_k", B, torch.int32, index)
     (p, p0), (m, m0) = _per_row(top_p, "top_p", B, torch.float32, index), _per_row(min_p, "min_p", B, torch.float32, index)
