@@ -110,7 +110,90 @@ def test_attention_keeps_many_small_weights_beside_a_large_one(B, n, drop):
     assert (want > 8 * tol).all()  # what is lost would be seen
 
 
+@pytest.mark.parametrize("Hq, Hk, page", [(9, 1, 16), (24, 2, 64), (40, 2, 128)])
+def test_attention_of_wide_heads_in_several_tiles(Hq, Hk, page):
+    """Head dim 256 with more than eight query heads a key head: their pages are read by several tiles."""
+    lens = [1, 700, 64, 2100, 0, 33]
+    cache, table = filled_cache(lens, Hk, page, 256, "cuda", seed=Hq)
+    q = torch.randn(len(lens), Hq, 256, generator=torch.Generator().manual_seed(2)).bfloat16().cuda()
+    for window in (None, 50):
+        out = F.kv8_decode_attn(q, *cache, table, _i32([n - 1 for n in lens]), 0.002, window=window)
+        want, tol = attention64(q.cpu(), _cpu(cache), table.cpu(), lens, 0.002, window)
+        assert ((out.cpu().double() - want).abs() <= tol).all() and (out[4] == 0).all()
+
+
+def test_a_sequence_alone_has_the_output_that_it_has_in_a_batch():
+    """Within the bound of each: the work is dealt otherwise, so the bits may differ."""
+    lens = [50, 0, 333, 64]
+    cache, table = filled_cache(lens, 2, 16, 64, "cuda")
+    big = torch.randn(3, 9, 64, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    q, slots, seq = big[:, 2:8], [2, 0, 2], _i32([n - 1 for n in lens])
+    want, tol = attention64(q.cpu(), _cpu(cache), table.cpu()[slots], [lens[s] for s in slots], 0.01)
+    for i, slot in enumerate(slots):
+        out = F.kv8_decode_attn(q[i:i + 1], *cache, table, seq, 0.01, slots=_i32([slot]))
+        assert ((out.cpu().double() - want[i:i + 1]).abs() <= tol[i:i + 1]).all()
+
+
 # ---- RoPE and append -----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("D, page, Hq, Hk", [(128, 64, 4, 2), (64, 16, 3, 1), (64, 128, 2, 2), (96, 32, 5, 1)])
+def test_rope_append_brings_earlier_rows_to_a_grown_scale(D, page, Hq, Hk, f32):
+    """Codes and scales are those of the definition's append of the rotated row: earlier rows of the page at the new scale, later
+    ones and other pages as they were.  The first query heads have the keys' values, so they show the keys as they were rotated
+    and rounded; those are held to 64 bits.  Far positions, with and without a shift of them."""
+    from trl_b200.ops import cuda as K
+    from trl_b200.oracle import ops as R
+
+    g = torch.Generator().manual_seed(D + page)
+    B, blocks, half, theta = 6, 70, D // 2, 1e4
+    lens = [(blocks - 3) * page + page // 2, 5, 0, 40 * page + 1, -1, 17 * page + page - 1]
+    cache, table = filled_cache([max(1, n + 1) for n in lens], Hk, page, D, "cuda", seed=page)
+    for c, s in zip(cache[:2], cache[2:]):
+        c.view(torch.uint8)[(c.view(torch.uint8) & 0x7F) == 0x7F] = 0x55
+        s.copy_(torch.ldexp(torch.ones(s.shape), torch.randint(-9, 0, s.shape, generator=g)))
+    for delta in (None, torch.tensor([3, 900, 0, -2, 7, 11], dtype=torch.int32)):
+        # sizes from 2^-6 to 2^9: scales of 2^-9 .. 2^-1, for magnitudes up to 224, grow in some pages and stay in others
+        x = torch.randn(B, Hq + 2 * Hk, D, generator=g) * 2.0 ** torch.randint(-6, 10, (B, 1, 1), generator=g)
+        x[:, :Hk] = x[:, Hq:Hq + Hk]
+        x = x.bfloat16()
+        got, was = [t.clone() for t in cache], _cpu(cache)
+        q = torch.full((B, Hq, D), 9.0, dtype=torch.bfloat16, device="cuda")
+        src = x.view(B, -1).cuda()
+        K.kv8_rope_append(src.float() if f32 else src, None, None, None, 1e-6, _i32(lens), None, table, q, *got, Hq, theta,
+                          pos_delta=None if delta is None else delta.cuda())
+        K.check_status()
+        got, q = _cpu(got), q.cpu()
+        # an angle is off by what its exponent of up to 13.3 is in 32 bits (three roundings of 2^-24 of it) and 2^-22: below 2^-18.5
+        pos = torch.tensor(lens).double() + (0 if delta is None else delta.double())
+        ang = pos[:, None, None] * theta ** (-torch.arange(half).double() * 2 / D)
+        y = x[:, :Hq].double()
+        lo, hi, size = y[..., :half], y[..., half:], (y[..., :half].square() + y[..., half:].square()).sqrt().repeat(1, 1, 2)
+        want = torch.cat([lo * ang.cos() - hi * ang.sin(), hi * ang.cos() + lo * ang.sin()], -1)
+        tol = torch.finfo(q.dtype).eps / 2 * want.abs() + size * (ang.abs().repeat(1, 1, 2) * 2.0**-18.5 + 2.0**-20)
+        live = torch.tensor(lens) >= 0
+        assert ((q.double() - want).abs() <= tol)[live].all() and (q[~live] == 9).all()
+        grown = 0
+        for i, n in enumerate(lens):
+            if n < 0:
+                continue
+            page_id, row = int(table[i, n // page]), n % page
+            for which, new in ((0, q[i, :Hk].float()), (1, x[i, Hq + Hk:].float())):
+                codes, scale, c0, s0 = got[which][page_id], got[2 + which][page_id], was[which][page_id], was[2 + which][page_id]
+                need = R.kv8_scale(new.abs().amax(-1))
+                now = torch.maximum(s0, need) if row else need
+                assert torch.equal(scale, now)
+                again = (c0[:, :row].float() * (s0 / now)[:, None, None]).to(c0.dtype)
+                assert torch.equal(codes[:, :row].view(torch.uint8), again.view(torch.uint8))
+                assert torch.equal(codes[:, row].view(torch.uint8), (new / now[:, None]).to(c0.dtype).view(torch.uint8))
+                assert torch.equal(codes[:, row + 1:].view(torch.uint8), c0[:, row + 1:].view(torch.uint8))
+                grown += int(row > 0 and bool((now > s0).any()))
+        assert grown > 0
+        rest = sorted(set(range(cache[0].shape[0])) - {int(table[i, n // page]) for i, n in enumerate(lens) if n >= 0})
+        for a, b in zip(got, was):
+            a, b = (t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t for t in (a, b))
+            assert torch.equal(a[rest], b[rest])
+
+
 @pytest.mark.parametrize("f32", [False, True])
 def test_rope_append_reports_slots_that_the_table_does_not_have(f32):
     """They are treated as idle: their sums are cleared, nothing is written for them, the other rows are as ever."""
