@@ -32,3 +32,13 @@ def test_attention_refuses_more_steps_than_it_can_count():
     with pytest.raises(ValueError, match="2\\^31 steps"):
         K.kv8_decode_attn(torch.zeros(B, 1, 64, dtype=torch.bfloat16), *F.kv8_alloc(2, 1, 128, 64), table,
                           torch.full((B,), -1, dtype=torch.int32), 1.0)
+
+
+@pytest.mark.parametrize("kv8", [False, True])
+def test_only_prompts_into_an_8_bit_cache_need_starts(kv8):
+    from types import SimpleNamespace
+
+    from trl_b200.rollout.engine import _PrefillKV
+
+    hook = _PrefillKV(SimpleNamespace(kv8=kv8), None, None, torch.tensor([2, 0], dtype=torch.int32))
+    assert (hook.starts.tolist() == [0, 0]) if kv8 else hook.starts is None

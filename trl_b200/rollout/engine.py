@@ -104,7 +104,7 @@ class _PrefillKV:
 
     def __init__(self, engine: "RolloutEngine", tok_slot, tok_pos, slots=None):
         self.e, self.tok_slot, self.tok_pos = engine, tok_slot, tok_pos
-        self.slots, self.starts = slots, None if slots is None else torch.zeros_like(slots)
+        self.slots, self.starts = slots, torch.zeros_like(slots) if engine.kv8 else None
 
     def attend(self, layer_idx, q, k, v, ctx):
         from ..ops import cuda as K
