@@ -3,8 +3,8 @@
 //   o = sum_j softmax_j(scale q . k_j) v_j,   k_j = code * k_scale[page, head],  v_j = code * v_scale[page, head]
 //
 // Bound by the cache's bytes: 2 D bytes a token and key head for 4 G D operations (G query heads share a key head).  Measured, with
-// 32 query and 8 key heads of 128: 131067 tokens of one sequence 54.5 us (268 MB: 5.3 TB/s in the main kernel), 128 sequences of up to
-// 8192 tokens 49.9 us; 64 sequences of 1024 tokens with 28 and 4 heads 22.5 us, of which 4 us pass before the first codes are
+// 32 query and 8 key heads of 128: 131067 tokens of one sequence 54.1 us (268 MB: 5.3 TB/s in the main kernel), 128 sequences of up to
+// 8192 tokens 50.7 us; 64 sequences of 1024 tokens with 28 and 4 heads 22.4 us, of which 4 us pass before the first codes are
 // there and 4 us in the join.
 //
 // A warp takes 16 tokens a step.  Each warp has a queue of steps in shared memory that its first lane keeps filled by TMA, a few
@@ -31,7 +31,7 @@
 //
 // Where there are no more rows than SMs and the block table has room for few steps a warp only (kv8_attn_alone), each row gets a
 // block of its own instead (by_row): no list of all rows, no parts, no second kernel.  One sequence of 211 tokens with 14 and 2
-// heads of 64 takes 6.3 us so, 10.2 us from the list.
+// heads of 64 takes 6.4 us so, 10.2 us from the list.
 #include <cuda_fp16.h>
 
 #include "kv8.cuh"

@@ -24,9 +24,11 @@
 // A row that fits into the shared memory of a cluster is read once and stays there for all of it, larger ones are read again for
 // each pass (SfSampler::fast); the few rows that need what fast() leaves out are read again and, where their order is not that of
 // z, divided in each pass (SfSampler::run).
-// Measured: one row of 152064 bf16 logits with top-k 20 and top-p 0.8 13.3 us; 64 rows with top-p 0.95 71 us (32 rows 48 us), of which the
-// flattest row's 61 us are: load and mass 8, list given up 4, histogram 8, its border's bins 8, draw 20, list of the bracket 5,
-// border 5, last draw 3; 256 rows of 128256 fp32 logits with parameters of all kinds 114 us.
+// Measured: one row of 152064 bf16 logits with top-k 20 and top-p 0.8 13.8 us; 64 rows with top-p 0.95 64 us (32 rows 48 us), of which the
+// flattest row's 60 us are: load and mass 8, list given up 3, histogram 9, its border's bins 8, draw 19, list of the bracket 4,
+// border 5, last draw 3; 256 rows of 128256 fp32 logits with parameters of all kinds 114 us.  run(), which top-k above 512 (256 for
+// each block of the cluster) needs: 64 rows of 152064 bf16 logits 48 us at top-k 600, 51 at 1000, 107 at 2000, with top-k 500 29 us; fp32
+// logits at temperature 0.7, which it divides in each pass, 53, 55 and 105 us, at temperature 1 44, 46 and 89.
 // Counts and the sums over lists are integers, other sums are taken in a fixed order: results do not depend on timing.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
@@ -1823,9 +1825,9 @@ template <typename T>
 int sample_filtered_pick(const SampleArgs& a, int B, cudaStream_t st) {
   // Blocks a row, up to the 8 of a portable cluster: enough to hold it in their shared memory, and as many more as all rows find a
   // place for at once.  More rows than that are not held: they get as many blocks as find a place, and at least two, so that a long
-  // row (top-p of a flat one takes five times as long as top-k) has two SMs.  Measured with 256 rows of 128256 fp32 logits, all of
-  // one kind: held 311 us, two blocks 194, one block 194; of all kinds: 170, 116, 160.  64 rows of 152064 bf16 logits: held 67 us,
-  // not held 72; 32 of them with 8 blocks each 48, with 5 56; 72 of them, held in two waves, 93.
+  // row (top-p of a flat one takes five times as long as top-k) has two SMs.  Measured with 256 rows of 128256 fp32 logits, flat and
+  // with top-p 0.95: held 315 us, two blocks 181, one block 165; with parameters of all kinds: 181, 114, 146.  64 rows of 152064 bf16
+  // logits: held 64 us, not held 66; 32 of them with 8 blocks each 48, with 5 55; 72 of them: held in two waves 71, not held 77.
   constexpr long long N = 16 / sizeof(T);
   int device = 0, C = 1;
   const cudaError_t e = cudaGetDevice(&device);

@@ -201,7 +201,9 @@ def kv8_decode_attn(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens
 
     Sequence i sees the positions up to ``seq_lens[slot]`` (its newest token, which has been appended) in row ``slots[i]``
     (default: i) of ``block_table``, with ``window`` only the last so many of them; ``seq_lens`` below 0: none, and zeros come
-    back.  Query heads share key heads in equal groups.  ``out``: a dense tensor like ``q`` to write to."""
+    back.  Query heads share key heads in equal groups.  ``out``: a dense tensor like ``q`` to write to.  A call has at most 4096
+    sequences and less than 2^31 steps of 16 tokens in all that the block table has room for.  Queries, keys or values that are
+    not finite come out as NaN where they are in sight."""
     args = (q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, scale)
     if q.is_cuda:
         return _cuda().kv8_decode_attn(*args, slots=slots, window=window, out=out)
@@ -217,7 +219,7 @@ def sample_filtered(logits, rng, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0)
     number is hashed: a row's draw depends on its word and its logits alone.  ``temperature``, ``top_k``, ``top_p`` and
     ``min_p`` are numbers or tensors [B].
 
-    With z = logits / temperature: top-k keeps what is at least the k-th largest z (0: all); top-p keeps, most likely first
+    With z = logits / temperature in fp32 (+inf and what is beyond fp32 count as its largest number): top-k keeps what is at least the k-th largest z (0: all); top-p keeps, most likely first
     and the lower token first among equals, each token before which at most ``top_p`` of the mass left by top-k stands (1:
     all); min-p keeps what has at least ``min_p`` (up to 1) of the largest probability.  Temperature 0 takes the most likely
     token, the lowest among equals.  The log-probability is that in the distribution over what is kept.  NaN counts as -inf;
